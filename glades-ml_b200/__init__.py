@@ -10,4 +10,6 @@ from .capi import (  # noqa: F401
     GL_MAX_WEIGHT_LAYERS, ACT, OUT, MODE_REFERENCE, MODE_BATCHED, BIAS_MEAN, BIAS_REFERENCE,
     GEMM_AUTO, GEMM_FFMA, GEMM_TCGEN05, GEMM_GRID_FUSED, NetDesc, Metrics, GladesError, Net, lib, lib_path,
     make_desc, weight_count, shard_range, device_count, tc_variant_counts, tc_engine_counts, ffma_route,
+    F32, BF16, F16, OrthoItem, MuonItem, layer_norm, layer_norm_backward_workspace, layer_norm_backward, ortho_items, muon_items,
+    orthogonalize_workspace, orthogonalize, muon_workspace, muon_step, orthogonalize_status,
 )

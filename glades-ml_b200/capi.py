@@ -13,6 +13,7 @@ OUT = {"regression": 0, "classification": 1, "kl": 2}
 MODE_REFERENCE, MODE_BATCHED = 0, 1
 BIAS_MEAN, BIAS_REFERENCE = 0, 1
 GEMM_AUTO, GEMM_FFMA, GEMM_TCGEN05, GEMM_GRID_FUSED = 0, 1, 2, 3
+F32, BF16, F16 = 0, 1, 2  # element types of the operators on device buffers
 
 
 class NetDesc(C.Structure):
@@ -33,6 +34,17 @@ class NetDesc(C.Structure):
         ("gemm", C.c_int32),
         ("device", C.c_int32),
     ]
+
+
+class OrthoItem(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("d_in", C.c_void_p), ("ld_in", C.c_int64), ("d_out", C.c_void_p),
+                ("ld_out", C.c_int64)]
+
+
+class MuonItem(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("lr", C.c_float), ("d_grad", C.c_void_p), ("ld_grad", C.c_int64),
+                ("d_momentum", C.c_void_p), ("d_momentum_out", C.c_void_p), ("ld_momentum", C.c_int64), ("d_weight", C.c_void_p),
+                ("d_weight_out", C.c_void_p), ("ld_weight", C.c_int64)]
 
 
 class Metrics(C.Structure):
@@ -171,6 +183,14 @@ def lib():
         "gl_matmul_static": (C.c_int, [vp, i64, i64, vp, i64, i64, vp, i64, i32, i32, i32, i32]),
         "gl_matmul_static_error": (C.c_char_p, []),
         "gl_standardize_table": (C.c_int, [vp, i64, i32, vp, vp, vp, i32, vp, C.POINTER(i32), vp, C.POINTER(i32), vp, i32]),
+        "gl_layer_norm": (C.c_int, [vp, i64, vp, vp, vp, i64, vp, vp, i64, i32, f32, i32, vp, i32]),
+        "gl_layer_norm_backward_workspace": (i64, [i64, i32]),
+        "gl_layer_norm_backward": (C.c_int, [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, i32, i32, vp, i64, vp, i32]),
+        "gl_orthogonalize_workspace": (i64, [C.POINTER(OrthoItem), i32]),
+        "gl_orthogonalize": (C.c_int, [C.POINTER(OrthoItem), i32, _f32p, i32, f32, i32, vp, i64, vp, i32]),
+        "gl_muon_workspace": (i64, [C.POINTER(MuonItem), i32]),
+        "gl_muon_step": (C.c_int, [C.POINTER(MuonItem), i32, f32, i32, f32, _f32p, i32, f32, i32, vp, i64, vp, i32]),
+        "gl_orthogonalize_status": (C.c_int, [vp, vp, i32]),
         "gl_onehot_fill": (C.c_int, [vp, vp, i64, i32, f32, f32, i32]),
         "gl_timer_start": (C.c_int, [vp]),
         "gl_timer_stop": (C.c_int, [vp, C.POINTER(C.c_double)]),
@@ -230,6 +250,74 @@ def shard_range(rows, rank, world):
     f, c = C.c_int64(), C.c_int64()
     lib().gl_shard_range(rows, rank, world, C.byref(f), C.byref(c))
     return f.value, c.value
+
+
+# ---- operators on device buffers: pointers and streams are integers (a tensor's data_ptr(), a stream's cuda_stream) ----
+def layer_norm(d_x, ldx, d_gain, d_shift, d_y, ldy, d_mean, d_rstd, rows, n, eps=1e-5, dtype=F32, stream=0, device=0):
+    _check(lib().gl_layer_norm(d_x, ldx, d_gain, d_shift, d_y, ldy, d_mean, d_rstd, rows, n, eps, dtype, stream, device))
+
+
+def layer_norm_backward_workspace(rows, n):
+    return _size(lib().gl_layer_norm_backward_workspace(rows, n))
+
+
+def layer_norm_backward(d_dy, lddy, d_x, ldx, d_gain, d_mean, d_rstd, d_dx, lddx, d_dgain, d_dshift, rows, n, d_work, work_bytes,
+                        dtype=F32, stream=0, device=0):
+    _check(lib().gl_layer_norm_backward(d_dy, lddy, d_x, ldx, d_gain, d_mean, d_rstd, d_dx, lddx, d_dgain, d_dshift, rows, n, dtype,
+                                        d_work, work_bytes, stream, device))
+
+
+def _items(kind, rows):
+    return (kind * len(rows))(*[kind(**r) for r in rows])
+
+
+def ortho_items(rows):
+    """gl_ortho_item array from dicts of its fields."""
+    return _items(OrthoItem, rows)
+
+
+def muon_items(rows):
+    """gl_muon_item array from dicts of its fields."""
+    return _items(MuonItem, rows)
+
+
+def _coefficients(coefficients, steps):
+    if coefficients is None:
+        return None
+    flat = [float(v) for c in coefficients for v in c]
+    if len(flat) != 3 * steps:
+        raise ValueError("coefficients: %d steps of three numbers each" % steps)
+    return (C.c_float * len(flat))(*flat)
+
+
+def orthogonalize_workspace(items):
+    return _size(lib().gl_orthogonalize_workspace(items, len(items)))
+
+
+def orthogonalize(items, d_work, work_bytes, coefficients=None, steps=5, eps=1e-7, dtype=F32, stream=0, device=0):
+    _check(lib().gl_orthogonalize(items, len(items), _coefficients(coefficients, steps), steps, eps, dtype, d_work, work_bytes, stream,
+                                  device))
+
+
+def muon_workspace(items):
+    return _size(lib().gl_muon_workspace(items, len(items)))
+
+
+def muon_step(items, d_work, work_bytes, momentum=0.95, nesterov=True, weight_decay=0.0, coefficients=None, steps=5, eps=1e-7,
+              dtype=F32, stream=0, device=0):
+    _check(lib().gl_muon_step(items, len(items), momentum, 1 if nesterov else 0, weight_decay, _coefficients(coefficients, steps), steps,
+                              eps, dtype, d_work, work_bytes, stream, device))
+
+
+def orthogonalize_status(d_work, stream=0, device=0):
+    """Waits for the stream; raises GladesError where a bounded wait of the last call on this workspace ran out."""
+    _check(lib().gl_orthogonalize_status(d_work, stream, device))
+
+
+def _size(n):
+    if n < 0:
+        _check(int(n))
+    return int(n)
 
 
 def _ptr(a):

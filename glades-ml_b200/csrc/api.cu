@@ -38,6 +38,16 @@ static int fail(int code, const char* fmt, ...)
 	return code;
 }
 
+int glb::report_error(int code, const char* fmt, ...)
+{
+	char buf[512];
+	va_list ap;
+	va_start(ap, fmt);
+	vsnprintf(buf, sizeof buf, fmt, ap);
+	va_end(ap);
+	return fail(code, "%s", buf);
+}
+
 #define CU(call)                                                                                     \
 	do                                                                                               \
 	{                                                                                                \

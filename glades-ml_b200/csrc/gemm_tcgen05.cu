@@ -628,6 +628,32 @@ bool tc_make_rows_map(void* out128, const float* base, long long stages, long lo
 	          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool tc_make_parts_map(void* out128, const __half* base, long long rows, long long cols, long long ld, long long plane, int planes, int box_cols,
+                       int box_rows)
+{
+	EncodeTiledFn fn = encode_fn();
+	if (!fn) return false;
+	cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+	cuuint64_t str[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+	cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 2};
+	cuuint32_t es[3] = {1, 1, 1};
+	return fn(reinterpret_cast<CUtensorMap*>(out128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dim, str, box, es,
+	          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tc_make_parts_map_mn(void* out128, const __half* base, long long k, long long cols, long long ld, long long plane, int planes, int box_k,
+                          int box_cols)
+{
+	EncodeTiledFn fn = encode_fn();
+	if (!fn) return false;
+	cuuint64_t dim[4] = {64, (cuuint64_t)k, (cuuint64_t)((cols + 63) / 64), (cuuint64_t)planes};
+	cuuint64_t str[3] = {(cuuint64_t)ld * 2, 128, (cuuint64_t)plane * 2};
+	cuuint32_t box[4] = {64, (cuuint32_t)box_k, (cuuint32_t)(box_cols / 64), 2};
+	cuuint32_t es[4] = {1, 1, 1, 1};
+	return fn(reinterpret_cast<CUtensorMap*>(out128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dim, str, box, es,
+	          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tc_make_operand_map_f32(void* out128, const float* ptr, int mn, long long R, long long K, long long ld, int box_r)
 {
 	CUtensorMap* m = reinterpret_cast<CUtensorMap*>(out128);

@@ -323,6 +323,36 @@ size_t standardize_table_bytes(int width);
 cudaError_t launch_standardize(const StandardizeArgs& a, cudaStream_t s);
 float order_float_host(int i);
 
+// ---- layer norm (layer_norm.cu) --------------------------------------------------------------------
+struct LayerNormArgs
+{
+	const void* x;      // [rows][n], pitch ldx
+	long long ldx;
+	const void* dy;     // backward
+	long long lddy;
+	void* y;            // forward
+	long long ldy;
+	void* dx;           // backward, or NULL
+	long long lddx;
+	const float* gain;  // [n] or NULL: ones
+	const float* shift; // [n] or NULL: zeros
+	float* mean;        // [rows]; forward: written unless NULL, backward: read
+	float* rstd;
+	float2* part;       // backward: [layer_norm_partial_rows][n] scratch, or NULL: no dgain, no dshift
+	float* dgain;       // backward: [n] or NULL
+	float* dshift;
+	long long rows;
+	int n;
+	float eps;
+};
+size_t layer_norm_partial_rows(long long rows, int n);
+// rows >= 1; type: GL_F32, GL_BF16 or GL_F16
+cudaError_t launch_layer_norm(const LayerNormArgs& a, int type, cudaStream_t s);
+cudaError_t launch_layer_norm_backward(const LayerNormArgs& a, int type, cudaStream_t s);
+
+// ---- errors of entry points outside api.cu: the text that gl_last_error() returns; returns code
+int report_error(int code, const char* fmt, ...);
+
 // ---- synthetic inputs (synth.cu) ---------------------------------------------------------------
 // out[j] = element (first + j) of stream `stream_id`; `first` must be even for dist 1
 cudaError_t launch_synth_fill(float* out, long long n, long long first, unsigned long long seed, unsigned stream_id, int dist,

@@ -1,0 +1,42 @@
+// Orthogonalisation of matrices and the weight update built on it (orthogonalize.cu).
+#pragma once
+#include "internal.h"
+
+namespace glb {
+
+constexpr int ORTHO_MAX_MATRICES = GL_MAX_WEIGHT_LAYERS;  // of one launch
+constexpr int ORTHO_MAX_STEPS = 16;
+
+// One row-major matrix.  Orthogonalisation: out = O(grad).  Update step: mom_out = mu mom + grad,
+// w_out = (1 - lr decay) w - lr O(u) with u = grad + mu mom_out (nesterov) or mom_out.
+struct OrthoMatrix
+{
+	int rows, cols;
+	const void* grad;
+	long long ld_grad;
+	void* out;
+	long long ld_out;
+	const float* mom;
+	float* mom_out;
+	long long ld_mom;
+	const float* w;
+	float* w_out;
+	long long ld_w;
+	float lr;
+};
+struct OrthoArgs
+{
+	const OrthoMatrix* mat;
+	int count, steps, type, step, nesterov;
+	float mu, decay, eps;
+	float coef[ORTHO_MAX_STEPS][3];
+	int* status;  // device word that a wait that runs out raises, or NULL: the workspace's
+};
+// Bounds on the singular values of X before every step (steps + 1), and on the eigenvalues of A and P; false where the
+// coefficients let them leave the range that the fp16 parts are scaled for.
+bool ortho_bounds(const float (*coef)[3], int steps, double* sx, double* sa, double* sp);
+size_t ortho_workspace_bytes(const OrthoMatrix* m, int count);
+int* ortho_status(void* work);  // where a workspace keeps its status word
+cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, cudaStream_t s);
+
+}  // namespace glb

@@ -364,6 +364,69 @@ int gl_standardize_table(const float* d_raw, int64_t rows, int32_t cols, const i
                          const int32_t* to_output, int32_t flag, float* d_x, int32_t* nx, float* d_y, int32_t* ny,
                          float* stats_out, int32_t device);
 
+/* ---- operators on device buffers, queued in the caller's stream ---------------------------- */
+/* They queue their work on `stream` (a cudaStream_t of `device`; NULL: the legacy default stream) and return: no
+ * synchronisation, no allocation, the current device as it was; a call can be captured into a CUDA graph.  Scratch memory is
+ * the caller's: `d_work`, at least as many bytes as the operator's _workspace function says, any alignment, needs no
+ * initialisation, belongs to one call (or graph replay) until that has finished.  Element types: */
+enum { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
+
+/* Layer norm of the rows of x [rows][n]: mean and variance (divided by n) of each row, xh = (x - mean) / sqrt(variance +
+ * eps), y = gain * xh + shift.  x and y are of `type`, ldx and ldy (>= n) elements from row to row; gain and shift, fp32 [n],
+ * may each be NULL (ones, zeros).  d_mean and d_rstd, fp32 [rows], receive mean and 1 / sqrt(variance + eps) for the backward
+ * pass; each may be NULL.  All arithmetic is fp32, y is rounded once.  y may be x (with the same pitch).  rows may be 0. */
+int gl_layer_norm(const void* d_x, int64_t ldx, const float* d_gain, const float* d_shift, void* d_y, int64_t ldy, float* d_mean,
+                  float* d_rstd, int64_t rows, int32_t n, float eps, int32_t type, void* stream, int32_t device);
+/* The backward pass: from dy (`type`, pitch lddy), x and the forward pass's mean and rstd: dx (`type`, pitch lddx, may be NULL,
+ * may be dy or x with the same pitch) and the sums over the rows dgain = sum dy * xh, dshift = sum dy (fp32 [n], each may be NULL).
+ * The sums are taken in a fixed order: two calls give the same bits.  rows == 0 gives dgain = dshift = 0. */
+int64_t gl_layer_norm_backward_workspace(int64_t rows, int32_t n);
+int gl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const float* d_gain, const float* d_mean,
+                           const float* d_rstd, void* d_dx, int64_t lddx, float* d_dgain, float* d_dshift, int64_t rows, int32_t n,
+                           int32_t type, void* d_work, int64_t work_bytes, void* stream, int32_t device);
+
+/* Orthogonalisation of a list of matrices by Newton-Schulz products:
+ *     X = U / (|U|_F + eps);  `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
+ * (for a tall matrix with X^T X from the right, the same numbers).  It keeps the singular vectors of U and brings the singular values
+ * near 1.  coefficients: host array [steps][3] of a, b, c, or NULL: 3.4445, -4.7750, 2.0315 in every step; 1 <= steps <= 16.
+ * Coefficients under which a singular value of [0, 1] could grow beyond 16 are refused (GL_ERR_INVALID).  Every product is
+ * fp32-faithful (three fp16 products on tensor cores), the result is rounded to the output's type once.  A zero matrix
+ * gives zeros; a matrix with a NaN or an infinity gives NaN.  In and out are row-major of `type`, pitches in elements; out may
+ * be in.  (A column-major matrix is the transposed one row-major: its result comes out transposed too.) */
+typedef struct gl_ortho_item {
+	int32_t rows, cols;
+	const void* d_in;
+	int64_t ld_in;
+	void* d_out;
+	int64_t ld_out;
+} gl_ortho_item;
+int64_t gl_orthogonalize_workspace(const gl_ortho_item* items, int32_t count);
+int gl_orthogonalize(const gl_ortho_item* items, int32_t count, const float* coefficients, int32_t steps, float eps, int32_t type,
+                     void* d_work, int64_t work_bytes, void* stream, int32_t device);
+
+/* Momentum update of a list of weight matrices whose direction is orthogonalised, O() as above:
+ *     M' = momentum * M + G;   U = G + momentum * M' (nesterov) or M';   W' = (1 - lr * weight_decay) W - lr O(U)
+ * G is of `type`, M and W are fp32, each with its own pitch; M' and W' go to d_momentum_out and d_weight_out, which may be
+ * d_momentum and d_weight.  lr is the matrix's own: users scale it with sqrt(max(1, rows / cols)) or the like. */
+typedef struct gl_muon_item {
+	int32_t rows, cols;
+	float lr;
+	const void* d_grad;
+	int64_t ld_grad;
+	const float* d_momentum;
+	float* d_momentum_out;
+	int64_t ld_momentum;
+	const float* d_weight;
+	float* d_weight_out;
+	int64_t ld_weight;
+} gl_muon_item;
+int64_t gl_muon_workspace(const gl_muon_item* items, int32_t count);
+int gl_muon_step(const gl_muon_item* items, int32_t count, float momentum, int32_t nesterov, float weight_decay, const float* coefficients,
+                 int32_t steps, float eps, int32_t type, void* d_work, int64_t work_bytes, void* stream, int32_t device);
+/* Waits for `stream` and reports whether a bounded wait inside the last gl_orthogonalize or gl_muon_step call on this workspace ran out
+ * (GL_ERR_TIMEOUT: its results hold nothing of use). */
+int gl_orthogonalize_status(const void* d_work, void* stream, int32_t device);
+
 /* ---- measurement helpers (no counterpart in the reference) ------------------------------ */
 /* CUDA events on the handle's own stream around whatever is queued between the two calls. */
 int gl_timer_start(gl_net* net);
