@@ -76,8 +76,7 @@ int check_steps(const char* name, OrthoArgs& a, const float* coefficients, int s
 	if (!(eps >= 0.0f) || isinf(eps)) return report_error(GL_ERR_INVALID, "%s: eps must be a number >= 0", name);
 	for (int k = 0; k < steps; ++k)
 		for (int j = 0; j < 3; ++j) a.coef[k][j] = coefficients ? coefficients[3 * k + j] : kQuintic[j];
-	double sx[ORTHO_MAX_STEPS + 1], sa[ORTHO_MAX_STEPS], sp[ORTHO_MAX_STEPS];
-	if (!ortho_bounds(a.coef, steps, sx, sa, sp))
+	if (!ortho_coefficients_ok(a.coef, steps))
 		return report_error(GL_ERR_INVALID, "%s: under these coefficients a singular value could grow beyond 16", name);
 	a.steps = steps;
 	a.eps = eps;
@@ -103,7 +102,7 @@ int64_t workspace(const char* name, const ITEM* items, int count)
 			m[i].cols = items[i].cols;
 			total += 64.0 * ((double)items[i].rows + 128) * ((double)items[i].cols + 128);
 		}
-		if (total > 9e18) return report_error(GL_ERR_TOO_LARGE, "%s: the matrices are too large", name);
+		if (total > 4e18) return report_error(GL_ERR_TOO_LARGE, "%s: the matrices are too large", name);
 		return (int64_t)ortho_workspace_bytes(m.data(), count);
 	}
 	catch (const std::bad_alloc&)
@@ -122,7 +121,7 @@ int run_ortho(const char* name, OrthoArgs& a, const std::vector<OrthoMatrix>& m,
 	if (int r = check_device(device)) return r;
 	OnDevice guard(device);
 	if (guard.error != cudaSuccess) return finish(name, guard.error);
-	return finish(name, launch_orthogonalize(a, d_work, static_cast<cudaStream_t>(stream)));
+	return finish(name, launch_orthogonalize(a, d_work, (size_t)work_bytes, static_cast<cudaStream_t>(stream)));
 }
 
 }  // namespace

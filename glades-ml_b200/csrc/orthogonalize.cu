@@ -1,17 +1,32 @@
 // Orthogonalisation of matrices by a polynomial iteration, and the weight update that is built on it.
-//     X_0 = U / (|U|_F + eps),   A = X X^T,   P = a I + b A + c A^2,   X <- P X,   O = X_last
+//     X_0 = U / (|U|_F + eps),   A = X X^T,   R = b A + c A^2,   X <- a X + R X,   O = X_last
 // drives the singular values of U towards 1 and keeps its singular vectors.  X is held with its short side p as rows (a tall
-// matrix is transposed on the way in and on the way out), so that A and P are p x p.
+// matrix is transposed on the way in and on the way out), so that A and R are p x p.
+//
+// Several steps on the short side alone ("a group"): P = a + R is a polynomial of A and commutes with it, so the next step's
+// A is P A P, and the group's X is (P_n .. P_1) X.  A group of n steps costs one product with X on both sides (A) and one with X
+// on one side instead of n of each, and 2 (n - 1) + (n - 1) more products of p x p matrices:
+//     T = a A + R A,   A' = a T + T R,   Q' = P Q  as  q' + Qr' = a q + (a Qr + q R + R Qr)
+// 15 p^2 q + 5 p^3 multiply-adds become 6 p^2 q + 14 p^3 for five steps in groups of three and two (symmetric products by half).
+// A's rounding is absolute, so small singular values lose digits with every further step of a group: three steps from the start,
+// where the elements of A are small, and two later stay within the error of fp32 products (emulated and measured); see groups_of.
 //
 // Bound: tensor cores.  Every product is fp32-faithful on three fp16 products (hi*hi + hi*lo + lo*hi), as the layer products of
 // gemm_tcgen05.cu; unlike there the scales are known beforehand -- all singular values stay below a bound that follows from
-// the coefficients alone -- so no product waits for a largest element, and lo is not scaled: the three products share one
-// accumulator, tensor memory holds two of them, and the MMAs of one chunk run while the chunk in front is drained.  The
-// error floor of an unscaled lo is 2^-25 of a unit, 2^-38 of the largest element.
-// A and A^2 are symmetric: tiles above the diagonal are left out, an element below it is stored at both places.
+// the coefficients alone -- so no product waits for a largest element, and lo is not scaled (its error floor is 2^-25 of a unit,
+// 2^-38 of the largest element): tensor memory holds two accumulators of a tile, and the MMAs of one chunk run while the
+// chunk in front is drained.  On tiles of at most 128 columns hi and lo of the second operand lie one behind the other in
+// shared memory and are one operand of twice the columns, [hi*hi | hi*lo]: two MMAs instead of three, an accumulator for
+// each half, fewer reads of shared memory.  On 256 columns, which no longer fit so, the three products share one.
+// a X (b A, a T, ..) is where the epilogue's registers start from, loaded while the first chunk is computed: inside the accumulator
+// it would be truncated with every addition, which doubles the error of the result (3.3e-6 against 1.3e-6 of a 256 x 256
+// matrix, fp32 products: 2.5e-6).
+// A, R, T and Q are symmetric: tiles above the diagonal are left out, an element below it is stored at both places.
 //
-// One cooperative launch walks all steps of all matrices: norm, scaling, then three phases per step, a grid barrier after
-// each.  Within a phase every CTA takes the tiles cta, cta + grid, ... of all matrices.
+// One cooperative launch walks all steps of all matrices: norm, scaling, then rounds of products that do not depend on one
+// another, a grid barrier after each.  Within a round every CTA takes the items cta, cta + grid, ... of all matrices.  Where a
+// round has too few tiles for the SMs, its tiles are split along k: the parts go to scratch in fp32, and after one more
+// barrier all warps of the GPU add them up, 32 x 32 elements at a time, in a fixed order.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -28,14 +43,21 @@ using namespace tc;
 namespace {
 
 constexpr int OR_BK = 32;      // k per pipeline stage
-// Stages whose products an accumulator takes before it is drained: the tensor core truncates as it adds, so a chain of n
-// additions drifts by up to n * 2^-24 towards zero; 4 stages are 24 additions.
-constexpr int OR_CHUNK = 4;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
+constexpr int OR_SMS = 148;
+constexpr int OR_SPLIT_KB = 4; // stages that a part of a split tile has at least
+constexpr int OR_MAX_OPS = 4 * ORTHO_MAX_STEPS;
+constexpr int OR_MAX_ROUNDS = 64;  // at most 55 are needed: step by step three per step, in groups of n 3 n + 1
+constexpr int OR_PLANES = 6;   // p x p matrices of a grouped program
 
 template <int BN>
 struct OrSmem
 {
+	static constexpr bool PAIR = BN <= 128;                  // hi and lo of B as one operand of 2 * BN columns
+	// Stages whose products an accumulator takes before it is drained: the tensor core truncates as it adds, so a chain of n
+	// additions drifts by up to n * 2^-24 towards zero; 12 (4) stages are 24 additions of full size.
+	static constexpr int CHUNK = PAIR ? 12 : 4;
+	static constexpr int COLUMNS = PAIR ? 2 * BN : BN;       // of an accumulator
 	static constexpr int STAGES = BN == 256 ? 4 : (BN == 128 ? 6 : 8);
 	static constexpr int EC = BN < 128 ? BN : 128;           // columns per epilogue warp
 	static constexpr int EPI_WARPS = 4 * (BN / EC);
@@ -45,15 +67,32 @@ struct OrSmem
 	static constexpr int STAGE_BYTES = 2 * A_BYTES + 2 * B_BYTES;
 	static constexpr int TILES_BYTES = STAGES * STAGE_BYTES;
 	static constexpr int STAGING_BYTES = EPI_WARPS * 4096;   // at least a piece of the elementwise phases, 64 x 64 floats
+	static constexpr int PIECES = 4 * (BN / 32);             // 32 x 32 pieces of a tile
 	static constexpr int TOTAL = TILES_BYTES + STAGING_BYTES + 1024 /*alignment slack*/ + 512 /*barriers, sums*/;
+};
+
+// Matrices of parts that an operation names: 0 .. 5 p x p, 6 and 7 the two X.
+enum { ID_A = 0, ID_X = 6, ID_NONE = -1 };
+// out = f (A B^T or A B + w1 E1 + w2 E2); the factors hold the parts' scales
+struct OrOp
+{
+	signed char a, b, e1, e2, out;  // out ID_NONE: the result
+	signed char round;
+	float f, w1, w2, so;
+};
+struct OrProgram
+{
+	OrOp op[OR_MAX_OPS];
+	int count, rounds, planes;
+	unsigned char first[OR_MAX_ROUNDS + 1];  // operations first[r] .. first[r + 1] - 1 are round r's
 };
 
 struct OrMat
 {
 	OrthoMatrix m;
-	int p, q, tall;
+	int p, q, tall, grouped;
 	long long ldx, planex;  // halfs: row pitch and size of one part of X; parts in the order X0 hi, X0 lo, X1 hi, X1 lo
-	long long lds, planes;  // the same of A hi, A lo, P hi, P lo
+	long long lds, planes;  // the same of the p x p matrices
 	__half* X;
 	__half* S;
 	int units;              // pieces of the elementwise phases in front of this matrix's, and their number along a row
@@ -61,120 +100,175 @@ struct OrMat
 };
 struct OrMaps
 {
-	CUtensorMap xa, xb, xn, sa, sb;  // X as K-major A operand, K-major B operand, MN-major B operand; A and P as K-major operands
+	CUtensorMap xa, xb, xn, sa, sb;  // X as K-major A operand, K-major B operand, MN-major B operand; p x p as K-major operands
 };
 struct OrParams
 {
 	OrMaps maps[ORTHO_MAX_MATRICES];
 	OrMat mat[ORTHO_MAX_MATRICES];
-	int count, steps, units;
+	OrProgram prog[2];      // step by step; in groups
+	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
+	unsigned long long reduce;  // rounds with split tiles
+	int count, rounds, units;
 	int type, step, nesterov, reset;
-	float mu, decay, eps;
-	float coef[ORTHO_MAX_STEPS][3];
-	int ex[ORTHO_MAX_STEPS + 1], ea[ORTHO_MAX_STEPS], ep[ORTHO_MAX_STEPS];  // exponents of the scales of X, A, P
+	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
-	double* part;  // [matrix][grid] sums of squares
+	double* sums;  // [matrix][grid] sums of squares
+	float4* part;  // parts of split tiles
 };
 
-enum { PHASE_GRAM = 0, PHASE_POLY = 1, PHASE_APPLY = 2 };
-
-// A phase's tiles of one matrix: rows m-tile by m-tile; of a symmetric product only the tiles that reach the diagonal.
-__host__ __device__ inline int sym_tiles_of_row(int mt, int bn) { return (mt * TC_BM + TC_BM - 1) / bn + 1; }
-__host__ __device__ inline int phase_tiles(int p, int q, int phase, int bn)
+// An operation's tiles of one matrix, of a symmetric product only those that reach the diagonal.
+__host__ __device__ inline bool op_symmetric(const OrOp& o) { return o.b < ID_X || o.a >= ID_X; }
+__host__ __device__ inline int op_kb(const OrOp& o, int p, int q) { return ((o.a >= ID_X ? q : p) + OR_BK - 1) / OR_BK; }
+__host__ __device__ inline int tiles_of_row(int mt, int tn, int bn)
+{
+	const int c = (mt * TC_BM + TC_BM - 1) / bn + 1;
+	return c < tn ? c : tn;
+}
+__host__ __device__ inline int op_tiles(const OrOp& o, int p, int q, int bn)
 {
 	const int tm = (p + TC_BM - 1) / TC_BM;
-	if (phase == PHASE_APPLY) return tm * ((q + bn - 1) / bn);
+	if (!op_symmetric(o)) return tm * ((q + bn - 1) / bn);
 	const int tn = (p + bn - 1) / bn;
+	// (in closed form but for the rows that tn cuts off)
 	int n = 0;
-	for (int mt = 0; mt < tm; ++mt)
-	{
-		const int c = sym_tiles_of_row(mt, bn);
-		n += c < tn ? c : tn;
-	}
+	for (int mt = 0; mt < tm; ++mt) n += tiles_of_row(mt, tn, bn);
 	return n;
 }
 
-struct OrTile
+struct OrItem
 {
-	int mat, m0, n0, kb;
+	int mat, op, m0, n0, kb0, kb1, split, slot;  // slot: of a split tile's first part
 };
-// tile t of a phase, or false
+// the tile t of operation o
 template <int BN>
-__device__ __forceinline__ bool find_tile(const OrParams& P, int phase, int t, OrTile& o)
+__device__ __forceinline__ void tile_origin(const OrOp& o, int p, int q, int t, int& m0, int& n0)
 {
+	const int tm = (p + TC_BM - 1) / TC_BM;
+	if (!op_symmetric(o))
+	{
+		m0 = (t % tm) * TC_BM;
+		n0 = (t / tm) * BN;
+		return;
+	}
+	const int tn = (p + BN - 1) / BN;
+	for (int mt = tm - 1;; --mt)
+	{
+		const int n = tiles_of_row(mt, tn, BN);
+		if (t < n || mt == 0)
+		{
+			m0 = mt * TC_BM;
+			n0 = t * BN;
+			return;
+		}
+		t -= n;
+	}
+}
+// item t of a round, or false
+template <int BN>
+__device__ __forceinline__ bool find_item(const OrParams& P, int round, int t, OrItem& it)
+{
+	int slot = 0;
 	for (int i = 0; i < P.count; ++i)
 	{
-		const int p = P.mat[i].p, q = P.mat[i].q;
-		const int tm = (p + TC_BM - 1) / TC_BM;
-		if (phase == PHASE_APPLY)
+		const OrMat& M = P.mat[i];
+		const OrProgram& g = P.prog[M.grouped];
+		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
 		{
-			const int n = tm * ((q + BN - 1) / BN);
+			const int s = P.split[i][k];
+			const int n = op_tiles(g.op[k], M.p, M.q, BN) * s;
 			if (t < n)
 			{
-				o.mat = i;
-				o.m0 = (t % tm) * TC_BM;
-				o.n0 = (t / tm) * BN;
-				o.kb = (p + OR_BK - 1) / OR_BK;
+				const int tile = t / s, part = t - tile * s;
+				const int kb = op_kb(g.op[k], M.p, M.q);
+				it.mat = i;
+				it.op = k;
+				it.split = s;
+				it.kb0 = kb * part / s;
+				it.kb1 = kb * (part + 1) / s;
+				it.slot = slot + t;
+				tile_origin<BN>(g.op[k], M.p, M.q, tile, it.m0, it.n0);
 				return true;
 			}
 			t -= n;
-			continue;
+			if (s > 1) slot += n;
 		}
-		const int tn = (p + BN - 1) / BN;
-		for (int mt = tm - 1; mt >= 0; --mt)
+	}
+	return false;
+}
+// tile t of a round's split operations, or false
+template <int BN>
+__device__ __forceinline__ bool find_split(const OrParams& P, int round, int t, OrItem& it)
+{
+	int slot = 0;
+	for (int i = 0; i < P.count; ++i)
+	{
+		const OrMat& M = P.mat[i];
+		const OrProgram& g = P.prog[M.grouped];
+		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
 		{
-			const int n = min(tn, sym_tiles_of_row(mt, BN));
+			const int s = P.split[i][k];
+			if (s < 2) continue;
+			const int n = op_tiles(g.op[k], M.p, M.q, BN);
 			if (t < n)
 			{
-				o.mat = i;
-				o.m0 = mt * TC_BM;
-				o.n0 = t * BN;
-				o.kb = ((phase == PHASE_GRAM ? q : p) + OR_BK - 1) / OR_BK;
+				it.mat = i;
+				it.op = k;
+				it.split = s;
+				it.slot = slot + t * s;
+				tile_origin<BN>(g.op[k], M.p, M.q, t, it.m0, it.n0);
 				return true;
 			}
 			t -= n;
+			slot += n * s;
 		}
 	}
 	return false;
 }
 
+// ---- elements of the caller's matrices, four neighbours at a time ------------------------------------------------
 __device__ __forceinline__ float load_typed(const void* p, long long i, int type)
 {
 	if (type == GL_F32) return static_cast<const float*>(p)[i];
 	if (type == GL_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 	return __half2float(static_cast<const __half*>(p)[i]);
 }
-__device__ __forceinline__ void store_typed(void* p, long long i, float v, int type)
+// `left` of them exist; wide: a 16-byte (8-byte) boundary
+__device__ __forceinline__ void load4(const void* p, long long i, int type, bool wide, int left, float (&v)[4])
 {
-	if (type == GL_F32) static_cast<float*>(p)[i] = v;
-	else if (type == GL_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-	else static_cast<__half*>(p)[i] = __float2half_rn(v);
+	if (wide && left >= 4)
+	{
+		if (type == GL_F32)
+		{
+			const float4 w = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+			v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+			return;
+		}
+		const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i);
+#pragma unroll
+		for (int k = 0; k < 4; ++k)
+		{
+			const unsigned short u = (unsigned short)((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
+			v[k] = type == GL_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+		}
+		return;
+	}
+#pragma unroll
+	for (int k = 0; k < 4; ++k) v[k] = k < left ? load_typed(p, i + k, type) : 0.0f;
 }
-
-// What element (r, c) contributes: the gradient itself, or the momentum that it makes (left in mom_out by the first visit).
-__device__ __forceinline__ float first_visit(const OrParams& P, const OrthoMatrix& m, int r, int c)
+__device__ __forceinline__ void store4(float* p, long long i, bool wide, int left, const float (&v)[4])
 {
-	const float g = load_typed(m.grad, (long long)r * m.ld_grad + c, P.type);
-	if (!P.step) return g;
-	const long long i = (long long)r * m.ld_mom + c;
-	const float v = fmaf(P.mu, m.mom[i], g);
-	m.mom_out[i] = v;
-	return P.nesterov ? fmaf(P.mu, v, g) : v;
-}
-__device__ __forceinline__ float second_visit(const OrParams& P, const OrthoMatrix& m, int r, int c)
-{
-	if (!P.step) return load_typed(m.grad, (long long)r * m.ld_grad + c, P.type);
-	const float v = m.mom_out[(long long)r * m.ld_mom + c];
-	return P.nesterov ? fmaf(P.mu, v, load_typed(m.grad, (long long)r * m.ld_grad + c, P.type)) : v;
+	if (wide && left >= 4)
+	{
+		*reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
+		return;
+	}
+#pragma unroll
+	for (int k = 0; k < 4; ++k)
+		if (k < left) p[i + k] = v[k];
 }
 
 // hi and lo of x * s, lo unscaled
-__device__ __forceinline__ void split_plain(float x, float s, __half& hi, __half& lo)
-{
-	const float xs = x * s;
-	hi = __float2half_rn(xs);
-	lo = __float2half_rn(xs - __half2float(hi));
-}
 __device__ __forceinline__ void split_pair(float x, float y, float s, uint32_t& hi, uint32_t& lo)
 {
 	const float xs = x * s, ys = y * s;
@@ -185,8 +279,9 @@ __device__ __forceinline__ void split_pair(float x, float y, float s, uint32_t& 
 	lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// 32 x 32 piece, a row per lane: as the rows of a matrix of parts.  Through shared memory, eight rows of 64 bytes per access.
-__device__ __forceinline__ void store_rows(const float (&v)[32], float s, __half* hi, __half* lo, long long ld, uint32_t area, int lane)
+// ---- 32 x 32 pieces, a row per lane --------------------------------------------------------------------------------
+// as the rows of a matrix of parts: through shared memory, four rows of 128 bytes (hi and lo) per access
+__device__ __forceinline__ void store_rows(const float (&v)[32], float s, __half* hi, long long plane, long long ld, uint32_t area, int lane)
 {
 	__syncwarp();
 #pragma unroll
@@ -200,26 +295,38 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], float s, __half
 		asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (uint32_t)(((k + 4) ^ (lane & 7)) << 4)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
 	}
 	__syncwarp();
+	const int k = lane & 7;
+	__half* d = hi + (k < 4 ? 0 : plane) + (long long)(lane >> 3) * ld + (k & 3) * 8;
 #pragma unroll
 	for (int i = 0; i < 8; ++i)
 	{
-		const int r = i * 4 + (lane >> 3), k = lane & 7;
+		const int r = i * 4 + (lane >> 3);
 		uint4 w;
 		asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(area + (uint32_t)r * 128u + (uint32_t)((k ^ (r & 7)) << 4)));
-		__half* d = (k < 4 ? hi : lo) + (long long)r * ld + (k & 3) * 8;
 		*reinterpret_cast<uint4*>(d) = w;
+		d += 4 * ld;
 	}
 }
-// the same piece transposed: column j is row j of the destination
-__device__ __forceinline__ void store_columns(const float (&v)[32], float s, __half* hi, __half* lo, long long ld, int lane)
+// acc += w * (32 elements of row r from column c on of the matrix of parts id)
+__device__ __forceinline__ void add_parts(float* acc, float w, int id, const OrMat& M, int r, int c)
 {
+	if (id == ID_NONE) return;
+	const long long plane = id >= ID_X ? M.planex : M.planes;
+	const __half* hi = id >= ID_X ? M.X + 2 * (id - ID_X) * plane + r * M.ldx + c : M.S + 2 * id * plane + r * M.lds + c;
 #pragma unroll
-	for (int j = 0; j < 32; ++j)
+	for (int k = 0; k < 4; ++k)
 	{
-		__half h, l;
-		split_plain(v[j], s, h, l);
-		hi[(long long)j * ld + lane] = h;
-		lo[(long long)j * ld + lane] = l;
+		const uint4 h4 = *reinterpret_cast<const uint4*>(hi + 8 * k);
+		const uint4 l4 = *reinterpret_cast<const uint4*>(hi + plane + 8 * k);
+		const __half2* h = reinterpret_cast<const __half2*>(&h4);
+		const __half2* l = reinterpret_cast<const __half2*>(&l4);
+#pragma unroll
+		for (int i = 0; i < 4; ++i)
+		{
+			const float2 x = __half22float2(h[i]), y = __half22float2(l[i]);
+			acc[8 * k + 2 * i] = fmaf(w, x.x + y.x, acc[8 * k + 2 * i]);
+			acc[8 * k + 2 * i + 1] = fmaf(w, x.y + y.y, acc[8 * k + 2 * i + 1]);
+		}
 	}
 }
 // 32 x 32 floats in shared memory, element (r, c) at r * 32 + (c ^ r): rows and columns without bank conflicts
@@ -230,6 +337,142 @@ __device__ __forceinline__ float square_get(uint32_t area, int r, int c)
 	float v;
 	asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(square_at(area, r, c)) : "memory");
 	return v;
+}
+// v: column per lane
+__device__ __forceinline__ void transpose(float (&v)[32], uint32_t area, int lane)
+{
+	__syncwarp();
+#pragma unroll
+	for (int j = 0; j < 32; ++j) square_put(area, lane, j, v[j]);
+	__syncwarp();
+#pragma unroll
+	for (int j = 0; j < 32; ++j) v[j] = square_get(area, j, lane);
+}
+
+// the result's elements of column (tall: row) c0 + lane ... of the caller's matrix: v[j] is element (r + j, c) of it
+template <int TYPE>
+__device__ __forceinline__ void store_result(const float (&v)[32], void* out, long long ld, int r, int c, int rows, int cols)
+{
+	if (c >= cols) return;
+	const int n = rows - r;
+	const long long i = r * ld + c;
+#pragma unroll
+	for (int j = 0; j < 32; ++j)
+		if (j < n)
+		{
+			if (TYPE == GL_F32) static_cast<float*>(out)[i + j * ld] = v[j];
+			else if (TYPE == GL_BF16) static_cast<__nv_bfloat16*>(out)[i + j * ld] = __float2bfloat16_rn(v[j]);
+			else static_cast<__half*>(out)[i + j * ld] = __float2half_rn(v[j]);
+		}
+}
+__device__ __forceinline__ void update_weights(const float (&v)[32], const OrthoMatrix& m, float decay, int r, int c)
+{
+	if (c >= m.cols) return;
+	const int n = m.rows - r;
+	const float keep = 1.0f - m.lr * decay;
+	const float* w = m.w + r * m.ld_w + c;
+	float* o = m.w_out + r * m.ld_w + c;
+#pragma unroll
+	for (int b = 0; b < 32; b += 16)
+	{
+		float x[16];
+#pragma unroll
+		for (int j = 0; j < 16; ++j) x[j] = b + j < n ? w[(b + j) * m.ld_w] : 0.0f;
+#pragma unroll
+		for (int j = 0; j < 16; ++j)
+			if (b + j < n) o[(b + j) * m.ld_w] = fmaf(-m.lr, v[b + j], keep * x[j]);
+	}
+}
+
+// what becomes of a piece of a product: rows r0 + lane, columns c0 ..
+__device__ __forceinline__ void finish_piece(const OrParams& P, const OrMat& M, const OrOp& o, float (&v)[32], int r0, int c0, uint32_t area, int lane)
+{
+#pragma unroll
+	for (int i = 0; i < 32; ++i) v[i] *= o.f;
+	if (o.out == ID_NONE)
+	{
+		if (!M.tall) transpose(v, area, lane);
+		// a wide matrix: lane = column, v = rows r0 ..; a tall one is transposed already: lane = its column, v = its rows c0 ..
+		const int r = M.tall ? c0 : r0, c = (M.tall ? r0 : c0) + lane;
+		if (P.step) update_weights(v, M.m, P.decay, r, c);
+		else if (P.type == GL_F32) store_result<GL_F32>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
+		else if (P.type == GL_BF16) store_result<GL_BF16>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
+		else store_result<GL_F16>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
+		return;
+	}
+	if (o.out >= ID_X)
+	{
+		store_rows(v, o.so, M.X + 2 * (o.out - ID_X) * M.planex + (long long)r0 * M.ldx + c0, M.planex, M.ldx, area, lane);
+		return;
+	}
+	__half* D = M.S + 2 * o.out * M.planes;
+	if (c0 == r0)
+	{
+		// on the diagonal: the upper half becomes the lower half's mirror image
+		__syncwarp();
+#pragma unroll
+		for (int j = 0; j < 32; ++j) square_put(area, lane, j, v[j]);
+		__syncwarp();
+#pragma unroll
+		for (int j = 0; j < 32; ++j)
+			if (j > lane) v[j] = square_get(area, j, lane);
+	}
+	store_rows(v, o.so, D + (long long)r0 * M.lds + c0, M.planes, M.lds, area, lane);
+	if (c0 != r0)
+	{
+		transpose(v, area, lane);
+		store_rows(v, o.so, D + (long long)c0 * M.lds + r0, M.planes, M.lds, area, lane);
+	}
+}
+// pieces that lie outside the matrix, or above the diagonal of a symmetric result (another piece's mirror image)
+__device__ __forceinline__ bool piece_needed(const OrMat& M, const OrOp& o, int r0, int c0)
+{
+	if (r0 >= M.p) return false;
+	return op_symmetric(o) ? c0 <= r0 : c0 < M.q;
+}
+
+__device__ __forceinline__ bool elect_one()
+{
+	uint32_t p;
+	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+	return p != 0;
+}
+// A bounded wait of a whole warp, which stays together: what the issuing warps compute can then live in uniform registers
+// (one lane on its own spends 70 clocks on the operands of every MMA it issues).
+__device__ __noinline__ static bool warp_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag, int code)
+{
+	const long long t0 = clock64();
+	for (;;)
+	{
+		if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
+		if (__any_sync(0xFFFFFFFFu, *abort_flag != 0)) return false;
+		if (__any_sync(0xFFFFFFFFu, clock64() - t0 > TC_WAIT_CYCLES))
+		{
+			if ((threadIdx.x & 31) == 0)
+			{
+				*abort_flag = 1;
+				atomicExch(err_flag, code);
+			}
+			return false;
+		}
+	}
+}
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag, int code)
+{
+	return __all_sync(0xFFFFFFFFu, mbar_try(bar, parity)) || warp_wait_slow(bar, parity, abort_flag, err_flag, code);
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
+{
+	asm volatile(
+	    "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+	    "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+	    "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+	    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+	      "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+	      "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+	      "=r"(r[31])
+	    : "r"(taddr)
+	    : "memory");
 }
 
 template <int BN>
@@ -253,7 +496,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	double* warp_sums = reinterpret_cast<double*>(tail + 8);  // 10 at most
 
 	cg::grid_group grid = cg::this_grid();
-	const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+	const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
 	if (threadIdx.x == 0)
 	{
@@ -274,34 +517,60 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	}
 	if (warp == 1)
 	{
-		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN) : "memory");
+		asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * S::COLUMNS) : "memory");
 		asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 	}
 	asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 	__syncthreads();
 	asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-	const uint32_t tmem_base = *tmem_slot;
+	const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, *tmem_slot, 0);
 
-	// ---- sums of squares, in double (a product of two floats is exact there and does not leave its range)
+	// ---- the elementwise phases: pieces of 64 x 64 elements; piece u of matrix i belongs to CTA (M.units + u) mod grid in both.
+	// Four neighbours per thread and turn, the loads of all its turns ahead of the stores.
+	constexpr int QUADS = OR_UNIT * OR_UNIT / 4;
+	constexpr int TURNS = (QUADS + THREADS - 1) / THREADS;
+	auto wide_ok = [](const void* p, long long ld, int size) { return (((uintptr_t)p | (uintptr_t)(ld * size)) & (4 * size - 1)) == 0; };
+	// sums of squares, in double (a product of two floats is exact there and does not leave its range)
 	for (int i = 0; i < P.count; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const int units = M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
+		const OrthoMatrix& m = M.m;
+		const bool wg = wide_ok(m.grad, m.ld_grad, P.type == GL_F32 ? 4 : 2);
+		const bool wm = P.step && wide_ok(m.mom, m.ld_mom, 4) && wide_ok(m.mom_out, m.ld_mom, 4);
+		const int units = M.units_per_row * ((m.rows + OR_UNIT - 1) / OR_UNIT);
 		double sum = 0.0;
-		// (unit u of matrix i belongs to CTA (M.units + u) mod grid, here and in the next phase)
 		const int first = ((int)blockIdx.x - M.units % (int)gridDim.x + (int)gridDim.x) % (int)gridDim.x;
 		for (int u = first; u < units; u += gridDim.x)
 		{
 			const int r0 = (u / M.units_per_row) * OR_UNIT, c0 = (u % M.units_per_row) * OR_UNIT;
-#pragma unroll 4
-			for (int e = threadIdx.x; e < OR_UNIT * OR_UNIT; e += THREADS)
+			float g[TURNS][4], v[TURNS][4];
+#pragma unroll
+			for (int k = 0; k < TURNS; ++k)
 			{
-				const int r = r0 + e / OR_UNIT, c = c0 + e % OR_UNIT;
-				if (r < M.m.rows && c < M.m.cols)
+				const int e = threadIdx.x + k * THREADS;
+				const int r = r0 + e / (OR_UNIT / 4), c = c0 + e % (OR_UNIT / 4) * 4;
+				const int left = e < QUADS && r < m.rows ? m.cols - c : 0;
+				load4(m.grad, (long long)r * m.ld_grad + c, P.type, wg, left, g[k]);
+				if (P.step) load4(m.mom, (long long)r * m.ld_mom + c, GL_F32, wm, left, v[k]);
+			}
+#pragma unroll
+			for (int k = 0; k < TURNS; ++k)
+			{
+				if (P.step)
 				{
-					const double v = first_visit(P, M.m, r, c);
-					sum = fma(v, v, sum);
+					const int e = threadIdx.x + k * THREADS;
+					const int r = r0 + e / (OR_UNIT / 4), c = c0 + e % (OR_UNIT / 4) * 4;
+					const int left = e < QUADS && r < m.rows ? m.cols - c : 0;
+#pragma unroll
+					for (int j = 0; j < 4; ++j)
+					{
+						v[k][j] = fmaf(P.mu, v[k][j], g[k][j]);
+						g[k][j] = P.nesterov ? fmaf(P.mu, v[k][j], g[k][j]) : v[k][j];
+					}
+					store4(m.mom_out, (long long)r * m.ld_mom + c, wm, left, v[k]);
 				}
+#pragma unroll
+				for (int j = 0; j < 4; ++j) sum = fma((double)g[k][j], (double)g[k][j], sum);
 			}
 		}
 #pragma unroll
@@ -313,66 +582,90 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		{
 			double t = 0.0;
 			for (int w = 0; w < THREADS / 32; ++w) t += warp_sums[w];
-			P.part[i * gridDim.x + blockIdx.x] = t;
+			P.sums[i * gridDim.x + blockIdx.x] = t;
 		}
 	}
 	grid.sync();
 
-	// ---- X_0: scaled, split, the short side as rows
+	// X_0: scaled, split, the short side as rows
 	for (int i = 0; i < P.count; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const int units = M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
+		const OrthoMatrix& m = M.m;
+		const bool wg = wide_ok(m.grad, m.ld_grad, P.type == GL_F32 ? 4 : 2);
+		const bool wm = P.step && wide_ok(m.mom_out, m.ld_mom, 4);
+		const int units = M.units_per_row * ((m.rows + OR_UNIT - 1) / OR_UNIT);
 		const int first = ((int)blockIdx.x - M.units % (int)gridDim.x + (int)gridDim.x) % (int)gridDim.x;
 		if (first >= units) continue;
 		if (warp == 0)
 		{
 			double t = 0.0;
-			for (int k = lane; k < (int)gridDim.x; k += 32) t += P.part[i * gridDim.x + k];
+			for (int k = lane; k < (int)gridDim.x; k += 32) t += P.sums[i * gridDim.x + k];
 #pragma unroll
 			for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
 			if (lane == 0) warp_sums[0] = t;
 		}
 		__syncthreads();
-		const float norm = (float)sqrt(warp_sums[0]) + P.eps;
-		const float s = pow2f(P.ex[0]);
+		const double inv = 1.0 / ((double)(float)sqrt(warp_sums[0]) + (double)P.eps);
+		const float s = P.s0;
 		__syncthreads();
 		for (int u = first; u < units; u += gridDim.x)
 		{
 			const int r0 = (u / M.units_per_row) * OR_UNIT, c0 = (u % M.units_per_row) * OR_UNIT;
-#pragma unroll 4
-			for (int e = threadIdx.x; e < OR_UNIT * OR_UNIT; e += THREADS)
+			float g[TURNS][4], v[TURNS][4];
+#pragma unroll
+			for (int k = 0; k < TURNS; ++k)
 			{
-				const int rr = e / OR_UNIT, cc = e % OR_UNIT;
+				const int e = threadIdx.x + k * THREADS;
+				const int r = r0 + e / (OR_UNIT / 4), c = c0 + e % (OR_UNIT / 4) * 4;
+				const int left = e < QUADS && r < m.rows ? m.cols - c : 0;
+				if (!P.step || P.nesterov) load4(m.grad, (long long)r * m.ld_grad + c, P.type, wg, left, g[k]);
+				if (P.step) load4(m.mom_out, (long long)r * m.ld_mom + c, GL_F32, wm, left, v[k]);
+			}
+#pragma unroll
+			for (int k = 0; k < TURNS; ++k)
+			{
+				const int e = threadIdx.x + k * THREADS;
+				const int rr = e / (OR_UNIT / 4), cc = e % (OR_UNIT / 4) * 4;
 				const int r = r0 + rr, c = c0 + cc;
-				if (r < M.m.rows && c < M.m.cols)
+				if (e >= QUADS || r >= m.rows || c >= m.cols) continue;
+				float x[4];
+#pragma unroll
+				for (int j = 0; j < 4; ++j)
 				{
-					const float x = second_visit(P, M.m, r, c) / norm;
-					if (M.tall) piece[rr * OR_UNIT + (cc ^ (rr & 31))] = x;
-					else
-					{
-						__half h, l;
-						split_plain(x, s, h, l);
-						M.X[r * M.ldx + c] = h;
-						M.X[M.planex + r * M.ldx + c] = l;
-					}
+					const float w = !P.step ? g[k][j] : (P.nesterov ? fmaf(P.mu, v[k][j], g[k][j]) : v[k][j]);
+					x[j] = (float)((double)w * inv);
+				}
+				if (M.tall)
+				{
+#pragma unroll
+					for (int j = 0; j < 4; ++j) piece[rr * OR_UNIT + ((cc + j) ^ (rr & 31))] = x[j];
+				}
+				else
+				{
+					// (what lies beyond the last column is never read)
+					uint2 h, l;
+					split_pair(x[0], x[1], s, h.x, l.x);
+					split_pair(x[2], x[3], s, h.y, l.y);
+					*reinterpret_cast<uint2*>(M.X + r * M.ldx + c) = h;
+					*reinterpret_cast<uint2*>(M.X + M.planex + r * M.ldx + c) = l;
 				}
 			}
 			if (M.tall)
 			{
 				__syncthreads();
-#pragma unroll 4
-				for (int e = threadIdx.x; e < OR_UNIT * OR_UNIT; e += THREADS)
+#pragma unroll
+				for (int k = 0; k < 2 * TURNS; ++k)
 				{
-					const int cc = e / OR_UNIT, rr = e % OR_UNIT;
+					// two rows of the matrix (columns of X) per thread and turn, neighbouring lanes neighbouring pairs
+					const int e = threadIdx.x + k * THREADS;
+					const int cc = e / (OR_UNIT / 2), rr = e % (OR_UNIT / 2) * 2;
 					const int r = r0 + rr, c = c0 + cc;
-					if (r < M.m.rows && c < M.m.cols)
-					{
-						__half h, l;
-						split_plain(piece[rr * OR_UNIT + (cc ^ (rr & 31))], s, h, l);
-						M.X[c * M.ldx + r] = h;
-						M.X[M.planex + c * M.ldx + r] = l;
-					}
+					if (cc >= OR_UNIT || r >= m.rows || c >= m.cols) continue;
+					uint32_t h, l;
+					split_pair(piece[rr * OR_UNIT + (cc ^ (rr & 31))], piece[(rr + 1) * OR_UNIT + (cc ^ ((rr + 1) & 31))], s, h, l);
+					*reinterpret_cast<uint32_t*>(M.X + c * M.ldx + r) = h;
+					*reinterpret_cast<uint32_t*>(M.X + M.planex + c * M.ldx + r) = l;
 				}
 				__syncthreads();
 			}
@@ -382,231 +675,242 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	grid.sync();
 
 	// ---- the products
-	int s = 0;             // producer, MMA lane: next stage, and how often (mod 2) the ring has been walked
+	int s = 0;             // producer, MMA warp: next stage, and how often (mod 2) the ring has been walked
 	uint32_t ph = 0;
 	int issued = 0;
-	int buf = 0;           // MMA lane, epilogue: next accumulator, and how often (mod 2) both have been used
+	int buf = 0;           // MMA warp, epilogue: next accumulator, and how often (mod 2) both have been used
 	uint32_t aph = 0;
 	bool ok = true;
-	const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-	const int half = (warp - 2) >> 2;
-	for (int step = 0; step < P.steps; ++step)
+	for (int round = 0; round < P.rounds; ++round)
 	{
-		const int cur = step & 1;
-		for (int phase = PHASE_GRAM; phase <= PHASE_APPLY; ++phase)
+		OrItem t;
+		if (warp == 0)
 		{
-			OrTile t;
-			if (warp == 0 && lane == 0)
+			// ------------------------------------------------ TMA producer
+			asm volatile("fence.proxy.async;" ::: "memory");
+			const bool leader = elect_one();
+			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
 			{
-				// ------------------------------------------------ TMA producer
-				asm volatile("fence.proxy.async;" ::: "memory");
-				for (int ti = blockIdx.x; ok && find_tile<BN>(P, phase, ti, t); ti += gridDim.x)
+				const OrMaps& mp = P.maps[t.mat];
+				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
+				const bool ax = o.a >= ID_X, bx = o.b >= ID_X;
+				const CUtensorMap* ma = ax ? &mp.xa : &mp.sa;
+				const CUtensorMap* mb = ax ? &mp.xb : &mp.sb;
+				const int pa = 2 * (ax ? o.a - ID_X : o.a), pb = 2 * (bx ? o.b - ID_X : o.b);
+				const bool mn = bx && !ax;
+				for (int kb = t.kb0; kb < t.kb1; ++kb)
 				{
-					const OrMaps& mp = P.maps[t.mat];
-					const int plane_a = phase == PHASE_GRAM ? 2 * cur : (phase == PHASE_POLY ? 0 : 2);
-					const CUtensorMap* ma = phase == PHASE_GRAM ? &mp.xa : &mp.sa;
-					for (int kb = 0; kb < t.kb; ++kb)
+					const uint32_t full = bar0 + 8 * s;
+					if (!warp_wait(full + 8 * STAGES, ph ^ 1u, abort_flag, P.status, 1))
 					{
-						const uint32_t full = bar0 + 8 * s;
-						if (!mbar_wait(full + 8 * STAGES, ph ^ 1u, abort_flag, P.status, 1))
-						{
-							ok = false;
-							break;
-						}
+						ok = false;
+						break;
+					}
+					if (leader)
+					{
 						mbar_expect_tx(full, S::STAGE_BYTES);
 						const uint32_t sa = base + s * S::STAGE_BYTES;
-						tma_load_3d(sa, ma, full, kb * OR_BK, t.m0, plane_a);
-						if (phase == PHASE_APPLY) tma_load_4d(sa + 2 * S::A_BYTES, &mp.xn, full, 0, kb * OR_BK, t.n0 / 64, 2 * cur);
-						else if (phase == PHASE_GRAM) tma_load_3d(sa + 2 * S::A_BYTES, &mp.xb, full, kb * OR_BK, t.n0, 2 * cur);
-						else tma_load_3d(sa + 2 * S::A_BYTES, &mp.sb, full, kb * OR_BK, t.n0, 0);
-						++issued;
-						if (++s == STAGES)
-						{
-							s = 0;
-							ph ^= 1u;
-						}
+						tma_load_3d(sa, ma, full, kb * OR_BK, t.m0, pa);
+						if (mn) tma_load_4d(sa + 2 * S::A_BYTES, &mp.xn, full, 0, kb * OR_BK, t.n0 / 64, pb);
+						else tma_load_3d(sa + 2 * S::A_BYTES, mb, full, kb * OR_BK, t.n0, pb);
+					}
+					__syncwarp();
+					++issued;
+					if (++s == STAGES)
+					{
+						s = 0;
+						ph ^= 1u;
 					}
 				}
 			}
-			else if (warp == 1 && lane == 0)
+		}
+		else if (warp == 1)
+		{
+			// ------------------------------------------------ MMA issuer (layouts and descriptors: gemm_tcgen05.cu)
+			const bool leader = elect_one();
+			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
 			{
-				// ------------------------------------------------ MMA issuer (layouts and descriptors: gemm_tcgen05.cu)
-				const uint32_t b_mn = phase == PHASE_APPLY ? 1u : 0u;
+				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
+				const uint32_t b_mn = o.b >= ID_X && o.a < ID_X ? 1u : 0u;
 				const uint32_t idesc = (1u << 4) | (b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
+				const uint32_t idesc2 = (1u << 4) | (b_mn << 16) | ((uint32_t)(S::COLUMNS >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 				const uint64_t desc_a = make_smem_desc(base, 0u, 512u, 4u);
 				const uint64_t desc_b = make_smem_desc(base + 2 * S::A_BYTES, b_mn ? 128u * OR_BK : 0u, b_mn ? 1024u : 512u, b_mn ? 2u : 4u);
 				const uint32_t a_step = 32u >> 4, b_step = b_mn ? 2048u >> 4 : 32u >> 4;
 				constexpr uint32_t A_LO = S::A_BYTES >> 4, B_LO = S::B_BYTES >> 4;
-				for (int ti = blockIdx.x; ok && find_tile<BN>(P, phase, ti, t); ti += gridDim.x)
+				int in = 0;
+				for (int left = t.kb1 - t.kb0; left > 0; --left)
 				{
-					int in = 0;
-					for (int left = t.kb; left > 0; --left)
+					if (in == 0)
 					{
-						if (in == 0)
-						{
-							if (!mbar_wait(bar_acc_empty + 8 * buf, aph ^ 1u, abort_flag, P.status, 4)) { ok = false; break; }
-						}
-						const uint32_t full = bar0 + 8 * s;
-						if (!mbar_wait(full, ph, abort_flag, P.status, 2)) { ok = false; break; }
-						asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-						const uint32_t off = (uint32_t)s * (S::STAGE_BYTES >> 4);
-						const uint64_t a0 = desc_a + off, b0 = desc_b + off;
-						const uint64_t a1 = a0 + a_step, b1 = b0 + b_step;
-						const uint32_t d = tmem_base + (uint32_t)(buf * BN);
-						umma_f16(d, a0, b0 + B_LO, idesc, (uint32_t)in);
-						umma_f16(d, a0 + A_LO, b0, idesc, 1u);
-						umma_f16(d, a1, b1 + B_LO, idesc, 1u);
-						umma_f16(d, a1 + A_LO, b1, idesc, 1u);
-						umma_f16(d, a0, b0, idesc, 1u);
-						umma_f16(d, a1, b1, idesc, 1u);
-						umma_commit(full + 8 * STAGES);
-						if (++in == OR_CHUNK || left == 1)
-						{
-							umma_commit(bar_acc_full + 8 * buf);
-							in = 0;
-							buf ^= 1;
-							aph ^= (uint32_t)(buf == 0);
-						}
-						if (++s == STAGES)
-						{
-							s = 0;
-							ph ^= 1u;
-						}
+						if (!warp_wait(bar_acc_empty + 8 * buf, aph ^ 1u, abort_flag, P.status, 4)) { ok = false; break; }
 					}
-				}
-			}
-			else if (warp >= 2)
-			{
-				// ------------------------------------------------ epilogue
-				const bool last = phase == PHASE_APPLY && step == P.steps - 1;
-				const int es = phase == PHASE_GRAM ? 2 * P.ex[step] : (phase == PHASE_POLY ? 2 * P.ea[step] : P.ep[step] + P.ex[step]);
-				const float inv = pow2f(-es);
-				const float so = pow2f(phase == PHASE_GRAM ? P.ea[step] : (phase == PHASE_POLY ? P.ep[step] : P.ex[step + 1]));
-				const uint32_t area = staging0 + (uint32_t)(warp - 2) * 4096u;
-				for (int ti = blockIdx.x; ok && find_tile<BN>(P, phase, ti, t); ti += gridDim.x)
-				{
-					const OrMat& M = P.mat[t.mat];
-					float acc[EC];
-#pragma unroll
-					for (int i = 0; i < EC; ++i) acc[i] = 0.0f;
-					for (int done = 0; done < t.kb; done += OR_CHUNK)
+					const uint32_t full = bar0 + 8 * s;
+					if (!warp_wait(full, ph, abort_flag, P.status, 2)) { ok = false; break; }
+					asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+					const uint32_t off = (uint32_t)s * (S::STAGE_BYTES >> 4);
+					const uint64_t a0 = desc_a + off, b0 = desc_b + off;
+					const uint64_t a1 = a0 + a_step, b1 = b0 + b_step;
+					const uint32_t d = tmem_base + (uint32_t)(buf * S::COLUMNS);
+					const bool ends = in + 1 == S::CHUNK || left == 1;
+					if (leader)
 					{
-						if (!mbar_wait(bar_acc_full + 8 * buf, aph, abort_flag, P.status, 3))
+						if (S::PAIR)
 						{
-							ok = false;
-							break;
+							umma_f16(d, a0, b0, idesc2, (uint32_t)in);
+							umma_f16(d, a1, b1, idesc2, 1u);
+							umma_f16(d + BN, a0 + A_LO, b0, idesc, 1u);
+							umma_f16(d + BN, a1 + A_LO, b1, idesc, 1u);
 						}
-						asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-						const uint32_t taddr = tmem_base + lane_base + (uint32_t)(buf * BN + half * EC);
-#pragma unroll
-						for (int c = 0; c < EC / 16; ++c)
+						else
 						{
-							uint32_t r[16];
-							tmem_ld16(taddr + (uint32_t)(c * 16), r);
-							asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-							for (int e = 0; e < 16; ++e) acc[c * 16 + e] += __uint_as_float(r[e]);
+							umma_f16(d, a0, b0 + B_LO, idesc, (uint32_t)in);
+							umma_f16(d, a0 + A_LO, b0, idesc, 1u);
+							umma_f16(d, a1, b1 + B_LO, idesc, 1u);
+							umma_f16(d, a1 + A_LO, b1, idesc, 1u);
+							umma_f16(d, a0, b0, idesc, 1u);
+							umma_f16(d, a1, b1, idesc, 1u);
 						}
-						asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-						__syncwarp();
-						if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_acc_empty + 8 * buf) : "memory");
+						umma_commit(full + 8 * STAGES);
+						if (ends) umma_commit(bar_acc_full + 8 * buf);
+					}
+					__syncwarp();
+					++in;
+					if (ends)
+					{
+						in = 0;
 						buf ^= 1;
 						aph ^= (uint32_t)(buf == 0);
 					}
-					if (!ok) break;
-					const int r0 = t.m0 + (warp & 3) * 32;
-					if (r0 >= M.p) continue;
+					if (++s == STAGES)
+					{
+						s = 0;
+						ph ^= 1u;
+					}
+				}
+			}
+		}
+		else
+		{
+			// ------------------------------------------------ epilogue
+			const uint32_t area = staging0 + (uint32_t)(warp - 2) * 4096u;
+			const int quarter = warp & 3, half = (warp - 2) >> 2;
+			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
+			{
+				const OrMat& M = P.mat[t.mat];
+				const OrOp& o = P.prog[M.grouped].op[t.op];
+				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
+				float acc[EC];
+#pragma unroll
+				for (int i = 0; i < EC; ++i) acc[i] = 0.0f;
+				if (t.kb0 == 0)
+				{
 #pragma unroll
 					for (int pc = 0; pc < EC / 32; ++pc)
+						if (piece_needed(M, o, r0, c00 + pc * 32))
+						{
+							add_parts(acc + pc * 32, o.w1, o.e1, M, r0 + lane, c00 + pc * 32);
+							add_parts(acc + pc * 32, o.w2, o.e2, M, r0 + lane, c00 + pc * 32);
+						}
+				}
+				for (int done = t.kb0; done < t.kb1; done += S::CHUNK)
+				{
+					if (!warp_wait(bar_acc_full + 8 * buf, aph, abort_flag, P.status, 3))
 					{
-						const int c0 = t.n0 + half * EC + pc * 32;
-						float v[32];
+						ok = false;
+						break;
+					}
+					asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+					const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * S::COLUMNS + half * EC);
+					if (S::PAIR)
+					{
 #pragma unroll
-						for (int i = 0; i < 32; ++i) v[i] = acc[pc * 32 + i] * inv;
-						if (phase == PHASE_APPLY)
+						for (int c = 0; c < EC / 32; ++c)
 						{
-							if (c0 >= M.q) continue;
-							if (!last)
-							{
-								__half* X = M.X + 2 * (cur ^ 1) * M.planex + (long long)r0 * M.ldx + c0;
-								store_rows(v, so, X, X + M.planex, M.ldx, area, lane);
-								continue;
-							}
-							const OrthoMatrix& m = M.m;
-							const float keep = 1.0f - m.lr * P.decay;
-							__syncwarp();
-							if (!M.tall)
-							{
+							uint32_t r[32];
+							tmem_ld32(taddr + (uint32_t)(BN + c * 32), r);
+							asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-								for (int j = 0; j < 32; ++j) square_put(area, lane, j, v[j]);
-								__syncwarp();
-							}
-							// row j of the piece (column j of a tall matrix's), one element per lane
-#pragma unroll
-							for (int j = 0; j < 32; ++j)
-							{
-								const int r = M.tall ? c0 + j : r0 + j, c = M.tall ? r0 + lane : c0 + lane;
-								if (r >= m.rows || c >= m.cols) continue;
-								const float o = M.tall ? v[j] : square_get(area, j, lane);
-								if (!P.step) store_typed(m.out, r * m.ld_out + c, o, P.type);
-								else
-								{
-									const long long i = r * m.ld_w + c;
-									m.w_out[i] = fmaf(-m.lr, o, keep * m.w[i]);
-								}
-							}
-							continue;
-						}
-						// a symmetric result: what lies above the diagonal is another tile's mirror image
-						if (c0 > r0) continue;
-						__half* out = M.S + (phase == PHASE_POLY ? 2 * M.planes : 0);
-						if (phase == PHASE_POLY)
-						{
-							const float b = P.coef[step][1], c = P.coef[step][2], ia = pow2f(-P.ea[step]);
-							const __half* A = M.S + (long long)(r0 + lane) * M.lds + c0;
-#pragma unroll
-							for (int k = 0; k < 4; ++k)
-							{
-								const uint4 h4 = *reinterpret_cast<const uint4*>(A + 8 * k);
-								const uint4 l4 = *reinterpret_cast<const uint4*>(A + M.planes + 8 * k);
-								const __half2* h = reinterpret_cast<const __half2*>(&h4);
-								const __half2* l = reinterpret_cast<const __half2*>(&l4);
-#pragma unroll
-								for (int i = 0; i < 4; ++i)
-								{
-									const float2 x = __half22float2(h[i]), y = __half22float2(l[i]);
-									v[8 * k + 2 * i] = fmaf(c, v[8 * k + 2 * i], b * ((x.x + y.x) * ia));
-									v[8 * k + 2 * i + 1] = fmaf(c, v[8 * k + 2 * i + 1], b * ((x.y + y.y) * ia));
-								}
-							}
-						}
-						if (c0 == r0)
-						{
-							// on the diagonal: the upper half becomes the lower half's mirror image
-							__syncwarp();
-#pragma unroll
-							for (int j = 0; j < 32; ++j) square_put(area, lane, j, v[j]);
-							__syncwarp();
-#pragma unroll
-							for (int j = 0; j < 32; ++j)
-							{
-								if (j > lane) v[j] = square_get(area, j, lane);
-								if (j == lane && phase == PHASE_POLY) v[j] += P.coef[step][0];
-							}
-						}
-						__half* D = out + (long long)r0 * M.lds + c0;
-						store_rows(v, so, D, D + M.planes, M.lds, area, lane);
-						if (c0 != r0)
-						{
-							__half* T = out + (long long)c0 * M.lds + r0;
-							store_columns(v, so, T, T + M.planes, M.lds, lane);
+							for (int e = 0; e < 32; ++e) acc[c * 32 + e] += __uint_as_float(r[e]);
 						}
 					}
+#pragma unroll
+					for (int c = 0; c < EC / 32; ++c)
+					{
+						uint32_t r[32];
+						tmem_ld32(taddr + (uint32_t)(c * 32), r);
+						asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+						for (int e = 0; e < 32; ++e) acc[c * 32 + e] += __uint_as_float(r[e]);
+					}
+					asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+					__syncwarp();
+					if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_acc_empty + 8 * buf) : "memory");
+					buf ^= 1;
+					aph ^= (uint32_t)(buf == 0);
+				}
+				if (!ok) break;
+#pragma unroll
+				for (int pc = 0; pc < EC / 32; ++pc)
+				{
+					const int c0 = c00 + pc * 32;
+					if (!piece_needed(M, o, r0, c0)) continue;
+					if (t.split > 1)
+					{
+						float4* d = P.part + ((long long)t.slot * S::PIECES + quarter * (BN / 32) + half * (EC / 32) + pc) * 256 + lane;
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+							d[j * 32] = make_float4(acc[pc * 32 + 4 * j], acc[pc * 32 + 4 * j + 1], acc[pc * 32 + 4 * j + 2], acc[pc * 32 + 4 * j + 3]);
+						continue;
+					}
+					float v[32];
+#pragma unroll
+					for (int i = 0; i < 32; ++i) v[i] = acc[pc * 32 + i];
+					finish_piece(P, M, o, v, r0, c0, area, lane);
+				}
+			}
+			asm volatile("fence.proxy.async;" ::: "memory");
+		}
+		if (P.reduce >> round & 1)
+		{
+			grid.sync();
+			if (warp >= 2)
+			{
+				const uint32_t area = staging0 + (uint32_t)(warp - 2) * 4096u;
+				const int warps = (int)gridDim.x * S::EPI_WARPS;
+				// (neighbouring pieces on different SMs)
+				for (int k = (warp - 2) * (int)gridDim.x + (int)blockIdx.x; find_split<BN>(P, round, k / S::PIECES, t); k += warps)
+				{
+					const OrMat& M = P.mat[t.mat];
+					const OrOp& o = P.prog[M.grouped].op[t.op];
+					const int pc = k % S::PIECES;
+					const int r0 = t.m0 + pc / (BN / 32) * 32, c0 = t.n0 + pc % (BN / 32) * 32;
+					if (!piece_needed(M, o, r0, c0)) continue;
+					float v[32];
+					const float4* d = P.part + ((long long)t.slot * S::PIECES + pc) * 256 + lane;
+#pragma unroll
+					for (int j = 0; j < 8; ++j)
+					{
+						const float4 x = d[j * 32];
+						v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+					}
+#pragma unroll 2
+					for (int part = 1; part < t.split; ++part)
+					{
+						d += S::PIECES * 256;
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+						{
+							const float4 x = d[j * 32];
+							v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+						}
+					}
+					finish_piece(P, M, o, v, r0, c0, area, lane);
 				}
 				asm volatile("fence.proxy.async;" ::: "memory");
 			}
-			if (!(phase == PHASE_APPLY && step == P.steps - 1)) grid.sync();
 		}
+		if (round + 1 < P.rounds) grid.sync();
 	}
 	if (*abort_flag)
 	{
@@ -619,111 +923,41 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	if (warp == 1)
 	{
 		asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN) : "memory");
+		asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * S::COLUMNS) : "memory");
 	}
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
 constexpr size_t OR_HEADER = 256;  // status word
-constexpr int OR_SMS = 148;
-constexpr size_t OR_PART = (size_t)ORTHO_MAX_MATRICES * OR_SMS * sizeof(double);
+constexpr size_t OR_SUMS = (size_t)ORTHO_MAX_MATRICES * OR_SMS * sizeof(double);
 size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 
-size_t matrix_bytes(int rows, int cols)
+struct Bounds
 {
-	const size_t p = round_up((size_t)std::min(rows, cols), 128), q = round_up((size_t)std::max(rows, cols), 128);
-	return (4 * p * q + 4 * p * p) * sizeof(__half);
-}
-
-// 2^e * bound < 2^15
-int exponent_for(double bound)
+	double sx[ORTHO_MAX_STEPS + 1];  // singular values of X before a step
+	double sa[ORTHO_MAX_STEPS];      // eigenvalues of A,
+	double sr[ORTHO_MAX_STEPS];      // of R = b A + c A^2,
+	double sp[ORTHO_MAX_STEPS];      // of a + R
+};
+// The largest singular value that a step may find follows from the extrema of its polynomial on [0, largest].
+bool bounds_of(const float (*coef)[3], int steps, Bounds& o)
 {
-	int e = 0;
-	frexp(bound, &e);  // bound < 2^e
-	return std::min(15 - e, 40);
-}
-
-template <int BN>
-bool make_maps(OrMaps& o, const OrMat& M)
-{
-	auto map3 = [&](CUtensorMap* m, const __half* base, long long rows, long long cols, long long ld, long long plane, int box_rows) {
-		return tc_make_parts_map(m, base, rows, cols, ld, plane, 4, OR_BK, box_rows);
-	};
-	return map3(&o.xa, M.X, M.p, M.q, M.ldx, M.planex, TC_BM) && map3(&o.xb, M.X, M.p, M.q, M.ldx, M.planex, BN) &&
-	       tc_make_parts_map_mn(&o.xn, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, BN) &&
-	       map3(&o.sa, M.S, M.p, M.p, M.lds, M.planes, TC_BM) && map3(&o.sb, M.S, M.p, M.p, M.lds, M.planes, BN);
-}
-
-// About how many clocks the products take: for each phase the CTA with the most work.  A k-block's six MMAs cost 768 clocks
-// on 256 columns, 400 on 128 and 300 on 64 (where reading A from shared memory bounds them), a tile about 2500 more.
-long long estimate(const OrParams& P, int bn)
-{
-	const long long per = bn == 256 ? 768 : (bn == 128 ? 400 : 300);
-	long long total = 0;
-	for (int phase = 0; phase < 3; ++phase)
-	{
-		long long load[OR_SMS] = {0}, worst = 0;
-		int t = 0;
-		for (int i = 0; i < P.count; ++i)
-		{
-			const int n = phase_tiles(P.mat[i].p, P.mat[i].q, phase, bn);
-			const long long kb = ((phase == PHASE_GRAM ? P.mat[i].q : P.mat[i].p) + OR_BK - 1) / OR_BK;
-			// (whole rounds at once, the rest one by one)
-			const long long rounds = n / OR_SMS;
-			for (int c = 0; c < OR_SMS && rounds; ++c) load[c] += rounds * (kb * per + 2500);
-			for (int k = 0; k < n % OR_SMS; ++k) load[(t + k) % OR_SMS] += kb * per + 2500;
-			t = (t + n) % OR_SMS;
-		}
-		for (long long l : load) worst = std::max(worst, l);
-		total += worst;
-	}
-	return total;
-}
-
-template <int BN>
-cudaError_t launch_width(OrParams& P, int grid_most, cudaStream_t s)
-{
-	for (int i = 0; i < P.count; ++i)
-		if (!make_maps<BN>(P.maps[i], P.mat[i])) return cudaErrorInvalidValue;
-	int sms = 0;
-	cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(ortho_kernel<BN>), OrSmem<BN>::TOTAL, &sms);
-	if (e != cudaSuccess) return e;
-	int most = 1;
-	for (int phase = 0; phase < 3; ++phase)
-	{
-		int n = 0;
-		for (int i = 0; i < P.count; ++i) n += phase_tiles(P.mat[i].p, P.mat[i].q, phase, BN);
-		most = std::max(most, n);
-	}
-	most = std::max(most, P.units);
-	int grid = std::min(std::min(sms, grid_most), most);
-	cudaLaunchConfig_t cfg = {};
-	cfg.gridDim = dim3((unsigned)grid);
-	cfg.blockDim = dim3(OrSmem<BN>::THREADS);
-	cfg.dynamicSmemBytes = OrSmem<BN>::TOTAL;
-	cfg.stream = s;
-	cudaLaunchAttribute at[1];
-	at[0].id = cudaLaunchAttributeCooperative;
-	at[0].val.cooperative = 1;
-	cfg.attrs = at;
-	cfg.numAttrs = 1;
-	return cudaLaunchKernelEx(&cfg, ortho_kernel<BN>, (const OrParams)P);
-}
-
-}  // namespace
-
-bool ortho_bounds(const float (*coef)[3], int steps, double* sx, double* sa, double* sp)
-{
-	// the largest singular value that a step may find, by the extrema of the step's polynomial on [0, largest]
-	sx[0] = 1.0 + 1e-5;  // (the norm's rounding)
+	o.sx[0] = 1.0 + 1e-5;  // (the norm's rounding)
 	for (int k = 0; k < steps; ++k)
 	{
-		const double a = coef[k][0], b = coef[k][1], c = coef[k][2], t = sx[k];
+		const double a = coef[k][0], b = coef[k][1], c = coef[k][2], t = o.sx[k];
 		if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-		sa[k] = t * t * (1.0 + 1e-5);
-		auto h = [&](double l) { return fabs(a + l * (b + l * c)); };  // P's eigenvalue for A's eigenvalue l
-		sp[k] = std::max(h(0.0), h(sa[k]));
-		if (c != 0.0 && -b / (2 * c) > 0.0 && -b / (2 * c) < sa[k]) sp[k] = std::max(sp[k], h(-b / (2 * c)));
+		o.sa[k] = t * t * (1.0 + 1e-5);
+		auto h = [&](double l) { return fabs(a + l * (b + l * c)); };
+		auto e = [&](double l) { return fabs(l * (b + l * c)); };
+		o.sr[k] = e(o.sa[k]);
+		o.sp[k] = std::max(h(0.0), h(o.sa[k]));
+		const double turn = c != 0.0 ? -b / (2 * c) : -1.0;
+		if (turn > 0.0 && turn < o.sa[k])
+		{
+			o.sr[k] = std::max(o.sr[k], e(turn));
+			o.sp[k] = std::max(o.sp[k], h(turn));
+		}
 		double most = h(t * t) * t;
 		// a + 3 b l + 5 c l^2 = 0 with l = s^2
 		double roots[2];
@@ -740,84 +974,367 @@ bool ortho_bounds(const float (*coef)[3], int steps, double* sx, double* sa, dou
 		else if (b != 0.0) roots[n++] = -a / (3 * b);
 		for (int i = 0; i < n; ++i)
 			if (roots[i] > 0.0 && roots[i] < t * t) most = std::max(most, h(roots[i]) * sqrt(roots[i]));
-		sx[k + 1] = most * (1.0 + 1e-4);
-		if (!(sx[k + 1] <= 16.0) || !(sp[k] <= 256.0)) return false;
+		o.sx[k + 1] = most * (1.0 + 1e-4);
+		if (!(o.sx[k + 1] <= 16.0) || !(o.sr[k] <= 256.0) || !(o.sp[k] <= 256.0)) return false;
 	}
 	return true;
 }
 
+// 2^e with 2^e * bound < 2^15
+float scale_under(double bound)
+{
+	int e = 0;
+	frexp(bound, &e);  // bound < 2^e
+	return ldexpf(1.0f, std::max(-40, std::min(15 - e, 40)));
+}
+
+// Steps of the groups.  A group multiplies what its A's rounding does to a small singular value by the product of its steps'
+// slopes at zero: up to 64 in the first group, whose A has elements of about 1/p, up to 16 later (the usual coefficients, 3.4445:
+// groups of three, two, two, ..).
+int groups_of(const float (*coef)[3], int steps, int* size)
+{
+	int n = 0;
+	for (int k = 0; k < steps; ++n)
+	{
+		double growth = std::max(1.0, (double)fabsf(coef[k][0]));
+		size[n] = 1;
+		for (++k; k < steps && size[n] < 3; ++k, ++size[n])
+		{
+			growth *= std::max(1.0, (double)fabsf(coef[k][0]));
+			if (growth > (n == 0 ? 64.0 : 16.0)) break;
+		}
+	}
+	return n;
+}
+
+void make_program(OrProgram& g, const float (*coef)[3], const Bounds& b, const int* size, int groups)
+{
+	bool alone = true;
+	for (int i = 0; i < groups; ++i) alone = alone && size[i] == 1;
+	const int T = 1, R0 = alone ? 1 : 2, Q0 = 4;
+	g.count = 0;
+	g.planes = alone ? 2 : OR_PLANES;
+	float scale[ID_X + 2] = {0};  // of the matrices' present contents
+	scale[ID_X] = scale_under(b.sx[0]);
+	int round = 0, k = 0, x = 0;
+	// out = f A B + w1 E1 + w2 E2
+	auto op = [&](int a, int bb, double f, int e1, double w1, int e2, double w2, int out, double bound) {
+		OrOp& o = g.op[g.count++];
+		o.a = (signed char)a; o.b = (signed char)bb; o.e1 = (signed char)e1; o.e2 = (signed char)e2; o.out = (signed char)out;
+		o.round = (signed char)round;
+		// (a factor of zero: so small a one that nothing of the product is left beside w1 E1)
+		const double factor = (fabs(f) < 0x1p-40 ? 0x1p-40 : f) / scale[a] / scale[bb];
+		o.f = (float)factor;
+		o.w1 = e1 == ID_NONE ? 0.0f : (float)(w1 / scale[e1] / factor);
+		o.w2 = e2 == ID_NONE ? 0.0f : (float)(w2 / scale[e2] / factor);
+		o.so = out == ID_NONE ? 1.0f : scale_under(bound);
+	};
+	for (int i = 0; i < groups; ++i)
+	{
+		op(ID_X + x, ID_X + x, 1.0, ID_NONE, 0, ID_NONE, 0, ID_A, b.sa[k]);
+		scale[ID_A] = g.op[g.count - 1].so;
+		++round;
+		int Q = ID_NONE;
+		double q = 1.0, qbound = 1.0;
+		for (int j = 0; j < size[i]; ++j, ++k)
+		{
+			const double a = coef[k][0];
+			const bool more = j + 1 < size[i];
+			const int R = alone ? R0 : R0 + (j & 1);
+			op(ID_A, ID_A, coef[k][2], ID_A, coef[k][1], ID_NONE, 0, R, b.sr[k]);
+			scale[R] = g.op[g.count - 1].so;
+			++round;
+			qbound *= b.sp[k];
+			int next = R;
+			float next_scale = scale[R];
+			if (j > 0)
+			{
+				next = Q == Q0 ? Q0 + 1 : Q0;
+				op(R, Q, 1.0, Q, a, R, q, next, qbound + fabs(q * a));
+				next_scale = g.op[g.count - 1].so;
+			}
+			float t_scale = 0.0f;
+			if (more)
+			{
+				op(R, ID_A, 1.0, ID_A, a, ID_NONE, 0, T, b.sa[k] * b.sp[k]);
+				t_scale = g.op[g.count - 1].so;
+			}
+			if (j > 0 || more) ++round;
+			scale[next] = next_scale;
+			Q = next;
+			q = j > 0 ? q * a : a;
+			if (more)
+			{
+				scale[T] = t_scale;
+				op(T, R, 1.0, T, a, ID_NONE, 0, ID_A, b.sa[k + 1]);
+				scale[ID_A] = g.op[g.count - 1].so;
+				++round;
+			}
+		}
+		op(Q, ID_X + x, 1.0, ID_X + x, q, ID_NONE, 0, i + 1 < groups ? ID_X + (x ^ 1) : ID_NONE, b.sx[k]);
+		scale[ID_X + (x ^ 1)] = g.op[g.count - 1].so;
+		x ^= 1;
+		++round;
+	}
+	g.rounds = round;
+	int at = 0;
+	for (int r = 0; r <= OR_MAX_ROUNDS; ++r)
+	{
+		while (at < g.count && g.op[at].round < r) ++at;
+		g.first[r] = (unsigned char)at;
+	}
+}
+
+// A launch's plan: programs, which matrix takes which, the width of the tiles, how far tiles are split.
+struct Plan
+{
+	int bn;
+	int slots;  // of split tiles' parts
+};
+
+// About how many clocks an item of kb stages costs: a stage's six MMAs and what surrounds them, then draining and storing.
+long long item_clocks(int bn, long long kb) { return kb * (bn == 256 ? 960 : (bn == 128 ? 520 : 400)) + 4000; }
+constexpr long long ROUND_CLOCKS = 9000;   // a round's barrier, first copies, last stores
+constexpr long long REDUCE_CLOCKS = 6000;  // the further barrier and the sums of a round with split tiles
+
+// The splits of tiles of width bn, and about how many clocks the rounds take: for each the CTA with the most work.
+long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OPS], unsigned long long* reduce, int* slots)
+{
+	long long total = 0;
+	*reduce = 0;
+	*slots = 0;
+	for (int round = 0; round < P.rounds; ++round)
+	{
+		int tiles = 0;
+		long long work = 0;
+		auto each = [&](auto&& f) {
+			for (int i = 0; i < P.count; ++i)
+			{
+				const OrProgram& g = P.prog[P.mat[i].grouped];
+				for (int k = g.first[round]; k < g.first[round + 1]; ++k) f(i, k, op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, bn), op_kb(g.op[k], P.mat[i].p, P.mat[i].q));
+			}
+		};
+		each([&](int, int, int n, int kb) {
+			tiles += n;
+			work += (long long)n * kb;
+		});
+		// Parts of about equal length for all operations, so many that every SM has one; a tile that is shorter stays whole.
+		const long long share = std::max<long long>(OR_SPLIT_KB, (work + OR_SMS - 1) / OR_SMS);
+		long long load[OR_SMS] = {0}, worst = 0;
+		int t = 0, used = 0;
+		each([&](int i, int k, int n, int kb) {
+			int s = tiles * 2 <= OR_SMS ? (int)std::min<long long>(255, kb / share) : 1;
+			if (s < 1) s = 1;
+			split[i][k] = (unsigned char)s;
+			if (s > 1) used += n * s;
+			const long long each_kb = (kb + s - 1) / s;
+			const long long rounds = (long long)n * s / OR_SMS;
+			for (int c = 0; c < OR_SMS && rounds; ++c) load[c] += rounds * item_clocks(bn, each_kb);
+			const int rest = (int)((long long)n * s % OR_SMS);
+			for (int c = 0; c < rest; ++c) load[(t + c) % OR_SMS] += item_clocks(bn, each_kb);
+			t = (t + rest) % OR_SMS;
+		});
+		for (long long l : load) worst = std::max(worst, l);
+		total += worst + ROUND_CLOCKS;
+		if (used)
+		{
+			*reduce |= 1ull << round;
+			total += REDUCE_CLOCKS;
+		}
+		*slots = std::max(*slots, used);
+	}
+	return total;
+}
+
+// Grouped steps save multiply-adds (of matrices that are not nearly square) and cost rounds.
+bool may_group(int p, int q) { return q > p + p / 16; }  // (a group's six p x p matrices instead of two)
+bool worth_grouping(const OrProgram* prog, int p, int q)
+{
+	if (!may_group(p, q)) return false;
+	double clocks[2];
+	for (int v = 0; v < 2; ++v)
+	{
+		double work = 0.0;
+		for (int k = 0; k < prog[v].count; ++k) work += (double)op_tiles(prog[v].op[k], p, q, 128) * op_kb(prog[v].op[k], p, q);
+		clocks[v] = work * 520 / OR_SMS + (double)prog[v].rounds * ROUND_CLOCKS;
+	}
+	return clocks[1] < clocks[0];
+}
+
+size_t matrix_bytes(const OrMat& M, int planes)
+{
+	const size_t p = round_up((size_t)M.p, 128), q = round_up((size_t)M.q, 128);
+	return (4 * p * q + 2 * planes * p * p) * sizeof(__half);
+}
+
+// Fills everything of P that does not depend on the workspace's address; returns the bytes of workspace.
+size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int count, Plan& plan)
+{
+	memset(&P, 0, sizeof P);
+	P.count = count;
+	P.type = a.type;
+	P.step = a.step;
+	P.nesterov = a.nesterov;
+	P.mu = a.mu;
+	P.decay = a.decay;
+	P.eps = a.eps;
+	Bounds b;
+	bounds_of(a.coef, a.steps, b);
+	P.s0 = scale_under(b.sx[0]);
+	int size[ORTHO_MAX_STEPS];
+	for (int k = 0; k < a.steps; ++k) size[k] = 1;
+	make_program(P.prog[0], a.coef, b, size, a.steps);
+	const int groups = groups_of(a.coef, a.steps, size);
+	make_program(P.prog[1], a.coef, b, size, groups);
+	for (int i = 0; i < count; ++i)
+	{
+		OrMat& M = P.mat[i];
+		M.m = m[i];
+		M.tall = M.m.rows > M.m.cols;
+		M.p = std::min(M.m.rows, M.m.cols);
+		M.q = std::max(M.m.rows, M.m.cols);
+		M.grouped = groups < a.steps && worth_grouping(P.prog, M.p, M.q);
+	}
+	// the matrices with the longest products first: what is left for the last CTAs of a round is small
+	std::stable_sort(P.mat, P.mat + count, [](const OrMat& x, const OrMat& y) { return (double)x.p * x.q > (double)y.p * y.q; });
+	size_t bytes = 0;
+	for (int i = 0; i < count; ++i)
+	{
+		OrMat& M = P.mat[i];
+		const OrProgram& g = P.prog[M.grouped];
+		P.rounds = std::max(P.rounds, g.rounds);
+		M.ldx = (long long)round_up(M.q, 128);
+		M.planex = M.ldx * (long long)round_up(M.p, 128);
+		M.lds = (long long)round_up(M.p, 128);
+		M.planes = M.lds * M.lds;
+		M.units = P.units;
+		M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
+		P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
+		bytes += matrix_bytes(M, g.planes);
+	}
+	long long best = -1;
+	for (int bn : {256, 128, 64})
+	{
+		static thread_local unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
+		unsigned long long reduce;
+		int slots;
+		const long long c = plan_width(P, bn, split, &reduce, &slots);
+		if (best >= 0 && c >= best) continue;
+		best = c;
+		plan.bn = bn;
+		plan.slots = slots;
+		P.reduce = reduce;
+		memcpy(P.split, split, sizeof split);
+	}
+	return OR_HEADER + round_up(OR_SUMS, 256) + (size_t)plan.slots * 128 * plan.bn * sizeof(float) + bytes;
+}
+
+template <int BN>
+bool make_maps(OrMaps& o, const OrMat& M, int planes)
+{
+	return tc_make_parts_map(&o.xa, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, TC_BM) &&
+	       tc_make_parts_map(&o.xb, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, BN) &&
+	       tc_make_parts_map_mn(&o.xn, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, BN) &&
+	       tc_make_parts_map(&o.sa, M.S, M.p, M.p, M.lds, M.planes, 2 * planes, OR_BK, TC_BM) &&
+	       tc_make_parts_map(&o.sb, M.S, M.p, M.p, M.lds, M.planes, 2 * planes, OR_BK, BN);
+}
+
+template <int BN>
+cudaError_t launch_width(OrParams& P, cudaStream_t s)
+{
+	for (int i = 0; i < P.count; ++i)
+		if (!make_maps<BN>(P.maps[i], P.mat[i], P.prog[P.mat[i].grouped].planes)) return cudaErrorInvalidValue;
+	int sms = 0;
+	cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(ortho_kernel<BN>), OrSmem<BN>::TOTAL, &sms);
+	if (e != cudaSuccess) return e;
+	// no more CTAs than the largest round has items and pieces
+	int most = P.units;
+	for (int round = 0; round < P.rounds; ++round)
+	{
+		int n = 0, pieces = 0;
+		for (int i = 0; i < P.count; ++i)
+		{
+			const OrProgram& g = P.prog[P.mat[i].grouped];
+			for (int k = g.first[round]; k < g.first[round + 1]; ++k)
+			{
+				const int tiles = op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, BN);
+				n += tiles * P.split[i][k];
+				if (P.split[i][k] > 1) pieces += tiles * OrSmem<BN>::PIECES;
+			}
+		}
+		most = std::max(most, std::max(n, pieces));
+	}
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = dim3((unsigned)std::min(std::min(sms, OR_SMS), most));
+	cfg.blockDim = dim3(OrSmem<BN>::THREADS);
+	cfg.dynamicSmemBytes = OrSmem<BN>::TOTAL;
+	cfg.stream = s;
+	cudaLaunchAttribute at[1];
+	at[0].id = cudaLaunchAttributeCooperative;
+	at[0].val.cooperative = 1;
+	cfg.attrs = at;
+	cfg.numAttrs = 1;
+	return cudaLaunchKernelEx(&cfg, ortho_kernel<BN>, (const OrParams)P);
+}
+
+thread_local OrParams t_params;
+
+}  // namespace
+
+bool ortho_coefficients_ok(const float (*coef)[3], int steps)
+{
+	Bounds b;
+	return bounds_of(coef, steps, b);
+}
+
+// (whatever the steps, the coefficients and the plan that they lead to)
 size_t ortho_workspace_bytes(const OrthoMatrix* m, int count)
 {
 	size_t most = 0;
 	for (int first = 0; first < count; first += ORTHO_MAX_MATRICES)
 	{
-		size_t b = 0;
-		for (int i = first; i < std::min(count, first + ORTHO_MAX_MATRICES); ++i) b += matrix_bytes(m[i].rows, m[i].cols);
-		most = std::max(most, b);
+		size_t bytes = 0;
+		double parts = 0.0;  // of split tiles, at most one per SM
+		for (int i = first; i < std::min(count, first + ORTHO_MAX_MATRICES); ++i)
+		{
+			OrMat M;
+			M.p = std::min(m[i].rows, m[i].cols);
+			M.q = std::max(m[i].rows, m[i].cols);
+			bytes += matrix_bytes(M, may_group(M.p, M.q) ? OR_PLANES : 2);
+			const double kb = ceil(M.q / (double)OR_BK);
+			if (kb >= 2 * OR_SPLIT_KB) parts += 2 * ceil(M.p / 128.0) * ceil(M.q / 64.0) * kb / OR_SPLIT_KB;
+		}
+		most = std::max(most, bytes + (size_t)std::min(parts, (double)OR_SMS) * 128 * 256 * sizeof(float));
 	}
-	return 256 + OR_HEADER + round_up(OR_PART, 256) + most;  // (256: the caller's pointer need not be aligned)
+	return 256 + OR_HEADER + round_up(OR_SUMS, 256) + most;  // (256: the caller's pointer need not be aligned)
 }
 
 int* ortho_status(void* work) { return reinterpret_cast<int*>(round_up((size_t)work, 256)); }
 
-cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, cudaStream_t s)
+cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_bytes, cudaStream_t s)
 {
-	char* w = reinterpret_cast<char*>(ortho_status(work));
-	double sx[ORTHO_MAX_STEPS + 1], sa[ORTHO_MAX_STEPS], sp[ORTHO_MAX_STEPS];
-	if (!ortho_bounds(a.coef, a.steps, sx, sa, sp)) return cudaErrorInvalidValue;
+	OrParams& P = t_params;
 	for (int first = 0; first < a.count; first += ORTHO_MAX_MATRICES)
 	{
-		static thread_local OrParams P;
-		memset(&P, 0, sizeof P);
-		P.count = std::min(ORTHO_MAX_MATRICES, a.count - first);
-		P.steps = a.steps;
-		P.type = a.type;
-		P.step = a.step;
-		P.nesterov = a.nesterov;
-		P.mu = a.mu;
-		P.decay = a.decay;
-		P.eps = a.eps;
-		P.reset = first == 0;
-		P.status = a.status ? a.status : reinterpret_cast<int*>(w);
-		if (a.status) P.reset = 0;
-		P.part = reinterpret_cast<double*>(w + OR_HEADER);
-		for (int k = 0; k < a.steps; ++k)
-		{
-			for (int j = 0; j < 3; ++j) P.coef[k][j] = a.coef[k][j];
-			P.ea[k] = exponent_for(sa[k]);
-			P.ep[k] = exponent_for(sp[k]);
-		}
-		for (int k = 0; k <= a.steps; ++k) P.ex[k] = exponent_for(sx[k]);
-		char* at = w + OR_HEADER + round_up(OR_PART, 256);
+		Plan plan;
+		const size_t need = make_plan(P, a, a.mat + first, std::min(ORTHO_MAX_MATRICES, a.count - first), plan);
+		if (need + 256 > work_bytes) return cudaErrorInvalidValue;
+		char* at = reinterpret_cast<char*>(ortho_status(work));
+		P.status = a.status ? a.status : reinterpret_cast<int*>(at);
+		P.reset = first == 0 && !a.status;
+		at += OR_HEADER;
+		P.sums = reinterpret_cast<double*>(at);
+		at += round_up(OR_SUMS, 256);
+		P.part = reinterpret_cast<float4*>(at);
+		at += (size_t)plan.slots * 128 * plan.bn * sizeof(float);
 		for (int i = 0; i < P.count; ++i)
 		{
 			OrMat& M = P.mat[i];
-			M.m = a.mat[first + i];
-			M.tall = M.m.rows > M.m.cols;
-			M.p = std::min(M.m.rows, M.m.cols);
-			M.q = std::max(M.m.rows, M.m.cols);
-		}
-		// the matrices with the longest products first: what is left for the last CTAs of a phase is small
-		std::stable_sort(P.mat, P.mat + P.count, [](const OrMat& x, const OrMat& y) { return (double)x.p * x.q > (double)y.p * y.q; });
-		for (int i = 0; i < P.count; ++i)
-		{
-			OrMat& M = P.mat[i];
-			M.ldx = (long long)round_up(M.q, 128);
-			M.planex = M.ldx * (long long)round_up(M.p, 128);
-			M.lds = (long long)round_up(M.p, 128);
-			M.planes = M.lds * M.lds;
 			M.X = reinterpret_cast<__half*>(at);
 			M.S = M.X + 4 * M.planex;
-			at += matrix_bytes(M.m.rows, M.m.cols);
-			M.units = P.units;
-			M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
-			P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
+			at += matrix_bytes(M, P.prog[M.grouped].planes);
 		}
-		const long long c64 = estimate(P, 64), c128 = estimate(P, 128), c256 = estimate(P, 256);
-		cudaError_t e;
-		if (c256 <= c128 && c256 <= c64) e = launch_width<256>(P, OR_SMS, s);
-		else if (c128 <= c64) e = launch_width<128>(P, OR_SMS, s);
-		else e = launch_width<64>(P, OR_SMS, s);
+		const cudaError_t e = plan.bn == 256 ? launch_width<256>(P, s) : (plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s));
 		if (e != cudaSuccess) return e;
 	}
 	return cudaSuccess;

@@ -32,11 +32,11 @@ struct OrthoArgs
 	float coef[ORTHO_MAX_STEPS][3];
 	int* status;  // device word that a wait that runs out raises, or NULL: the workspace's
 };
-// Bounds on the singular values of X before every step (steps + 1), and on the eigenvalues of A and P; false where the
-// coefficients let them leave the range that the fp16 parts are scaled for.
-bool ortho_bounds(const float (*coef)[3], int steps, double* sx, double* sa, double* sp);
-size_t ortho_workspace_bytes(const OrthoMatrix* m, int count);
+// false where the coefficients let a singular value of [0, 1] (or an eigenvalue on the way) leave the range that the parts are
+// scaled for
+bool ortho_coefficients_ok(const float (*coef)[3], int steps);
+size_t ortho_workspace_bytes(const OrthoMatrix* m, int count);  // (only the shapes are looked at)
 int* ortho_status(void* work);  // where a workspace keeps its status word
-cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, cudaStream_t s);
+cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_bytes, cudaStream_t s);
 
 }  // namespace glb
