@@ -15,9 +15,10 @@
 // gemm_tcgen05.cu; unlike there the scales are known beforehand -- all singular values stay below a bound that follows from
 // the coefficients alone -- so no product waits for a largest element, and lo is not scaled (its error floor is 2^-25 of a unit,
 // 2^-38 of the largest element): tensor memory holds two accumulators of a tile, and the MMAs of one chunk run while the
-// chunk in front is drained.  On tiles of at most 128 columns hi and lo of the second operand lie one behind the other in
-// shared memory and are one operand of twice the columns, [hi*hi | hi*lo]: two MMAs instead of three, an accumulator for
-// each half, fewer reads of shared memory.  On 256 columns, which no longer fit so, the three products share one.
+// chunk in front is drained.  hi and lo of the second operand lie one behind the other in shared memory and are one operand of
+// twice the columns, [hi*hi | hi*lo], an accumulator for each half: two MMAs per 16 k instead of three, fewer reads of shared memory.
+// (Tiles of 256 columns, which only fit with one accumulator for all three products, lost: their epilogue holds 128 sums per
+// thread, spills, and the MMAs wait for it.  4096 x 4096, a step: 769 us against 655.)
 // a X (b A, a T, ..) is where the epilogue's registers start from, loaded while the first chunk is computed: inside the accumulator
 // it would be truncated with every addition, which doubles the error of the result (3.3e-6 against 1.3e-6 of a 256 x 256
 // matrix, fp32 products: 2.5e-6).
@@ -42,10 +43,12 @@ namespace glb {
 using namespace tc;
 namespace {
 
-constexpr int OR_BK = 32;      // k per pipeline stage
+// k per pipeline stage.  A stage costs the multiplying warp two waits and a commit, about 350 clocks, whatever its MMAs take: with
+// stages of 32 k that bounded both tiles (530 clocks per 32 k on 128 columns, 350 to 400 now).
+constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_SMS = 148;
-constexpr int OR_SPLIT_KB = 4; // stages that a part of a split tile has at least
+constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 constexpr int OR_MAX_OPS = 4 * ORTHO_MAX_STEPS;
 constexpr int OR_MAX_ROUNDS = 64;  // at most 55 are needed: step by step three per step, in groups of n 3 n + 1
 constexpr int OR_PLANES = 6;   // p x p matrices of a grouped program
@@ -53,15 +56,15 @@ constexpr int OR_PLANES = 6;   // p x p matrices of a grouped program
 template <int BN>
 struct OrSmem
 {
-	static constexpr bool PAIR = BN <= 128;                  // hi and lo of B as one operand of 2 * BN columns
 	// Stages whose products an accumulator takes before it is drained: the tensor core truncates as it adds, so a chain of n
-	// additions drifts by up to n * 2^-24 towards zero; 12 (4) stages are 24 additions of full size.
-	static constexpr int CHUNK = PAIR ? 12 : 4;
-	static constexpr int COLUMNS = PAIR ? 2 * BN : BN;       // of an accumulator
-	static constexpr int STAGES = BN == 256 ? 4 : (BN == 128 ? 6 : 8);
-	static constexpr int EC = BN < 128 ? BN : 128;           // columns per epilogue warp
-	static constexpr int EPI_WARPS = 4 * (BN / EC);
-	static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+	// additions drifts by up to n * 2^-24 towards zero; 6 stages are 24 additions of full size.
+	static constexpr int CHUNK = 6;
+	static constexpr int COLUMNS = 2 * BN;                   // of an accumulator
+	static constexpr int STAGES = BN == 128 ? 3 : 4;
+	static constexpr int EC = BN / 2;                        // columns per epilogue warp
+	static constexpr int EPI_WARPS = 8;
+	static constexpr int FIRST = 4;                          // epilogue warps 4 ..; 0 copies, 1 multiplies, 2 and 3 help with elementwise work
+	static constexpr int THREADS = 32 * (FIRST + EPI_WARPS);
 	static constexpr int A_BYTES = TC_BM * OR_BK * 2;
 	static constexpr int B_BYTES = BN * OR_BK * 2;
 	static constexpr int STAGE_BYTES = 2 * A_BYTES + 2 * B_BYTES;
@@ -109,6 +112,7 @@ struct OrParams
 	OrProgram prog[2];      // step by step; in groups
 	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
 	unsigned long long reduce;  // rounds with split tiles
+	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
 	int count, rounds, units;
 	int type, step, nesterov, reset;
 	float mu, decay, eps, s0;  // s0: X_0's scale
@@ -164,12 +168,12 @@ __device__ __forceinline__ void tile_origin(const OrOp& o, int p, int q, int t, 
 		t -= n;
 	}
 }
-// item t of a round, or false
+// item t < P.items[round] of a round
 template <int BN>
-__device__ __forceinline__ bool find_item(const OrParams& P, int round, int t, OrItem& it)
+__device__ __forceinline__ void find_item(const OrParams& P, int round, int t, OrItem& it)
 {
 	int slot = 0;
-	for (int i = 0; i < P.count; ++i)
+	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
 		const OrProgram& g = P.prog[M.grouped];
@@ -188,20 +192,19 @@ __device__ __forceinline__ bool find_item(const OrParams& P, int round, int t, O
 				it.kb1 = kb * (part + 1) / s;
 				it.slot = slot + t;
 				tile_origin<BN>(g.op[k], M.p, M.q, tile, it.m0, it.n0);
-				return true;
+				return;
 			}
 			t -= n;
 			if (s > 1) slot += n;
 		}
 	}
-	return false;
 }
-// tile t of a round's split operations, or false
+// tile t < P.splits[round] of a round's split operations
 template <int BN>
-__device__ __forceinline__ bool find_split(const OrParams& P, int round, int t, OrItem& it)
+__device__ __forceinline__ void find_split(const OrParams& P, int round, int t, OrItem& it)
 {
 	int slot = 0;
-	for (int i = 0; i < P.count; ++i)
+	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
 		const OrProgram& g = P.prog[M.grouped];
@@ -217,13 +220,12 @@ __device__ __forceinline__ bool find_split(const OrParams& P, int round, int t, 
 				it.split = s;
 				it.slot = slot + t * s;
 				tile_origin<BN>(g.op[k], M.p, M.q, t, it.m0, it.n0);
-				return true;
+				return;
 			}
 			t -= n;
 			slot += n * s;
 		}
 	}
-	return false;
 }
 
 // ---- elements of the caller's matrices, four neighbours at a time ------------------------------------------------
@@ -280,8 +282,10 @@ __device__ __forceinline__ void split_pair(float x, float y, float s, uint32_t& 
 }
 
 // ---- 32 x 32 pieces, a row per lane --------------------------------------------------------------------------------
-// as the rows of a matrix of parts: through shared memory, four rows of 128 bytes (hi and lo) per access
-__device__ __forceinline__ void store_rows(const float (&v)[32], float s, __half* hi, long long plane, long long ld, uint32_t area, int lane)
+// 16-byte chunk k (0 .. 3 hi, 4 .. 7 lo) of row r in the warp's staging area
+__device__ __forceinline__ uint32_t chunk_at(uint32_t area, int r, int k) { return area + (uint32_t)(r * 128 + ((k ^ (r & 7)) << 4)); }
+// the parts of v * s into the staging area
+__device__ __forceinline__ void stage_parts(const float (&v)[32], float s, uint32_t area, int lane)
 {
 	__syncwarp();
 #pragma unroll
@@ -290,22 +294,46 @@ __device__ __forceinline__ void store_rows(const float (&v)[32], float s, __half
 		uint32_t h[4], l[4];
 #pragma unroll
 		for (int i = 0; i < 4; ++i) split_pair(v[8 * k + 2 * i], v[8 * k + 2 * i + 1], s, h[i], l[i]);
-		const uint32_t row = area + (uint32_t)lane * 128u;
-		asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (uint32_t)((k ^ (lane & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-		asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (uint32_t)(((k + 4) ^ (lane & 7)) << 4)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
+		asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(area, lane, k)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+		asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(area, lane, k + 4)), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
 	}
 	__syncwarp();
+}
+// the staged piece as rows of a matrix of parts, four rows of 64 bytes of hi and of lo per access
+__device__ __forceinline__ void store_staged(__half* hi, long long plane, long long ld, uint32_t area, int lane)
+{
 	const int k = lane & 7;
 	__half* d = hi + (k < 4 ? 0 : plane) + (long long)(lane >> 3) * ld + (k & 3) * 8;
+	uint4 w[8];
+#pragma unroll
+	for (int i = 0; i < 8; ++i)
+		asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "r"(chunk_at(area, i * 4 + (lane >> 3), k)));
 #pragma unroll
 	for (int i = 0; i < 8; ++i)
 	{
-		const int r = i * 4 + (lane >> 3);
-		uint4 w;
-		asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(area + (uint32_t)r * 128u + (uint32_t)((k ^ (r & 7)) << 4)));
-		*reinterpret_cast<uint4*>(d) = w;
+		*reinterpret_cast<uint4*>(d) = w[i];
 		d += 4 * ld;
 	}
+}
+// The staged piece transposed in place, 8 x 8 elements at a time: lane l gives the address of row l % 8 of block l / 8 of four.
+__device__ __forceinline__ void transpose_staged(uint32_t area, int lane)
+{
+	uint32_t w[8][4];
+	const int b = lane >> 3, r = lane & 7;
+	// blocks (4 rows of blocks) x (4 columns of hi, 4 of lo): one access takes a column of blocks
+#pragma unroll
+	for (int k = 0; k < 8; ++k)
+		asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+		             : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+		             : "r"(chunk_at(area, b * 8 + r, k)));
+	__syncwarp();
+	// block (i, k) becomes block (k, i) of its part
+#pragma unroll
+	for (int k = 0; k < 8; ++k)
+		asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(chunk_at(area, (k & 3) * 8 + r, (k & 4) + b)),
+		             "r"(w[k][0]), "r"(w[k][1]), "r"(w[k][2]), "r"(w[k][3])
+		             : "memory");
+	__syncwarp();
 }
 // acc += w * (32 elements of row r from column c on of the matrix of parts id)
 __device__ __forceinline__ void add_parts(float* acc, float w, int id, const OrMat& M, int r, int c)
@@ -384,13 +412,37 @@ __device__ __forceinline__ void update_weights(const float (&v)[32], const Ortho
 	}
 }
 
-// what becomes of a piece of a product: rows r0 + lane, columns c0 ..
-__device__ __forceinline__ void finish_piece(const OrParams& P, const OrMat& M, const OrOp& o, float (&v)[32], int r0, int c0, uint32_t area, int lane)
+// What the epilogue needs of an operation and its matrix, asked for before the products are awaited: the parameters lie in
+// constant memory, whose first touch takes as long as a copy from L2.
+struct OrTarget
 {
-#pragma unroll
-	for (int i = 0; i < 32; ++i) v[i] *= o.f;
-	if (o.out == ID_NONE)
+	float f, so;
+	int kind, p, q;  // kind: 0 the caller's matrix, 1 symmetric, 2 X
+	__half* D;
+	long long plane, ld;
+	__device__ __forceinline__ OrTarget(const OrMat& M, const OrOp& o)
 	{
+		f = o.f;
+		so = o.so;
+		p = M.p;
+		q = M.q;
+		kind = op_symmetric(o) ? 1 : (o.out == ID_NONE ? 0 : 2);
+		plane = o.out >= ID_X ? M.planex : M.planes;
+		ld = o.out >= ID_X ? M.ldx : M.lds;
+		D = o.out >= ID_X ? M.X + 2 * (o.out - ID_X) * plane : M.S + 2 * (o.out < 0 ? 0 : o.out) * plane;
+		asm volatile("" : "+f"(f), "+f"(so), "+r"(p), "+r"(q), "+r"(kind), "+l"(plane), "+l"(ld), "+l"(D));
+	}
+	// pieces that lie outside the matrix, or above the diagonal of a symmetric result (another piece's mirror image)
+	__device__ __forceinline__ bool needs(int r0, int c0) const { return r0 < p && (kind == 1 ? c0 <= r0 : c0 < q); }
+};
+// what becomes of a piece of a product: rows r0 + lane, columns c0 ..
+__device__ __forceinline__ void finish_piece(const OrParams& P, int mat, const OrTarget& T, float (&v)[32], int r0, int c0, uint32_t area, int lane)
+{
+	if (T.kind == 0)
+	{
+#pragma unroll
+		for (int i = 0; i < 32; ++i) v[i] *= T.f;
+		const OrMat& M = P.mat[mat];
 		if (!M.tall) transpose(v, area, lane);
 		// a wide matrix: lane = column, v = rows r0 ..; a tall one is transposed already: lane = its column, v = its rows c0 ..
 		const int r = M.tall ? c0 : r0, c = (M.tall ? r0 : c0) + lane;
@@ -400,13 +452,7 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, const OrMat& M, 
 		else store_result<GL_F16>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
 		return;
 	}
-	if (o.out >= ID_X)
-	{
-		store_rows(v, o.so, M.X + 2 * (o.out - ID_X) * M.planex + (long long)r0 * M.ldx + c0, M.planex, M.ldx, area, lane);
-		return;
-	}
-	__half* D = M.S + 2 * o.out * M.planes;
-	if (c0 == r0)
+	if (T.kind == 1 && c0 == r0)
 	{
 		// on the diagonal: the upper half becomes the lower half's mirror image
 		__syncwarp();
@@ -417,18 +463,14 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, const OrMat& M, 
 		for (int j = 0; j < 32; ++j)
 			if (j > lane) v[j] = square_get(area, j, lane);
 	}
-	store_rows(v, o.so, D + (long long)r0 * M.lds + c0, M.planes, M.lds, area, lane);
-	if (c0 != r0)
+	stage_parts(v, T.f * T.so, area, lane);
+	store_staged(T.D + (long long)r0 * T.ld + c0, T.plane, T.ld, area, lane);
+	if (T.kind == 1 && c0 != r0)
 	{
-		transpose(v, area, lane);
-		store_rows(v, o.so, D + (long long)c0 * M.lds + r0, M.planes, M.lds, area, lane);
+		__syncwarp();
+		transpose_staged(area, lane);
+		store_staged(T.D + (long long)c0 * T.ld + r0, T.plane, T.ld, area, lane);
 	}
-}
-// pieces that lie outside the matrix, or above the diagonal of a symmetric result (another piece's mirror image)
-__device__ __forceinline__ bool piece_needed(const OrMat& M, const OrOp& o, int r0, int c0)
-{
-	if (r0 >= M.p) return false;
-	return op_symmetric(o) ? c0 <= r0 : c0 < M.q;
 }
 
 __device__ __forceinline__ bool elect_one()
@@ -472,6 +514,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
 	      "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
 	      "=r"(r[31])
 	    : "r"(taddr)
+	    : "memory");
+}
+
+// tcgen05.mma with descriptors given as a low word (the address moves) and a high word that stays; the accumulator is added to,
+// or (first) replaced
+__device__ __forceinline__ void mma(bool first, uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc)
+{
+	asm volatile(
+	    "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+	    "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
+	    "setp.eq.u32 p, %6, 0;\n\t"
+	    "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+	    "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)first)
 	    : "memory");
 }
 
@@ -671,7 +726,6 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			}
 		}
 	}
-	asm volatile("fence.proxy.async;" ::: "memory");  // (the copies read through another proxy what ordinary stores have written)
 	grid.sync();
 
 	// ---- the products
@@ -681,16 +735,20 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	int buf = 0;           // MMA warp, epilogue: next accumulator, and how often (mod 2) both have been used
 	uint32_t aph = 0;
 	bool ok = true;
+	OrItem t;              // copying and multiplying warps: a round's first item is looked up in front of the barrier before it
+	if (warp < 2 && (int)blockIdx.x < P.items[0]) find_item<BN>(P, 0, blockIdx.x, t);
 	for (int round = 0; round < P.rounds; ++round)
 	{
-		OrItem t;
+		const int items = P.items[round];
 		if (warp == 0)
 		{
 			// ------------------------------------------------ TMA producer
+			// (the copies read through another proxy what ordinary stores of all CTAs have written in front of the grid barrier)
 			asm volatile("fence.proxy.async;" ::: "memory");
 			const bool leader = elect_one();
-			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
+			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
+				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
 				const OrMaps& mp = P.maps[t.mat];
 				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
 				const bool ax = o.a >= ID_X, bx = o.b >= ID_X;
@@ -728,16 +786,19 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		{
 			// ------------------------------------------------ MMA issuer (layouts and descriptors: gemm_tcgen05.cu)
 			const bool leader = elect_one();
-			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
+			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
+				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
 				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
 				const uint32_t b_mn = o.b >= ID_X && o.a < ID_X ? 1u : 0u;
 				const uint32_t idesc = (1u << 4) | (b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 				const uint32_t idesc2 = (1u << 4) | (b_mn << 16) | ((uint32_t)(S::COLUMNS >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
-				const uint64_t desc_a = make_smem_desc(base, 0u, 512u, 4u);
-				const uint64_t desc_b = make_smem_desc(base + 2 * S::A_BYTES, b_mn ? 128u * OR_BK : 0u, b_mn ? 1024u : 512u, b_mn ? 2u : 4u);
+				// K-major: rows of 128 bytes, eight of them a group; MN-major: 64 columns by OR_BK k; 128-byte swizzle
+				const uint64_t desc_a = make_smem_desc(base, 0u, 1024u, 2u);
+				const uint64_t desc_b = make_smem_desc(base + 2 * S::A_BYTES, b_mn ? 128u * OR_BK : 0u, 1024u, 2u);
+				const uint32_t a_low = (uint32_t)desc_a, a_high = (uint32_t)(desc_a >> 32), b_low = (uint32_t)desc_b, b_high = (uint32_t)(desc_b >> 32);
 				const uint32_t a_step = 32u >> 4, b_step = b_mn ? 2048u >> 4 : 32u >> 4;
-				constexpr uint32_t A_LO = S::A_BYTES >> 4, B_LO = S::B_BYTES >> 4;
+				constexpr uint32_t A_LO = S::A_BYTES >> 4;
 				int in = 0;
 				for (int left = t.kb1 - t.kb0; left > 0; --left)
 				{
@@ -749,27 +810,16 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 					if (!warp_wait(full, ph, abort_flag, P.status, 2)) { ok = false; break; }
 					asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 					const uint32_t off = (uint32_t)s * (S::STAGE_BYTES >> 4);
-					const uint64_t a0 = desc_a + off, b0 = desc_b + off;
-					const uint64_t a1 = a0 + a_step, b1 = b0 + b_step;
+					const uint32_t a0 = a_low + off, b0 = b_low + off;
 					const uint32_t d = tmem_base + (uint32_t)(buf * S::COLUMNS);
 					const bool ends = in + 1 == S::CHUNK || left == 1;
 					if (leader)
 					{
-						if (S::PAIR)
+#pragma unroll
+						for (int k = 0; k < OR_BK / 16; ++k)
 						{
-							umma_f16(d, a0, b0, idesc2, (uint32_t)in);
-							umma_f16(d, a1, b1, idesc2, 1u);
-							umma_f16(d + BN, a0 + A_LO, b0, idesc, 1u);
-							umma_f16(d + BN, a1 + A_LO, b1, idesc, 1u);
-						}
-						else
-						{
-							umma_f16(d, a0, b0 + B_LO, idesc, (uint32_t)in);
-							umma_f16(d, a0 + A_LO, b0, idesc, 1u);
-							umma_f16(d, a1, b1 + B_LO, idesc, 1u);
-							umma_f16(d, a1 + A_LO, b1, idesc, 1u);
-							umma_f16(d, a0, b0, idesc, 1u);
-							umma_f16(d, a1, b1, idesc, 1u);
+							mma(k == 0 && in == 0, d, a0 + k * a_step, a_high, b0 + k * b_step, b_high, idesc2);
+							mma(false, d + BN, a0 + A_LO + k * a_step, a_high, b0 + k * b_step, b_high, idesc);
 						}
 						umma_commit(full + 8 * STAGES);
 						if (ends) umma_commit(bar_acc_full + 8 * buf);
@@ -790,15 +840,17 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				}
 			}
 		}
-		else
+		else if (warp >= S::FIRST)
 		{
 			// ------------------------------------------------ epilogue
-			const uint32_t area = staging0 + (uint32_t)(warp - 2) * 4096u;
-			const int quarter = warp & 3, half = (warp - 2) >> 2;
-			for (int ti = blockIdx.x; ok && find_item<BN>(P, round, ti, t); ti += gridDim.x)
+			const uint32_t area = staging0 + (uint32_t)(warp - S::FIRST) * 4096u;
+			const int quarter = warp & 3, half = (warp - S::FIRST) >> 2;
+			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
+				find_item<BN>(P, round, ti, t);
 				const OrMat& M = P.mat[t.mat];
 				const OrOp& o = P.prog[M.grouped].op[t.op];
+				const OrTarget target(M, o);
 				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
 				float acc[EC];
 #pragma unroll
@@ -807,7 +859,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				{
 #pragma unroll
 					for (int pc = 0; pc < EC / 32; ++pc)
-						if (piece_needed(M, o, r0, c00 + pc * 32))
+						if (target.needs(r0, c00 + pc * 32))
 						{
 							add_parts(acc + pc * 32, o.w1, o.e1, M, r0 + lane, c00 + pc * 32);
 							add_parts(acc + pc * 32, o.w2, o.e2, M, r0 + lane, c00 + pc * 32);
@@ -822,27 +874,17 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 					}
 					asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 					const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * S::COLUMNS + half * EC);
-					if (S::PAIR)
-					{
 #pragma unroll
-						for (int c = 0; c < EC / 32; ++c)
+					for (int c = 0; c < EC / 32; ++c)
+#pragma unroll
+						for (int h = 1; h >= 0; --h)
 						{
 							uint32_t r[32];
-							tmem_ld32(taddr + (uint32_t)(BN + c * 32), r);
+							tmem_ld32(taddr + (uint32_t)(h * BN + c * 32), r);
 							asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
 							for (int e = 0; e < 32; ++e) acc[c * 32 + e] += __uint_as_float(r[e]);
 						}
-					}
-#pragma unroll
-					for (int c = 0; c < EC / 32; ++c)
-					{
-						uint32_t r[32];
-						tmem_ld32(taddr + (uint32_t)(c * 32), r);
-						asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-						for (int e = 0; e < 32; ++e) acc[c * 32 + e] += __uint_as_float(r[e]);
-					}
 					asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 					__syncwarp();
 					if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar_acc_empty + 8 * buf) : "memory");
@@ -854,7 +896,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				for (int pc = 0; pc < EC / 32; ++pc)
 				{
 					const int c0 = c00 + pc * 32;
-					if (!piece_needed(M, o, r0, c0)) continue;
+					if (!target.needs(r0, c0)) continue;
 					if (t.split > 1)
 					{
 						float4* d = P.part + ((long long)t.slot * S::PIECES + quarter * (BN / 32) + half * (EC / 32) + pc) * 256 + lane;
@@ -866,26 +908,25 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 					float v[32];
 #pragma unroll
 					for (int i = 0; i < 32; ++i) v[i] = acc[pc * 32 + i];
-					finish_piece(P, M, o, v, r0, c0, area, lane);
+					finish_piece(P, t.mat, target, v, r0, c0, area, lane);
 				}
 			}
-			asm volatile("fence.proxy.async;" ::: "memory");
 		}
 		if (P.reduce >> round & 1)
 		{
 			grid.sync();
-			if (warp >= 2)
+			if (warp >= S::FIRST)
 			{
-				const uint32_t area = staging0 + (uint32_t)(warp - 2) * 4096u;
+				const uint32_t area = staging0 + (uint32_t)(warp - S::FIRST) * 4096u;
 				const int warps = (int)gridDim.x * S::EPI_WARPS;
 				// (neighbouring pieces on different SMs)
-				for (int k = (warp - 2) * (int)gridDim.x + (int)blockIdx.x; find_split<BN>(P, round, k / S::PIECES, t); k += warps)
+				for (int k = (warp - S::FIRST) * (int)gridDim.x + (int)blockIdx.x; k < P.splits[round] * S::PIECES; k += warps)
 				{
-					const OrMat& M = P.mat[t.mat];
-					const OrOp& o = P.prog[M.grouped].op[t.op];
+					find_split<BN>(P, round, k / S::PIECES, t);
+					const OrTarget target(P.mat[t.mat], P.prog[P.mat[t.mat].grouped].op[t.op]);
 					const int pc = k % S::PIECES;
 					const int r0 = t.m0 + pc / (BN / 32) * 32, c0 = t.n0 + pc % (BN / 32) * 32;
-					if (!piece_needed(M, o, r0, c0)) continue;
+					if (!target.needs(r0, c0)) continue;
 					float v[32];
 					const float4* d = P.part + ((long long)t.slot * S::PIECES + pc) * 256 + lane;
 #pragma unroll
@@ -905,12 +946,15 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 							v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
 						}
 					}
-					finish_piece(P, M, o, v, r0, c0, area, lane);
+					finish_piece(P, t.mat, target, v, r0, c0, area, lane);
 				}
-				asm volatile("fence.proxy.async;" ::: "memory");
 			}
 		}
-		if (round + 1 < P.rounds) grid.sync();
+		if (round + 1 < P.rounds)
+		{
+			if (warp < 2 && (int)blockIdx.x < P.items[round + 1]) find_item<BN>(P, round + 1, blockIdx.x, t);
+			grid.sync();
+		}
 	}
 	if (*abort_flag)
 	{
@@ -1092,12 +1136,12 @@ struct Plan
 	int slots;  // of split tiles' parts
 };
 
-// About how many clocks an item of kb stages costs: a stage's six MMAs and what surrounds them, then draining and storing.
-long long item_clocks(int bn, long long kb) { return kb * (bn == 256 ? 960 : (bn == 128 ? 520 : 400)) + 4000; }
-constexpr long long ROUND_CLOCKS = 9000;   // a round's barrier, first copies, last stores
-constexpr long long REDUCE_CLOCKS = 6000;  // the further barrier and the sums of a round with split tiles
+// About how many clocks (of 1.9 GHz), measured on rounds of one kind: an item of kb stages from its first copy to its last store,
+// what a round costs beside its items (its barrier), and a round with split tiles on top (another barrier and the sums).
+long long item_clocks(int bn, long long kb) { return kb * (bn == 128 ? 900 : 550) + (bn == 128 ? 7000 : 5000); }
+constexpr long long ROUND_CLOCKS = 3000, REDUCE_CLOCKS = 8000;
 
-// The splits of tiles of width bn, and about how many clocks the rounds take: for each the CTA with the most work.
+// Tiles of width bn: how far they are split, and about how many clocks the rounds take: for each the CTA with the most work.
 long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OPS], unsigned long long* reduce, int* slots)
 {
 	long long total = 0;
@@ -1118,30 +1162,36 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 			tiles += n;
 			work += (long long)n * kb;
 		});
-		// Parts of about equal length for all operations, so many that every SM has one; a tile that is shorter stays whole.
-		const long long share = std::max<long long>(OR_SPLIT_KB, (work + OR_SMS - 1) / OR_SMS);
-		long long load[OR_SMS] = {0}, worst = 0;
-		int t = 0, used = 0;
+		// whole tiles, or parts of about equal length for all operations, so many that every SM has one
+		const long long share = std::max<long long>(OR_SPLIT_K / OR_BK, (work + OR_SMS - 1) / OR_SMS);
+		auto parts = [&](bool whole, int kb) { return whole ? 1 : (int)std::max<long long>(1, std::min<long long>(255, kb / share)); };
+		auto clocks = [&](bool whole) {
+			long long load[OR_SMS] = {0}, worst = 0;
+			int t = 0, used = 0;
+			each([&](int, int, int n, int kb) {
+				const int s = parts(whole, kb);
+				if (s > 1) used += n * s;
+				const long long cost = item_clocks(bn, (kb + s - 1) / s);
+				const long long rounds = (long long)n * s / OR_SMS;
+				for (int c = 0; c < OR_SMS && rounds; ++c) load[c] += rounds * cost;
+				const int rest = (int)((long long)n * s % OR_SMS);
+				for (int c = 0; c < rest; ++c) load[(t + c) % OR_SMS] += cost;
+				t = (t + rest) % OR_SMS;
+			});
+			for (long long l : load) worst = std::max(worst, l);
+			return worst + ROUND_CLOCKS + (used ? REDUCE_CLOCKS : 0);
+		};
+		const long long cost = clocks(true);
+		const long long cost_split = tiles * 2 <= OR_SMS ? clocks(false) : cost;
+		const bool whole = cost <= cost_split;
+		int used = 0;
 		each([&](int i, int k, int n, int kb) {
-			int s = tiles * 2 <= OR_SMS ? (int)std::min<long long>(255, kb / share) : 1;
-			if (s < 1) s = 1;
-			split[i][k] = (unsigned char)s;
-			if (s > 1) used += n * s;
-			const long long each_kb = (kb + s - 1) / s;
-			const long long rounds = (long long)n * s / OR_SMS;
-			for (int c = 0; c < OR_SMS && rounds; ++c) load[c] += rounds * item_clocks(bn, each_kb);
-			const int rest = (int)((long long)n * s % OR_SMS);
-			for (int c = 0; c < rest; ++c) load[(t + c) % OR_SMS] += item_clocks(bn, each_kb);
-			t = (t + rest) % OR_SMS;
+			split[i][k] = (unsigned char)parts(whole, kb);
+			if (split[i][k] > 1) used += n * split[i][k];
 		});
-		for (long long l : load) worst = std::max(worst, l);
-		total += worst + ROUND_CLOCKS;
-		if (used)
-		{
-			*reduce |= 1ull << round;
-			total += REDUCE_CLOCKS;
-		}
+		if (used) *reduce |= 1ull << round;
 		*slots = std::max(*slots, used);
+		total += std::min(cost, cost_split);
 	}
 	return total;
 }
@@ -1156,7 +1206,7 @@ bool worth_grouping(const OrProgram* prog, int p, int q)
 	{
 		double work = 0.0;
 		for (int k = 0; k < prog[v].count; ++k) work += (double)op_tiles(prog[v].op[k], p, q, 128) * op_kb(prog[v].op[k], p, q);
-		clocks[v] = work * 520 / OR_SMS + (double)prog[v].rounds * ROUND_CLOCKS;
+		clocks[v] = work * 900 / OR_SMS + (double)prog[v].rounds * (ROUND_CLOCKS + REDUCE_CLOCKS);
 	}
 	return clocks[1] < clocks[0];
 }
@@ -1213,7 +1263,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		bytes += matrix_bytes(M, g.planes);
 	}
 	long long best = -1;
-	for (int bn : {256, 128, 64})
+	for (int bn : {128, 64})
 	{
 		static thread_local unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
 		unsigned long long reduce;
@@ -1251,7 +1301,7 @@ cudaError_t launch_width(OrParams& P, cudaStream_t s)
 	int most = P.units;
 	for (int round = 0; round < P.rounds; ++round)
 	{
-		int n = 0, pieces = 0;
+		int n = 0, splits = 0;
 		for (int i = 0; i < P.count; ++i)
 		{
 			const OrProgram& g = P.prog[P.mat[i].grouped];
@@ -1259,10 +1309,12 @@ cudaError_t launch_width(OrParams& P, cudaStream_t s)
 			{
 				const int tiles = op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, BN);
 				n += tiles * P.split[i][k];
-				if (P.split[i][k] > 1) pieces += tiles * OrSmem<BN>::PIECES;
+				if (P.split[i][k] > 1) splits += tiles;
 			}
 		}
-		most = std::max(most, std::max(n, pieces));
+		P.items[round] = n;
+		P.splits[round] = splits;
+		most = std::max(most, std::max(n, splits * OrSmem<BN>::PIECES));
 	}
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned)std::min(std::min(sms, OR_SMS), most));
@@ -1301,10 +1353,9 @@ size_t ortho_workspace_bytes(const OrthoMatrix* m, int count)
 			M.p = std::min(m[i].rows, m[i].cols);
 			M.q = std::max(m[i].rows, m[i].cols);
 			bytes += matrix_bytes(M, may_group(M.p, M.q) ? OR_PLANES : 2);
-			const double kb = ceil(M.q / (double)OR_BK);
-			if (kb >= 2 * OR_SPLIT_KB) parts += 2 * ceil(M.p / 128.0) * ceil(M.q / 64.0) * kb / OR_SPLIT_KB;
+			if (M.q > OR_SPLIT_K) parts += 2 * ceil(M.p / 128.0) * ceil(M.q / 64.0) * ceil(M.q / (double)OR_SPLIT_K);
 		}
-		most = std::max(most, bytes + (size_t)std::min(parts, (double)OR_SMS) * 128 * 256 * sizeof(float));
+		most = std::max(most, bytes + (size_t)std::min(parts, (double)OR_SMS) * 128 * 128 * sizeof(float));
 	}
 	return 256 + OR_HEADER + round_up(OR_SUMS, 256) + most;  // (256: the caller's pointer need not be aligned)
 }
@@ -1334,7 +1385,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			M.S = M.X + 4 * M.planex;
 			at += matrix_bytes(M, P.prog[M.grouped].planes);
 		}
-		const cudaError_t e = plan.bn == 256 ? launch_width<256>(P, s) : (plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s));
+		const cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
 		if (e != cudaSuccess) return e;
 	}
 	return cudaSuccess;

@@ -93,7 +93,7 @@ cudaError_t prepare_tc_launch(const void* kernel, int smem_bytes, int* sm_count)
 // fp32 operand for 16-deep k-blocks: K-contiguous rows (64-byte swizzle), or MN-contiguous as [r/32][k][r%32]
 bool tc_make_operand_map_f32(void* out128, const float* ptr, int mn, long long rows, long long k, long long ld, int box_rows);
 // A stack of `planes` [rows][cols] fp16 matrices (pitch ld, a plane `plane` halfs behind the other; both multiples of 64), in boxes of two
-// planes: as a K-contiguous operand (box_rows x box_cols = 32 k, 64-byte swizzle) ...
+// planes: as a K-contiguous operand (box_rows x box_cols = 64 k, 128-byte swizzle) ...
 bool tc_make_parts_map(void* out128, const __half* base, long long rows, long long cols, long long ld, long long plane, int planes, int box_cols,
                        int box_rows);
 // ... and, its rows being k, as a column-contiguous one ([cols/64][k][64]: box_k x box_cols, a multiple of 64; 128-byte swizzle)
