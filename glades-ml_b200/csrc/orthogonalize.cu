@@ -8,8 +8,8 @@
 // on one side instead of n of each, and 2 (n - 1) + (n - 1) more products of p x p matrices:
 //     T = a A + R A,   A' = a T + T R,   Q' = P Q  as  q' + Qr' = a q + (a Qr + q R + R Qr)
 // 15 p^2 q + 5 p^3 multiply-adds become 6 p^2 q + 14 p^3 for five steps in groups of three and two (symmetric products by half).
-// A's rounding is absolute, so small singular values lose digits with every further step of a group: three steps from the start,
-// where the elements of A are small, and two later stay within the error of fp32 products (emulated and measured); see groups_of.
+// A's rounding is absolute, so small singular values lose digits with every further step of a group: two steps, and
+// three from the start of a large matrix, whose A has small elements, stay within the error of fp32 products; see groups_allowed.
 //
 // Bound: tensor cores.  Every product is fp32-faithful on three fp16 products (hi*hi + hi*lo + lo*hi), as the layer products of
 // gemm_tcgen05.cu; unlike there the scales are known beforehand -- all singular values stay below a bound that follows from
@@ -34,8 +34,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "orthogonalize.h"
-#include "tc_device.cuh"
+#include "ortho_device.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -47,11 +46,9 @@ namespace {
 // stages of 32 k that bounded both tiles (530 clocks per 32 k on 128 columns, 350 to 400 now).
 constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
+constexpr int OR_PROGRAMS = 3;
 constexpr int OR_SMS = 148;
 constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
-constexpr int OR_MAX_OPS = 4 * ORTHO_MAX_STEPS;
-constexpr int OR_MAX_ROUNDS = 64;  // at most 55 are needed: step by step three per step, in groups of n 3 n + 1
-constexpr int OR_PLANES = 6;   // p x p matrices of a grouped program
 
 template <int BN>
 struct OrSmem
@@ -74,26 +71,10 @@ struct OrSmem
 	static constexpr int TOTAL = TILES_BYTES + STAGING_BYTES + 1024 /*alignment slack*/ + 512 /*barriers, sums*/;
 };
 
-// Matrices of parts that an operation names: 0 .. 5 p x p, 6 and 7 the two X.
-enum { ID_A = 0, ID_X = 6, ID_NONE = -1 };
-// out = f (A B^T or A B + w1 E1 + w2 E2); the factors hold the parts' scales
-struct OrOp
-{
-	signed char a, b, e1, e2, out;  // out ID_NONE: the result
-	signed char round;
-	float f, w1, w2, so;
-};
-struct OrProgram
-{
-	OrOp op[OR_MAX_OPS];
-	int count, rounds, planes;
-	unsigned char first[OR_MAX_ROUNDS + 1];  // operations first[r] .. first[r + 1] - 1 are round r's
-};
-
 struct OrMat
 {
 	OrthoMatrix m;
-	int p, q, tall, grouped;
+	int p, q, tall, program;
 	long long ldx, planex;  // halfs: row pitch and size of one part of X; parts in the order X0 hi, X0 lo, X1 hi, X1 lo
 	long long lds, planes;  // the same of the p x p matrices
 	__half* X;
@@ -109,7 +90,7 @@ struct OrParams
 {
 	OrMaps maps[ORTHO_MAX_MATRICES];
 	OrMat mat[ORTHO_MAX_MATRICES];
-	OrProgram prog[2];      // step by step; in groups
+	OrProgram prog[OR_PROGRAMS];  // step by step; in groups of two; with three steps in the first
 	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
 	unsigned long long reduce;  // rounds with split tiles
 	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
@@ -176,7 +157,7 @@ __device__ __forceinline__ void find_item(const OrParams& P, int round, int t, O
 	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.grouped];
+		const OrProgram& g = P.prog[M.program];
 		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
 		{
 			const int s = P.split[i][k];
@@ -207,7 +188,7 @@ __device__ __forceinline__ void find_split(const OrParams& P, int round, int t, 
 	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.grouped];
+		const OrProgram& g = P.prog[M.program];
 		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
 		{
 			const int s = P.split[i][k];
@@ -226,59 +207,6 @@ __device__ __forceinline__ void find_split(const OrParams& P, int round, int t, 
 			slot += n * s;
 		}
 	}
-}
-
-// ---- elements of the caller's matrices, four neighbours at a time ------------------------------------------------
-__device__ __forceinline__ float load_typed(const void* p, long long i, int type)
-{
-	if (type == GL_F32) return static_cast<const float*>(p)[i];
-	if (type == GL_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-	return __half2float(static_cast<const __half*>(p)[i]);
-}
-// `left` of them exist; wide: a 16-byte (8-byte) boundary
-__device__ __forceinline__ void load4(const void* p, long long i, int type, bool wide, int left, float (&v)[4])
-{
-	if (wide && left >= 4)
-	{
-		if (type == GL_F32)
-		{
-			const float4 w = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-			v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-			return;
-		}
-		const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i);
-#pragma unroll
-		for (int k = 0; k < 4; ++k)
-		{
-			const unsigned short u = (unsigned short)((k < 2 ? w.x : w.y) >> (16 * (k & 1)));
-			v[k] = type == GL_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
-		}
-		return;
-	}
-#pragma unroll
-	for (int k = 0; k < 4; ++k) v[k] = k < left ? load_typed(p, i + k, type) : 0.0f;
-}
-__device__ __forceinline__ void store4(float* p, long long i, bool wide, int left, const float (&v)[4])
-{
-	if (wide && left >= 4)
-	{
-		*reinterpret_cast<float4*>(p + i) = make_float4(v[0], v[1], v[2], v[3]);
-		return;
-	}
-#pragma unroll
-	for (int k = 0; k < 4; ++k)
-		if (k < left) p[i + k] = v[k];
-}
-
-// hi and lo of x * s, lo unscaled
-__device__ __forceinline__ void split_pair(float x, float y, float s, uint32_t& hi, uint32_t& lo)
-{
-	const float xs = x * s, ys = y * s;
-	const __half2 h = __floats2half2_rn(xs, ys);
-	const float2 f = __half22float2(h);
-	const __half2 l = __floats2half2_rn(xs - f.x, ys - f.y);
-	hi = *reinterpret_cast<const uint32_t*>(&h);
-	lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // ---- 32 x 32 pieces, a row per lane --------------------------------------------------------------------------------
@@ -473,36 +401,6 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, int mat, const O
 	}
 }
 
-__device__ __forceinline__ bool elect_one()
-{
-	uint32_t p;
-	asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
-	return p != 0;
-}
-// A bounded wait of a whole warp, which stays together: what the issuing warps compute can then live in uniform registers
-// (one lane on its own spends 70 clocks on the operands of every MMA it issues).
-__device__ __noinline__ static bool warp_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag, int code)
-{
-	const long long t0 = clock64();
-	for (;;)
-	{
-		if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
-		if (__any_sync(0xFFFFFFFFu, *abort_flag != 0)) return false;
-		if (__any_sync(0xFFFFFFFFu, clock64() - t0 > TC_WAIT_CYCLES))
-		{
-			if ((threadIdx.x & 31) == 0)
-			{
-				*abort_flag = 1;
-				atomicExch(err_flag, code);
-			}
-			return false;
-		}
-	}
-}
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err_flag, int code)
-{
-	return __all_sync(0xFFFFFFFFu, mbar_try(bar, parity)) || warp_wait_slow(bar, parity, abort_flag, err_flag, code);
-}
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
 {
 	asm volatile(
@@ -514,19 +412,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
 	      "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
 	      "=r"(r[31])
 	    : "r"(taddr)
-	    : "memory");
-}
-
-// tcgen05.mma with descriptors given as a low word (the address moves) and a high word that stays; the accumulator is added to,
-// or (first) replaced
-__device__ __forceinline__ void mma(bool first, uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc)
-{
-	asm volatile(
-	    "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-	    "mov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\t"
-	    "setp.eq.u32 p, %6, 0;\n\t"
-	    "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
-	    "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc), "r"((uint32_t)first)
 	    : "memory");
 }
 
@@ -750,7 +635,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			{
 				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
 				const OrMaps& mp = P.maps[t.mat];
-				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
+				const OrOp& o = P.prog[P.mat[t.mat].program].op[t.op];
 				const bool ax = o.a >= ID_X, bx = o.b >= ID_X;
 				const CUtensorMap* ma = ax ? &mp.xa : &mp.sa;
 				const CUtensorMap* mb = ax ? &mp.xb : &mp.sb;
@@ -789,7 +674,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
 				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
-				const OrOp& o = P.prog[P.mat[t.mat].grouped].op[t.op];
+				const OrOp& o = P.prog[P.mat[t.mat].program].op[t.op];
 				const uint32_t b_mn = o.b >= ID_X && o.a < ID_X ? 1u : 0u;
 				const uint32_t idesc = (1u << 4) | (b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 				const uint32_t idesc2 = (1u << 4) | (b_mn << 16) | ((uint32_t)(S::COLUMNS >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
@@ -849,7 +734,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			{
 				find_item<BN>(P, round, ti, t);
 				const OrMat& M = P.mat[t.mat];
-				const OrOp& o = P.prog[M.grouped].op[t.op];
+				const OrOp& o = P.prog[M.program].op[t.op];
 				const OrTarget target(M, o);
 				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
 				float acc[EC];
@@ -923,7 +808,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				for (int k = (warp - S::FIRST) * (int)gridDim.x + (int)blockIdx.x; k < P.splits[round] * S::PIECES; k += warps)
 				{
 					find_split<BN>(P, round, k / S::PIECES, t);
-					const OrTarget target(P.mat[t.mat], P.prog[P.mat[t.mat].grouped].op[t.op]);
+					const OrTarget target(P.mat[t.mat], P.prog[P.mat[t.mat].program].op[t.op]);
 					const int pc = k % S::PIECES;
 					const int r0 = t.m0 + pc / (BN / 32) * 32, c0 = t.n0 + pc % (BN / 32) * 32;
 					if (!target.needs(r0, c0)) continue;
@@ -1033,9 +918,9 @@ float scale_under(double bound)
 }
 
 // Steps of the groups.  A group multiplies what its A's rounding does to a small singular value by the product of its steps'
-// slopes at zero: up to 64 in the first group, whose A has elements of about 1/p, up to 16 later (the usual coefficients, 3.4445:
-// groups of three, two, two, ..).
-int groups_of(const float (*coef)[3], int steps, int* size)
+// slopes at zero.  It may be up to `first` in the first group, whose A has elements of about 1/p, and 16 later (the usual slope is
+// 3.4445: groups of two under a limit of 16, a first one of three under 64).
+int groups_of(const float (*coef)[3], int steps, double first, int* size)
 {
 	int n = 0;
 	for (int k = 0; k < steps; ++n)
@@ -1045,11 +930,14 @@ int groups_of(const float (*coef)[3], int steps, int* size)
 		for (++k; k < steps && size[n] < 3; ++k, ++size[n])
 		{
 			growth *= std::max(1.0, (double)fabsf(coef[k][0]));
-			if (growth > (n == 0 ? 64.0 : 16.0)) break;
+			if (growth > (n == 0 ? first : 16.0)) break;
 		}
 	}
 	return n;
 }
+// Error of five steps against fp32 products', 2-norms, emulated: groups of 3 and 2 -- p = 256: 1.5e-6 against 2.4e-6, 128: 1.8e-6
+// against 1.7e-6, 64: 2.5e-6 against 1.1e-6; of 2, 2 and 1 -- 128: 1.5e-6, 64: 1.1e-6, 32: 1.5e-6 against 0.9e-6.
+bool groups_allowed(int program, int p) { return program == 0 || p >= (program == 1 ? 64 : 192); }
 
 void make_program(OrProgram& g, const float (*coef)[3], const Bounds& b, const int* size, int groups)
 {
@@ -1129,6 +1017,19 @@ void make_program(OrProgram& g, const float (*coef)[3], const Bounds& b, const i
 	}
 }
 
+// The first `count` programs; returns X_0's scale.
+float make_programs(OrProgram* prog, int count, const OrthoArgs& a)
+{
+	Bounds b;
+	bounds_of(a.coef, a.steps, b);
+	int size[ORTHO_MAX_STEPS];
+	for (int k = 0; k < a.steps; ++k) size[k] = 1;
+	make_program(prog[0], a.coef, b, size, a.steps);
+	if (count > 1) make_program(prog[1], a.coef, b, size, groups_of(a.coef, a.steps, 16.0, size));
+	if (count > 2) make_program(prog[2], a.coef, b, size, groups_of(a.coef, a.steps, 64.0, size));
+	return scale_under(b.sx[0]);
+}
+
 // A launch's plan: programs, which matrix takes which, the width of the tiles, how far tiles are split.
 struct Plan
 {
@@ -1154,7 +1055,7 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 		auto each = [&](auto&& f) {
 			for (int i = 0; i < P.count; ++i)
 			{
-				const OrProgram& g = P.prog[P.mat[i].grouped];
+				const OrProgram& g = P.prog[P.mat[i].program];
 				for (int k = g.first[round]; k < g.first[round + 1]; ++k) f(i, k, op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, bn), op_kb(g.op[k], P.mat[i].p, P.mat[i].q));
 			}
 		};
@@ -1197,18 +1098,24 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 }
 
 // Grouped steps save multiply-adds (of matrices that are not nearly square) and cost rounds.
-bool may_group(int p, int q) { return q > p + p / 16; }  // (a group's six p x p matrices instead of two)
-bool worth_grouping(const OrProgram* prog, int p, int q)
+bool may_group(int p, int q) { return p >= 64 && q > p + p / 16; }  // (a group's six p x p matrices instead of two)
+int choose_program(const OrProgram* prog, int p, int q)
 {
-	if (!may_group(p, q)) return false;
-	double clocks[2];
-	for (int v = 0; v < 2; ++v)
+	int best = 0;
+	double least = 0.0;
+	for (int v = 0; v < (may_group(p, q) ? OR_PROGRAMS : 1); ++v)
 	{
+		if (!groups_allowed(v, p)) continue;
 		double work = 0.0;
 		for (int k = 0; k < prog[v].count; ++k) work += (double)op_tiles(prog[v].op[k], p, q, 128) * op_kb(prog[v].op[k], p, q);
-		clocks[v] = work * 900 / OR_SMS + (double)prog[v].rounds * (ROUND_CLOCKS + REDUCE_CLOCKS);
+		const double clocks = work * 900 / OR_SMS + (double)prog[v].rounds * (ROUND_CLOCKS + REDUCE_CLOCKS);
+		if (v == 0 || clocks < least)
+		{
+			best = v;
+			least = clocks;
+		}
 	}
-	return clocks[1] < clocks[0];
+	return best;
 }
 
 size_t matrix_bytes(const OrMat& M, int planes)
@@ -1228,14 +1135,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.mu = a.mu;
 	P.decay = a.decay;
 	P.eps = a.eps;
-	Bounds b;
-	bounds_of(a.coef, a.steps, b);
-	P.s0 = scale_under(b.sx[0]);
-	int size[ORTHO_MAX_STEPS];
-	for (int k = 0; k < a.steps; ++k) size[k] = 1;
-	make_program(P.prog[0], a.coef, b, size, a.steps);
-	const int groups = groups_of(a.coef, a.steps, size);
-	make_program(P.prog[1], a.coef, b, size, groups);
+	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
 	for (int i = 0; i < count; ++i)
 	{
 		OrMat& M = P.mat[i];
@@ -1243,7 +1143,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.tall = M.m.rows > M.m.cols;
 		M.p = std::min(M.m.rows, M.m.cols);
 		M.q = std::max(M.m.rows, M.m.cols);
-		M.grouped = groups < a.steps && worth_grouping(P.prog, M.p, M.q);
+		M.program = choose_program(P.prog, M.p, M.q);
 	}
 	// the matrices with the longest products first: what is left for the last CTAs of a round is small
 	std::stable_sort(P.mat, P.mat + count, [](const OrMat& x, const OrMat& y) { return (double)x.p * x.q > (double)y.p * y.q; });
@@ -1251,7 +1151,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	for (int i = 0; i < count; ++i)
 	{
 		OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.grouped];
+		const OrProgram& g = P.prog[M.program];
 		P.rounds = std::max(P.rounds, g.rounds);
 		M.ldx = (long long)round_up(M.q, 128);
 		M.planex = M.ldx * (long long)round_up(M.p, 128);
@@ -1293,7 +1193,7 @@ template <int BN>
 cudaError_t launch_width(OrParams& P, cudaStream_t s)
 {
 	for (int i = 0; i < P.count; ++i)
-		if (!make_maps<BN>(P.maps[i], P.mat[i], P.prog[P.mat[i].grouped].planes)) return cudaErrorInvalidValue;
+		if (!make_maps<BN>(P.maps[i], P.mat[i], P.prog[P.mat[i].program].planes)) return cudaErrorInvalidValue;
 	int sms = 0;
 	cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(ortho_kernel<BN>), OrSmem<BN>::TOTAL, &sms);
 	if (e != cudaSuccess) return e;
@@ -1304,7 +1204,7 @@ cudaError_t launch_width(OrParams& P, cudaStream_t s)
 		int n = 0, splits = 0;
 		for (int i = 0; i < P.count; ++i)
 		{
-			const OrProgram& g = P.prog[P.mat[i].grouped];
+			const OrProgram& g = P.prog[P.mat[i].program];
 			for (int k = g.first[round]; k < g.first[round + 1]; ++k)
 			{
 				const int tiles = op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, BN);
@@ -1367,11 +1267,23 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 	OrParams& P = t_params;
 	for (int first = 0; first < a.count; first += ORTHO_MAX_MATRICES)
 	{
+		// A list of small matrices only goes to one CTA for each of them; beside larger ones they ride along.
+		const int count = std::min(ORTHO_MAX_MATRICES, a.count - first);
+		int* const status = a.status ? a.status : ortho_status(work);
+		bool small = true;
+		for (int i = first; i < first + count && small; ++i) small = ortho_small(a.mat[i].rows, a.mat[i].cols);
+		if (small)
+		{
+			const float s0 = make_programs(P.prog, 1, a);
+			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, first, count, status, first == 0 && !a.status, s);
+			if (e != cudaSuccess) return e;
+			continue;
+		}
 		Plan plan;
-		const size_t need = make_plan(P, a, a.mat + first, std::min(ORTHO_MAX_MATRICES, a.count - first), plan);
+		const size_t need = make_plan(P, a, a.mat + first, count, plan);
 		if (need + 256 > work_bytes) return cudaErrorInvalidValue;
 		char* at = reinterpret_cast<char*>(ortho_status(work));
-		P.status = a.status ? a.status : reinterpret_cast<int*>(at);
+		P.status = status;
 		P.reset = first == 0 && !a.status;
 		at += OR_HEADER;
 		P.sums = reinterpret_cast<double*>(at);
@@ -1383,7 +1295,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			OrMat& M = P.mat[i];
 			M.X = reinterpret_cast<__half*>(at);
 			M.S = M.X + 4 * M.planex;
-			at += matrix_bytes(M, P.prog[M.grouped].planes);
+			at += matrix_bytes(M, P.prog[M.program].planes);
 		}
 		const cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
 		if (e != cudaSuccess) return e;

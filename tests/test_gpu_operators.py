@@ -381,9 +381,20 @@ def check_ortho(g, shapes, t="f32", steps=5, coefficients=None, kind="mixed", se
 
 @pytest.mark.parametrize("shape", [(1, 1), (1, 2), (2, 1), (3, 5), (16, 4), (1, 256), (256, 1), (31, 33), (64, 64), (65, 63), (100, 128),
                                    (127, 129), (128, 128), (129, 128), (200, 300), (256, 256), (256, 32), (257, 511), (500, 1000),
-                                   (1000, 784), (1024, 640), (640, 2000), (1100, 1300)])
+                                   (1000, 784), (1024, 640), (640, 2000), (1100, 1300),
+                                   # around the sizes that one CTA takes: 128 by about 320 at most, longer where narrower
+                                   (16, 16), (17, 64), (48, 65), (10, 2048), (16, 3400), (16, 3500), (30, 1000), (64, 600), (64, 900), (112, 320),
+                                   (128, 320), (128, 321), (320, 128), (64, 512), (64, 513), (513, 20), (120, 340), (2000, 33), (7, 5000), (5000, 12), (60000, 2), (1, 70000)])
 def test_orthogonalize_shapes(g, shape):
     check_ortho(g, [shape])
+
+
+def test_orthogonalize_small_matrices_alone_and_beside_large_ones(g):
+    """The same matrices on one CTA each and riding along with a large one."""
+    shapes = [(33, 90), (100, 128), (12, 700), (1, 9)]
+    check_ortho(g, shapes)
+    check_ortho(g, shapes + [(300, 400)])
+    check_ortho(g, [(3 + i, 40 + 13 * i) for i in range(21)])  # more than one launch takes
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
