@@ -160,6 +160,10 @@ def lib():
         "gl_stop": (None, [vp]),
         "gl_snapshot_submit": (C.c_int, [vp]),
         "gl_snapshot_collect": (C.c_int, [vp, vp, vp, vp, i32]),
+        "gl_set_layer_norm": (C.c_int, [vp, i32, f32]),
+        "gl_set_norm_weights": (C.c_int, [vp, i32, vp, vp]),
+        "gl_get_norm_weights": (C.c_int, [vp, i32, vp, vp]),
+        "gl_set_muon": (C.c_int, [vp, i32, f32, i32, f32, i32]),
         "gl_sync": (C.c_int, [vp]),
         "gl_kernel_launches": (i64, [vp]),
         "gl_tensor_core_launches": (i64, [vp]),
@@ -484,6 +488,24 @@ class Net:
             return None
         _check(st)
         return w, b[: self.H], z
+
+    def set_layer_norm(self, layer, eps=1e-5):
+        """Normalises hidden layer `layer` (1..H); eps < 0 takes the norm out."""
+        _check(lib().gl_set_layer_norm(self.h, layer, eps))
+
+    def set_norm_weights(self, layer, gain, shift):
+        gain, shift = _f32(gain), _f32(shift)
+        assert gain.size == shift.size == self.desc.sizes[layer]
+        _check(lib().gl_set_norm_weights(self.h, layer, _ptr(gain), _ptr(shift)))
+
+    def get_norm_weights(self, layer):
+        gain, shift = np.empty(self.desc.sizes[layer], np.float32), np.empty(self.desc.sizes[layer], np.float32)
+        _check(lib().gl_get_norm_weights(self.h, layer, _ptr(gain), _ptr(shift)))
+        return gain, shift
+
+    def set_muon(self, layer, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5):
+        """Weight layer `layer` (0..H) is updated by the orthogonalised momentum; steps=0: SGD again."""
+        _check(lib().gl_set_muon(self.h, layer, momentum, 1 if nesterov else 0, weight_decay, steps))
 
     def sync(self):
         _check(lib().gl_sync(self.h))

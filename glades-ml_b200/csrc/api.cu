@@ -19,6 +19,7 @@
 
 #include "host_copy.h"
 #include "internal.h"
+#include "orthogonalize.h"
 #include "tc_gemm.h"
 
 using namespace glb;
@@ -266,6 +267,29 @@ struct gl_net
 	std::vector<std::pair<uint64_t, int64_t>> reserved;  // (plan_code, rows) of the passes whose buffers exist
 	int64_t tcLaunches = 0;
 	int64_t lastWindowLaunches = 0;
+	// layer norm of hidden layers (gl_set_layer_norm): what W_l reads of layer l is then dN[l]
+	struct Norm
+	{
+		bool on = false;
+		float eps = 0.0f;
+		float* param = nullptr;  // gain | shift | their sums of the running window, n_l floats each
+		float *y = nullptr, *mean = nullptr, *rstd = nullptr;
+		size_t capY = 0, capMean = 0, capRstd = 0;
+	} norm[GL_MAX_WEIGHT_LAYERS + 1];
+	float* dE = nullptr;             // the error that arrives at a normalised layer's output, and the backward pass's scratch
+	float* normWork = nullptr;
+	size_t capE = 0, capNormWork = 0;
+	// orthogonalised updates (gl_set_muon)
+	struct Muon
+	{
+		bool on = false;
+		float momentum = 0.0f, decay = 0.0f;
+		int nesterov = 0, steps = 0;
+		float* dM = nullptr;         // the layer's momentum, like its weights
+	} muon[GL_MAX_WEIGHT_LAYERS];
+	char* muonWork = nullptr;
+	size_t capMuonWork = 0;
+	bool special = false;            // any of them: the network trains layer by layer
 	// workspace for splitting a partial wave of tiles along k (all tensor-core products of the compute stream)
 	TcSplitK sk = {nullptr, nullptr, nullptr, 0, 0};
 	unsigned skEpoch = 0;
@@ -598,6 +622,12 @@ extern "C" int gl_destroy(gl_net* n)
 	for (int l = 0; l < GL_MAX_WEIGHT_LAYERS; ++l) if (n->evRead[l]) cudaEventDestroy(n->evRead[l]);
 	if (n->evComm) cudaEventDestroy(n->evComm);
 	free_work(n);
+	for (gl_net::Norm& t : n->norm)
+	{
+		cudaFree(t.param); cudaFree(t.y); cudaFree(t.mean); cudaFree(t.rstd);
+	}
+	for (gl_net::Muon& t : n->muon) cudaFree(t.dM);
+	cudaFree(n->dE); cudaFree(n->normWork); cudaFree(n->muonWork);
 	cudaFree(n->dHlen); cudaFree(n->dHlast); cudaFree(n->dErrState); cudaFree(n->dMasks);
 	if (n->snapStream) cudaStreamSynchronize(n->snapStream);
 	cudaFree(n->dPreact); cudaFree(n->dSnap);
@@ -690,6 +720,8 @@ extern "C" int gl_set_weights(gl_net* n, const float* w, const float* bias)
 		CU(cudaMemsetAsync(n->dHlast, 0, (size_t)n->nw * sizeof(float), n->stream));
 		CU(cudaMemsetAsync(n->dErrState, 0, (size_t)n->total_nodes * sizeof(float), n->stream));
 	}
+	for (int l = 0; l <= n->H; ++l)
+		if (n->muon[l].on) CU(cudaMemsetAsync(n->muon[l].dM, 0, (size_t)(n->woff[l + 1] - n->woff[l]) * sizeof(float), n->stream));
 	CU(cudaMemsetAsync(n->dFlags, 0, 4 * sizeof(int), n->stream));
 	if (n->dpArena)  // the owners' sticky "non-finite weight" words belong to the old weights
 		CU(cudaMemsetAsync(n->dpArena + DP_WORD_BAD * sizeof(unsigned), 0, DP_MAX_WORLD * sizeof(unsigned), n->stream));
@@ -731,6 +763,53 @@ struct StateHeader
 };
 }  // namespace
 
+// What a network with normalised layers or orthogonalised updates adds to a checkpoint: two words that say which layers, gains and
+// shifts, momenta.
+static std::vector<float> special_layers(const gl_net* n)
+{
+	uint32_t words[2] = {0, 0};
+	for (int l = 0; l <= n->H; ++l)
+	{
+		words[0] |= (uint32_t)n->norm[l].on << l;
+		words[1] |= (uint32_t)n->muon[l].on << l;
+	}
+	std::vector<float> v(2);
+	memcpy(v.data(), words, sizeof words);
+	return v;
+}
+static size_t special_floats(const gl_net* n)
+{
+	if (!n->special) return 0;
+	size_t c = 2;
+	for (int l = 0; l <= n->H; ++l)
+	{
+		if (n->norm[l].on) c += (size_t)2 * n->d.sizes[l];
+		if (n->muon[l].on) c += (size_t)(n->woff[l + 1] - n->woff[l]);
+	}
+	return c;
+}
+static int special_state(gl_net* n, std::vector<float>& v, bool load)
+{
+	if (!load)
+	{
+		v = special_layers(n);
+		v.resize(special_floats(n));
+	}
+	size_t at = 2;
+	auto move = [&](float* d, size_t count) -> cudaError_t {
+		const cudaError_t e = load ? cudaMemcpy(d, v.data() + at, count * sizeof(float), cudaMemcpyHostToDevice)
+		                           : cudaMemcpy(v.data() + at, d, count * sizeof(float), cudaMemcpyDeviceToHost);
+		at += count;
+		return e;
+	};
+	for (int l = 0; l <= n->H; ++l)
+	{
+		if (n->norm[l].on) CU(move(n->norm[l].param, (size_t)2 * n->d.sizes[l]));
+		if (n->muon[l].on) CU(move(n->muon[l].dM, (size_t)(n->woff[l + 1] - n->woff[l])));
+	}
+	return 0;
+}
+
 extern "C" int gl_save_state(gl_net* n, const char* path)
 {
 	if (!n || !path) return fail(GL_ERR_INVALID, "gl_save_state: bad argument");
@@ -768,6 +847,12 @@ extern "C" int gl_save_state(gl_net* n, const char* path)
 		CU(cudaMemcpy(extra.data() + n->nw, n->dHlast, (size_t)n->nw * sizeof(float), cudaMemcpyDeviceToHost));
 		CU(cudaMemcpy(extra.data() + 2 * n->nw, n->dErrState, (size_t)n->total_nodes * sizeof(float), cudaMemcpyDeviceToHost));
 	}
+	// normalised layers' gains and shifts and the momenta of orthogonalised updates: format "S3", which layers first
+	if (n->special)
+	{
+		memcpy(h.magic, "GLB200S3", 8);
+		if (int r = special_state(n, extra, false)) return r;
+	}
 	FILE* f = fopen(path, "wb");
 	if (!f) return fail(GL_ERR_INVALID, "gl_save_state: cannot open %s for writing", path);
 	const bool ok = fwrite(&h, sizeof h, 1, f) == 1 && fwrite(buf.data(), sizeof(float), buf.size(), f) == buf.size() &&
@@ -783,7 +868,8 @@ extern "C" int gl_load_state(gl_net* n, const char* path)
 	FILE* f = fopen(path, "rb");
 	if (!f) return fail(GL_ERR_INVALID, "gl_load_state: cannot open %s", path);
 	StateHeader h;
-	if (fread(&h, sizeof h, 1, f) != 1 || (memcmp(h.magic, "GLB200S1", 8) != 0 && memcmp(h.magic, "GLB200S2", 8) != 0))
+	if (fread(&h, sizeof h, 1, f) != 1 || (memcmp(h.magic, "GLB200S1", 8) != 0 && memcmp(h.magic, "GLB200S2", 8) != 0 &&
+	                                      memcmp(h.magic, "GLB200S3", 8) != 0))
 	{
 		fclose(f);
 		return fail(GL_ERR_INVALID, "gl_load_state: %s is not a state file", path);
@@ -795,6 +881,13 @@ extern "C" int gl_load_state(gl_net* n, const char* path)
 		return fail(GL_ERR_INVALID, "gl_load_state: %s was written by a network %s dropout, this one is %s", path,
 		            with_dropout ? "with" : "without", n->dropout ? "with" : "without");
 	}
+	const bool special = memcmp(h.magic, "GLB200S3", 8) == 0;
+	if (special != n->special)
+	{
+		fclose(f);
+		return fail(GL_ERR_INVALID, "gl_load_state: %s was written by a network %s normalised layers or orthogonalised updates", path,
+		            special ? "with" : "without");
+	}
 	bool same = h.n_layers == n->d.n_layers && h.nw == n->nw && h.mode == n->d.mode && h.batch_size == n->d.batch_size;
 	for (int l = 0; same && l <= n->H + 1; ++l) same = h.sizes[l] == n->d.sizes[l];
 	const int64_t want_hist = n->dHist ? n->nw * (int64_t)n->d.batch_size : 0;
@@ -804,11 +897,13 @@ extern "C" int gl_load_state(gl_net* n, const char* path)
 		return fail(GL_ERR_INVALID, "gl_load_state: %s was written by a network of another shape, mode or minibatch size", path);
 	}
 	std::vector<float> buf((size_t)n->nw + GL_MAX_WEIGHT_LAYERS + (size_t)h.hist_floats);
-	std::vector<float> extra(with_dropout ? (size_t)2 * n->nw + (size_t)n->total_nodes : 0);
+	std::vector<float> extra(with_dropout ? (size_t)2 * n->nw + (size_t)n->total_nodes : special_floats(n));
 	const bool ok = fread(buf.data(), sizeof(float), buf.size(), f) == buf.size() &&
 	                (extra.empty() || fread(extra.data(), sizeof(float), extra.size(), f) == extra.size());
 	fclose(f);
 	if (!ok) return fail(GL_ERR_INVALID, "gl_load_state: %s is truncated", path);
+	if (special && memcmp(extra.data(), special_layers(n).data(), 2 * sizeof(float)) != 0)
+		return fail(GL_ERR_INVALID, "gl_load_state: %s was written by a network that normalises or orthogonalises other layers", path);
 	// the stored biases are indexed by layer (entry 0 unused); gl_set_weights takes them from hidden layer 1 on.
 	// It also clears the history and the status words.
 	if (int r = gl_set_weights(n, buf.data(), buf.data() + n->nw + 1)) return r;
@@ -824,7 +919,98 @@ extern "C" int gl_load_state(gl_net* n, const char* path)
 		CU(cudaMemcpy(n->dHlast, extra.data() + n->nw, (size_t)n->nw * sizeof(float), cudaMemcpyHostToDevice));
 		CU(cudaMemcpy(n->dErrState, extra.data() + 2 * n->nw, (size_t)n->total_nodes * sizeof(float), cudaMemcpyHostToDevice));
 	}
+	if (special)
+		if (int r = special_state(n, extra, true)) return r;
 	n->epochs = h.epochs;
+	return GL_OK;
+}
+
+// ---- normalised layers and orthogonalised updates ----------------------------------------------------------------
+static int special_allowed(gl_net* n, const char* name)
+{
+	if (!n) return fail(GL_ERR_INVALID, "%s: null handle", name);
+	if (n->d.mode != GL_MODE_BATCHED) return fail(GL_ERR_STATE, "%s needs a batched-mode network", name);
+	if (n->d.gemm == GL_GEMM_GRID_FUSED) return fail(GL_ERR_STATE, "%s: the whole-window kernel has neither normalised layers nor orthogonalised updates", name);
+	if (n->world > 1) return fail(GL_ERR_STATE, "%s: data-parallel networks have neither normalised layers nor orthogonalised updates", name);
+	for (const gl_net::Slot& t : n->slot)
+		if (t.pending) return fail(GL_ERR_STATE, "%s: a submitted window or batch is still in flight", name);
+	return GL_OK;
+}
+static void special_changed(gl_net* n)
+{
+	n->special = false;
+	for (int l = 0; l <= n->H; ++l) n->special = n->special || n->norm[l].on || n->muon[l].on;
+	n->reserved.clear();  // passes need other buffers now
+}
+
+extern "C" int gl_set_layer_norm(gl_net* n, int32_t layer, float eps)
+{
+	if (int r = special_allowed(n, "gl_set_layer_norm")) return r;
+	if (layer < 1 || layer > n->H) return fail(GL_ERR_INVALID, "gl_set_layer_norm: layer %d is no hidden layer", layer);
+	if (eps != eps || isinf(eps)) return fail(GL_ERR_INVALID, "gl_set_layer_norm: eps is no number");
+	if (int r = use_device(n)) return r;
+	gl_net::Norm& t = n->norm[layer];
+	if (eps >= 0.0f)
+	{
+		const size_t w = (size_t)n->d.sizes[layer];
+		if (!t.param) CU(cudaMalloc(&t.param, 4 * w * sizeof(float)));
+		std::vector<float> p(4 * w, 0.0f);
+		std::fill(p.begin(), p.begin() + w, 1.0f);
+		CU(cudaMemcpyAsync(t.param, p.data(), p.size() * sizeof(float), cudaMemcpyHostToDevice, n->stream));
+		CU(cudaStreamSynchronize(n->stream));
+	}
+	t.on = eps >= 0.0f;
+	t.eps = eps;
+	special_changed(n);
+	return GL_OK;
+}
+
+extern "C" int gl_set_norm_weights(gl_net* n, int32_t layer, const float* gain, const float* shift)
+{
+	if (!n || layer < 1 || layer > n->H || !n->norm[layer].on) return fail(GL_ERR_STATE, "gl_set_norm_weights: layer %d is not normalised", layer);
+	if (!gain || !shift) return fail(GL_ERR_INVALID, "gl_set_norm_weights: null argument");
+	if (int r = use_device(n)) return r;
+	const size_t w = (size_t)n->d.sizes[layer];
+	CU(cudaMemcpyAsync(n->norm[layer].param, gain, w * sizeof(float), cudaMemcpyHostToDevice, n->stream));
+	CU(cudaMemcpyAsync(n->norm[layer].param + w, shift, w * sizeof(float), cudaMemcpyHostToDevice, n->stream));
+	CU(cudaStreamSynchronize(n->stream));
+	return GL_OK;
+}
+
+extern "C" int gl_get_norm_weights(gl_net* n, int32_t layer, float* gain, float* shift)
+{
+	if (!n || layer < 1 || layer > n->H || !n->norm[layer].on) return fail(GL_ERR_STATE, "gl_get_norm_weights: layer %d is not normalised", layer);
+	if (!gain || !shift) return fail(GL_ERR_INVALID, "gl_get_norm_weights: null argument");
+	if (int r = use_device(n)) return r;
+	const size_t w = (size_t)n->d.sizes[layer];
+	CU(cudaMemcpyAsync(gain, n->norm[layer].param, w * sizeof(float), cudaMemcpyDeviceToHost, n->stream));
+	CU(cudaMemcpyAsync(shift, n->norm[layer].param + w, w * sizeof(float), cudaMemcpyDeviceToHost, n->stream));
+	CU(cudaStreamSynchronize(n->stream));
+	return GL_OK;
+}
+
+extern "C" int gl_set_muon(gl_net* n, int32_t layer, float momentum, int32_t nesterov, float weight_decay, int32_t steps)
+{
+	if (int r = special_allowed(n, "gl_set_muon")) return r;
+	if (layer < 0 || layer > n->H) return fail(GL_ERR_INVALID, "gl_set_muon: there is no weight layer %d", layer);
+	if (steps < 0 || steps > ORTHO_MAX_STEPS) return fail(GL_ERR_INVALID, "gl_set_muon: steps must be 0 (off) to %d", ORTHO_MAX_STEPS);
+	if (!isfinite(momentum) || !isfinite(weight_decay)) return fail(GL_ERR_INVALID, "gl_set_muon: momentum and weight decay must be numbers");
+	if (steps > 0 && (n->d.momentum[layer] != 0.0f || n->d.wd1[layer] != 0.0f || n->d.wd2[layer] != 0.0f))
+		return fail(GL_ERR_INVALID, "gl_set_muon: layer %d has a momentum or weight decay of its own in the descriptor", layer);
+	if (int r = use_device(n)) return r;
+	gl_net::Muon& t = n->muon[layer];
+	if (steps > 0)
+	{
+		const size_t bytes = (size_t)(n->woff[layer + 1] - n->woff[layer]) * sizeof(float);
+		if (!t.dM) CU(cudaMalloc(&t.dM, bytes));
+		CU(cudaMemsetAsync(t.dM, 0, bytes, n->stream));
+	}
+	t.on = steps > 0;
+	t.momentum = momentum;
+	t.nesterov = nesterov != 0;
+	t.decay = weight_decay;
+	t.steps = steps;
+	special_changed(n);
 	return GL_OK;
 }
 
@@ -1431,6 +1617,32 @@ static int dp_reserve_for(const gl_net* n, int M, int N)
 
 // Forward of `rows` rows starting at device pointer X; the last layer's outputs land in dA[H+1].  Every layer leaves its
 // activations in the forms that the plan's later products read: fp32 (dA), low TF32 parts (dLo), fp16 parts (sA), ReLU bits (dMask).
+// What W_l reads: the inputs, layer l's activations, or their normalisation.
+static const float* layer_input(const gl_net* n, int l, const float* X) { return l == 0 ? X : (n->norm[l].on ? n->norm[l].y : n->dA[l]); }
+
+// dN[l] from the activations of layer l
+static int normalise(gl_net* n, int l, int rows, bool train, int64_t* launches)
+{
+	gl_net::Norm& t = n->norm[l];
+	if (int r = grow_f32(n, &t.y, &t.capY, rows, l)) return r;
+	if (int r = grow(&t.mean, &t.capMean, (size_t)rows * sizeof(float))) return r;
+	if (int r = grow(&t.rstd, &t.capRstd, (size_t)rows * sizeof(float))) return r;
+	LayerNormArgs a = {};
+	a.x = n->dA[l];
+	a.y = t.y;
+	a.ldx = a.ldy = pitch32(n, l);
+	a.gain = t.param;
+	a.shift = t.param + n->d.sizes[l];
+	a.mean = train ? t.mean : nullptr;
+	a.rstd = train ? t.rstd : nullptr;
+	a.rows = rows;
+	a.n = n->d.sizes[l];
+	a.eps = t.eps;
+	GO(launch_layer_norm(a, GL_F32, n->stream));
+	++*launches;
+	return 0;
+}
+
 static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan, bool train, int64_t* launches)
 {
 	if (int r = grow(&n->dArgmax, &n->capArgmax, (size_t)rows * sizeof(int))) return r;
@@ -1492,7 +1704,7 @@ static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan
 	auto next_lo = [&](int l) { return l <= n->H && (plan.fwd[l] == ENG_TF32 || gradient_engine(n, plan, l, X, rows) == ENG_TF32); };
 	auto want_16 = [&](int l) { return (l <= n->H && plan.fwd[l] == ENG_F16) || (plan.bwd16 && l <= n->H); };
 	auto want_32 = [&](int l) {
-		if (l == n->H + 1) return true;
+		if (l == n->H + 1 || n->norm[l].on) return true;
 		if (plan.fwd[l] != ENG_F16) return true;
 		if (!train) return false;
 		const bool decay = n->d.wd1[l] != 0.0f || n->d.wd2[l] != 0.0f;
@@ -1504,7 +1716,14 @@ static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan
 	{
 		if (int r = dp_wait_layer(n, l)) return r;
 		const int N = n->d.sizes[l + 1], K = n->d.sizes[l];
-		const float* in = l == 0 ? X : n->dA[l];
+		const float* in = layer_input(n, l, X);
+		const bool normed = l < n->H && n->norm[l + 1].on;
+		// a normalised layer's parts, as the next product and the backward pass read them
+		auto next_parts = [&]() -> int {
+			if (normed)
+				if (int r = normalise(n, l + 1, rows, train, launches)) return r;
+			return derive(l + 1, layer_input(n, l + 1, X), want_16(l + 1), next_lo(l + 1), next_lo(l + 1) && want_16(l + 2));
+		};
 		const float* bias = (l >= 1) ? n->dBias + l : nullptr;
 		if (want_32(l + 1) || plan.fwd[l] == ENG_FFMA)
 			if (int r = grow_f32(n, &n->dA[l + 1], &n->capA[l + 1], rows, l + 1)) return r;
@@ -1528,9 +1747,9 @@ static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan
 			g.par = n->d.act_param[l];
 			g.chained = n->rowsLast;
 			if (int r = run_ffma(n, g, launches)) return r;
-			n->rowsLast = !n->dry && !n->profile && n->world == 1 && gemm_ffma_by_rows(g) && !(l < n->H && (want_16(l + 1) || next_lo(l + 1)));
+			n->rowsLast = !n->dry && !n->profile && n->world == 1 && gemm_ffma_by_rows(g) && !(l < n->H && (normed || want_16(l + 1) || next_lo(l + 1)));
 			if (l < n->H)
-				if (int r = derive(l + 1, n->dA[l + 1], want_16(l + 1), next_lo(l + 1), next_lo(l + 1) && want_16(l + 2))) return r;
+				if (int r = next_parts()) return r;
 			continue;
 		}
 		n->rowsLast = false;
@@ -1545,7 +1764,7 @@ static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan
 		g.par = n->d.act_param[l];
 		g.ldc = pitch32(n, l + 1);
 		if (want_32(l + 1)) g.C = n->dA[l + 1];
-		if (l < n->H)
+		if (l < n->H && !normed)
 		{
 			g.csc = n->dScales + SC_A + l + 1;
 			have_amax[l + 1] = true;
@@ -1585,6 +1804,8 @@ static int batched_forward(gl_net* n, const float* X, int rows, const Plan& plan
 			const Tf32Operand a = {in, n->dLo[l], pitch32(n, l), 0}, b = {n->dW + n->woff[l], n->dWlo + n->woff[l], K, 0};
 			if (int r = run_tf32(n, g, a, b, launches)) return r;
 		}
+		if (normed)
+			if (int r = next_parts()) return r;
 	}
 	return 0;
 }
@@ -1678,7 +1899,7 @@ static bool grid_fused_fits(const gl_net* n)
 }
 static bool grid_fused_ok(gl_net* n)
 {
-	if (n->world > 1) return false;
+	if (n->world > 1 || n->special) return false;
 	if (n->gfOk < 0)
 	{
 		const char* e = getenv("GLADES_GRID_FUSED");
@@ -1820,6 +2041,68 @@ static int grid_fused_launch(gl_net* n, const float* X, const float* Y, int64_t 
 	return GL_OK;
 }
 
+// The updates that no gradient's epilogue makes: gains and shifts of normalised layers, orthogonalised weight updates.
+static int special_updates(gl_net* n, int rows, int64_t* launches)
+{
+	std::vector<OrthoMatrix> m;
+	for (int l = 0; l <= n->H; ++l)
+	{
+		if (n->norm[l].on)
+		{
+			GO(launch_norm_update(n->norm[l].param, n->d.sizes[l], n->d.lr[l] / (float)rows, n->dFlags, n->stream));
+			++*launches;
+		}
+		if (!n->muon[l].on) continue;
+		OrthoMatrix t = {};
+		t.rows = n->d.sizes[l + 1];
+		t.cols = n->d.sizes[l];
+		t.grad = n->dG + n->woff[l];
+		t.mom = t.mom_out = n->muon[l].dM;
+		t.w = t.w_out = n->dW + n->woff[l];
+		t.ld_grad = t.ld_mom = t.ld_w = t.cols;
+		t.lr = n->d.lr[l] * sqrtf(std::max(1.0f, (float)t.rows / (float)t.cols));
+		m.push_back(t);
+	}
+	// layers of one setting in one call
+	std::vector<bool> done(m.size(), false);
+	for (int l = 0, i = 0; l <= n->H; ++l)
+	{
+		if (!n->muon[l].on) continue;
+		const gl_net::Muon& k = n->muon[l];
+		if (done[i++]) continue;
+		std::vector<OrthoMatrix> same;
+		for (int j = l, q = i - 1; j <= n->H; ++j)
+		{
+			const gl_net::Muon& o = n->muon[j];
+			if (!o.on) continue;
+			if (!done[q] && o.momentum == k.momentum && o.decay == k.decay && o.nesterov == k.nesterov && o.steps == k.steps)
+			{
+				done[q] = true;
+				same.push_back(m[q]);
+			}
+			++q;
+		}
+		OrthoArgs a = {};
+		a.mat = same.data();
+		a.count = (int)same.size();
+		a.steps = k.steps;
+		a.type = GL_F32;
+		a.step = 1;
+		a.nesterov = k.nesterov;
+		a.mu = k.momentum;
+		a.decay = k.decay;
+		a.eps = ORTHO_EPS;
+		a.status = n->dFlags + 1;
+		a.bad = n->dFlags;
+		for (int q = 0; q < k.steps; ++q) memcpy(a.coef[q], ORTHO_QUINTIC, sizeof a.coef[q]);
+		const size_t bytes = ortho_workspace_bytes(a.mat, a.count);
+		if (int r = grow(&n->muonWork, &n->capMuonWork, bytes)) return r;
+		GO(launch_orthogonalize(a, n->muonWork, n->capMuonWork, n->stream));
+		++*launches;
+	}
+	return 0;
+}
+
 static int batched_window(gl_net* n, const float* X, const float* Y, int rows, int64_t metric_rows, gl_metrics* out)
 {
 	DpTrace tr;
@@ -1867,7 +2150,7 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 	tr.mark("start", -1, n->stream);
 	GO(cudaMemsetAsync(sums2, 0, 2 * sizeof(double), n->stream));
 	// (the bias sums of layers whose deltas come from a product that leaves no partial sums are added up there)
-	if (plan.bwdTf) GO(cudaMemsetAsync(n->dG + n->nw, 0, GL_MAX_WEIGHT_LAYERS * sizeof(float), n->stream));
+	if (plan.bwdTf || n->special) GO(cudaMemsetAsync(n->dG + n->nw, 0, GL_MAX_WEIGHT_LAYERS * sizeof(float), n->stream));
 	if (int r = batched_forward(n, X, rows, plan, true, &launches)) return r;
 	tr.mark("forward done", -1, n->stream);
 
@@ -1924,6 +2207,74 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 		const int l = L - 1;
 		const int ni = n->d.sizes[l], no = n->d.sizes[L];
 		const int engine = errprop_engine(n, plan, l, rows);
+		if (n->norm[l].on)
+		{
+			// The product alone, then the norm's backward pass and the activation's derivative.
+			const long long ld = pitch32(n, l);
+			if (int r = grow(&n->dE, &n->capE, (size_t)rows * ld * sizeof(float))) return r;
+			if (int r = grow_f32(n, &n->dD[l], &n->capD[l], rows, l)) return r;
+			if (engine == ENG_FFMA)
+			{
+				GemmArgs g;
+				memset(&g, 0, sizeof g);
+				g.A = n->dD[L]; g.a_sm = pitch32(n, L); g.a_sk = 1;
+				g.B = n->dW + n->woff[l]; g.b_sn = 1; g.b_sk = ni;
+				g.C = n->dE; g.ldc = ld;
+				g.M = rows; g.N = ni; g.K = no;
+				g.epi = EPI_NONE;
+				if (int r = run_ffma(n, g, &launches)) return r;
+			}
+			else
+			{
+				TcGemmArgs g;
+				memset(&g, 0, sizeof g);
+				g.M = rows; g.N = ni; g.K = no;
+				g.epi = EPI_GRAD;  // (a product times alpha)
+				g.alpha = 1.0f;
+				g.C = n->dE;
+				g.ldc = ld;
+				if (engine == ENG_TF32)
+				{
+					if (int r = delta_lo(L)) return r;
+					const Tf32Operand a = {n->dD[L], n->dDlo[L], pitch32(n, L), 0}, b = {n->dW + n->woff[l], n->dWlo + n->woff[l], ni, 1};
+					if (int r = run_tf32(n, g, a, b, &launches)) return r;
+				}
+				else
+				{
+					g.A = operand(n->sD[L], n->dScales + SC_D + L, 0);
+					g.B = operand(n->sW[l], w_scale(n, l), 1);
+					if (int r = run_tc(n, g, &launches)) return r;
+				}
+			}
+			gl_net::Norm& t = n->norm[l];
+			if (int r = grow(&n->normWork, &n->capNormWork, layer_norm_partial_rows(rows, ni) * ni * sizeof(float2))) return r;
+			LayerNormArgs a = {};
+			a.x = n->dA[l];
+			a.dy = n->dE;
+			a.dx = n->dD[l];
+			a.ldx = a.lddy = a.lddx = ld;
+			a.gain = t.param;
+			a.mean = t.mean;
+			a.rstd = t.rstd;
+			a.part = reinterpret_cast<float2*>(n->normWork);
+			a.dgain = t.param + 2 * ni;
+			a.dshift = t.param + 3 * ni;
+			a.rows = rows;
+			a.n = ni;
+			GO(launch_layer_norm_backward(a, GL_F32, n->stream));
+			// (the scale record of D_l was zeroed with the others in front of the forward pass)
+			GO(launch_activation_gradient(n->dD[l], n->dA[l], rows, ni, ld, n->d.activation[l - 1], 0.01f, n->stream));
+			launches += 3;
+			if (tc)
+			{
+				gl_net::Split& s = n->sD[l];
+				if (int r = grow_split(n, s, rows, ni)) return r;
+				GO(launch_amax(n->dD[l], rows, ni, ld, n->dScales + SC_D + l, n->stream));
+				GO(launch_split(n->dD[l], rows, ni, ld, n->dScales + SC_D + l, s.hi, s.lo, s.ld, n->stream));
+				launches += 2;
+			}
+			return 0;
+		}
 		if (engine == ENG_TF32)
 		{
 			if (int r = delta_lo(L)) return r;
@@ -2026,7 +2377,9 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 	auto gradient = [&](int l, bool last) -> int {
 		const int L = l + 1;
 		const int ni = n->d.sizes[l], no = n->d.sizes[L];
-		const float* Al = (l == 0) ? X : n->dA[l];
+		const float* Al = layer_input(n, l, X);
+		const bool muon = n->muon[l].on;  // the mean gradient is stored, its update follows behind all gradients
+		const float alpha = muon ? 1.0f / (float)global_rows : n->d.lr[l];
 		const float* colterm = nullptr;
 		bool fused_store = false;
 		const double decay = fabs((double)n->d.wd1[l]) + fabs((double)n->d.wd2[l]);
@@ -2092,10 +2445,10 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 			}
 			g.M = no; g.N = ni; g.K = rows;
 			g.epi = EPI_GRAD;
-			g.alpha = n->d.lr[l];
+			g.alpha = alpha;
 			g.colterm = colterm;
 			g.sm_reserve = dp_reserve_for(n, no, ni);
-			if (fused_update) update_in_place(g);
+			if (fused_update && !muon) update_in_place(g);
 			else store_gradient(g);
 			if (int r = run_tf32(n, g, a, b, &launches)) return r;
 		}
@@ -2110,9 +2463,9 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 			if (n->scaledD[L]) g.A = n->dDs[L];
 			else g.kscale = n->dC[l];
 			g.epi = EPI_GRAD;
-			g.alpha = n->d.lr[l];
+			g.alpha = alpha;
 			g.colterm = colterm;
-			if (fused_update)
+			if (fused_update && !muon)
 			{
 				g.W = n->dW + n->woff[l];
 				g.inv_mb = 1.0f / (float)global_rows;
@@ -2137,11 +2490,11 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 			g.B = operand(n->sA[l], n->dScales + SC_A + l, 1);
 			g.M = no; g.N = ni; g.K = rows;
 			g.epi = EPI_GRAD;
-			g.alpha = n->d.lr[l];
+			g.alpha = alpha;
 			g.colterm = colterm;
 			g.decay_bound = (float)(decay * fabs((double)n->d.lr[l]) * (double)n->cSum[l]);
 			g.sm_reserve = dp_reserve_for(n, no, ni);
-			if (fused_update) update_in_place(g);
+			if (fused_update && !muon) update_in_place(g);
 			else store_gradient(g);
 			if (int r = run_tc(n, g, &launches)) return r;
 		}
@@ -2281,6 +2634,8 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 		for (int oi = 0; oi <= n->H; ++oi)
 			if (int r = gradient(order[oi], oi == n->H)) return r;
 	}
+	if (n->special)
+		if (int r = special_updates(n, global_rows, &launches)) return r;
 	if (n->dry) return GL_OK;
 	// scalar biases: this rank's sums, and on one GPU the update
 	auto finish_biases = [&](int apply) -> int {
@@ -2352,7 +2707,7 @@ static int batched_window(gl_net* n, const float* X, const float* Y, int rows, i
 			n->wPar ^= 1;
 			for (int l = 0; l <= n->H; ++l)
 			{
-				const bool tensor = gradient_engine(n, plan, l, X, rows) != ENG_FFMA;
+				const bool tensor = gradient_engine(n, plan, l, X, rows) != ENG_FFMA && !n->muon[l].on;
 				n->w16[l] = tensor && wants_w16(plan, l);
 				n->wLo[l] = tensor && wants_wlo(n, plan, l, rows);
 				n->wAmax[l] = tensor;
@@ -2501,7 +2856,7 @@ extern "C" int gl_train_window_host_result(gl_net* n, gl_metrics* out)
 // of the fused kernel (GLADES_SMALL_FUSED=0 keeps the per-layer kernels instead).
 static bool small_fused_ok(const gl_net* n)
 {
-	if (n->world > 1 || n->d.gemm == GL_GEMM_TCGEN05 || n->d.gemm == GL_GEMM_GRID_FUSED) return false;
+	if (n->world > 1 || n->special || n->d.gemm == GL_GEMM_TCGEN05 || n->d.gemm == GL_GEMM_GRID_FUSED) return false;
 	static int enabled = -1;
 	if (enabled < 0)
 	{
@@ -3241,6 +3596,7 @@ extern "C" int gl_dp_unique_id(void* id128)
 
 extern "C" int gl_dp_init(gl_net* n, int32_t rank, int32_t world, const void* id128)
 {
+	if (n && n->special) return fail(GL_ERR_STATE, "gl_dp_init: normalised layers and orthogonalised updates train on one GPU");
 	if (!n || !id128 || world < 1 || rank < 0 || rank >= world) return fail(GL_ERR_INVALID, "gl_dp_init: bad argument");
 	if (n->d.mode != GL_MODE_BATCHED) return fail(GL_ERR_STATE, "data parallelism needs a batched-mode network");
 	if (int r = use_device(n)) return r;
@@ -3402,6 +3758,8 @@ extern "C" int gl_snapshot_submit(gl_net* n)
 {
 	if (!n) return fail(GL_ERR_INVALID, "gl_snapshot_submit: null handle");
 	if (n->snapPending) return fail(GL_ERR_STATE, "a snapshot is already in flight: collect it first");
+	for (int l = 1; l <= n->H; ++l)
+		if (n->norm[l].on) return fail(GL_ERR_STATE, "gl_snapshot_submit: pre-activations of a network with normalised layers are not evaluated");
 	if (int r = use_device(n)) return r;
 	if (int r = dp_join(n)) return r;
 	if (!n->snapStream)

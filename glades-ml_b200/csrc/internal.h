@@ -350,6 +350,11 @@ size_t layer_norm_partial_rows(long long rows, int n);
 cudaError_t launch_layer_norm(const LayerNormArgs& a, int type, cudaStream_t s);
 cudaError_t launch_layer_norm_backward(const LayerNormArgs& a, int type, cudaStream_t s);
 
+// D *= derivative of the activation whose values are A, both [rows][n] of pitch ld
+cudaError_t launch_activation_gradient(float* D, const float* A, long long rows, int n, long long ld, int act, float par, cudaStream_t s);
+// param: gain | shift | dgain | dshift of n floats each; gain and shift -= step * their sums; flags[0] on a new value that is not finite
+cudaError_t launch_norm_update(float* param, int n, float step, int* flags, cudaStream_t s);
+
 // ---- errors of entry points outside api.cu: the text that gl_last_error() returns; returns code
 int report_error(int code, const char* fmt, ...);
 

@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "common.cuh"
 #include "internal.h"
 
 namespace glb {
@@ -420,6 +421,21 @@ __global__ void __launch_bounds__(LN_THREADS) norm_columns_kernel(const float2* 
 	if (dshift) dshift[c] = t.y;
 }
 
+// ---- a network's training step around them ------------------------------------------------------------------------
+__global__ void __launch_bounds__(LN_THREADS) activation_gradient_kernel(float* D, const float* A, long long rows, int n, long long ld, int act, float par)
+{
+	for (long long r = blockIdx.y; r < rows; r += gridDim.y)
+		for (int c = blockIdx.x * LN_THREADS + threadIdx.x; c < n; c += gridDim.x * LN_THREADS) D[r * ld + c] *= act_der_b(A[r * ld + c], act, par);
+}
+__global__ void __launch_bounds__(LN_THREADS) norm_update_kernel(float* param, int n, float step, int* flags)
+{
+	const int i = blockIdx.x * LN_THREADS + threadIdx.x;  // gain | shift
+	if (i >= 2 * n) return;
+	const float v = fmaf(-step, param[2 * (long long)n + i], param[i]);
+	param[i] = v;
+	if (!isfinite(v)) atomicOr(flags, 1);
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------
 // Lanes of a row: in one warp a power of two, else whole warps.
 int group_lanes(int n, int elems)
@@ -556,6 +572,19 @@ cudaError_t launch_layer_norm_backward(const LayerNormArgs& a, int type, cudaStr
 	if (type == GL_F32) return backward_type<float>(a, s);
 	if (type == GL_BF16) return backward_type<__nv_bfloat16>(a, s);
 	return backward_type<__half>(a, s);
+}
+
+cudaError_t launch_activation_gradient(float* D, const float* A, long long rows, int n, long long ld, int act, float par, cudaStream_t s)
+{
+	const dim3 grid((unsigned)((n + LN_THREADS - 1) / LN_THREADS), (unsigned)(rows < 4096 ? rows : 4096));
+	activation_gradient_kernel<<<grid, LN_THREADS, 0, s>>>(D, A, rows, n, ld, act, par);
+	return cudaGetLastError();
+}
+
+cudaError_t launch_norm_update(float* param, int n, float step, int* flags, cudaStream_t s)
+{
+	norm_update_kernel<<<(unsigned)((2 * (long long)n + LN_THREADS - 1) / LN_THREADS), LN_THREADS, 0, s>>>(param, n, step, flags);
+	return cudaGetLastError();
 }
 
 }  // namespace glb

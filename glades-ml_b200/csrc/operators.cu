@@ -67,15 +67,13 @@ int finish(const char* name, cudaError_t e)
 	return report_error(GL_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
-const float kQuintic[3] = {3.4445f, -4.7750f, 2.0315f};
-
 int check_steps(const char* name, OrthoArgs& a, const float* coefficients, int steps, float eps, int type)
 {
 	if (steps < 1 || steps > ORTHO_MAX_STEPS) return report_error(GL_ERR_INVALID, "%s: steps must be 1 to %d", name, ORTHO_MAX_STEPS);
 	if (!type_ok(type)) return report_error(GL_ERR_INVALID, "%s: unknown element type %d", name, type);
 	if (!(eps >= 0.0f) || isinf(eps)) return report_error(GL_ERR_INVALID, "%s: eps must be a number >= 0", name);
 	for (int k = 0; k < steps; ++k)
-		for (int j = 0; j < 3; ++j) a.coef[k][j] = coefficients ? coefficients[3 * k + j] : kQuintic[j];
+		for (int j = 0; j < 3; ++j) a.coef[k][j] = coefficients ? coefficients[3 * k + j] : ORTHO_QUINTIC[j];
 	if (!ortho_coefficients_ok(a.coef, steps))
 		return report_error(GL_ERR_INVALID, "%s: under these coefficients a singular value could grow beyond 16", name);
 	a.steps = steps;

@@ -37,6 +37,7 @@ struct SmParams
 	int count, type, step, nesterov, reset;
 	float mu, decay, eps, s0;
 	int* status;
+	int* bad;
 };
 
 __host__ __device__ inline int small_part(int rows) { return rows * 128; }  // bytes of hi (or lo) of a chunk
@@ -415,7 +416,11 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 				if (P.step)
 				{
 #pragma unroll
-					for (int j = 0; j < 4; ++j) x[j] = fmaf(-m.lr, x[j], keep * w[k][j]);
+					for (int j = 0; j < 4; ++j)
+					{
+						x[j] = fmaf(-m.lr, x[j], keep * w[k][j]);
+						if (P.bad && j < left && !isfinite(x[j])) atomicOr(P.bad, 1);
+					}
 					store4(m.w_out, r * m.ld_w + c, ww, left, x);
 				}
 				else if (P.type == GL_F32) store4(static_cast<float*>(m.out), r * m.ld_out + c, wo, left, x);
@@ -470,6 +475,7 @@ cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float 
 	P.mu = a.mu;
 	P.decay = a.decay;
 	P.eps = a.eps;
+	P.bad = a.bad;
 	P.s0 = s0;
 	P.status = status;
 	size_t smem = 0;

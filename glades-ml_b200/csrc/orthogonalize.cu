@@ -98,6 +98,7 @@ struct OrParams
 	int type, step, nesterov, reset;
 	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
+	int* bad;
 	double* sums;  // [matrix][grid] sums of squares
 	float4* part;  // parts of split tiles
 };
@@ -321,8 +322,9 @@ __device__ __forceinline__ void store_result(const float (&v)[32], void* out, lo
 			else static_cast<__half*>(out)[i + j * ld] = __float2half_rn(v[j]);
 		}
 }
-__device__ __forceinline__ void update_weights(const float (&v)[32], const OrthoMatrix& m, float decay, int r, int c)
+__device__ __forceinline__ void update_weights(const float (&v)[32], const OrthoMatrix& m, float decay, int* bad, int r, int c)
 {
+	bool finite = true;
 	if (c >= m.cols) return;
 	const int n = m.rows - r;
 	const float keep = 1.0f - m.lr * decay;
@@ -336,8 +338,14 @@ __device__ __forceinline__ void update_weights(const float (&v)[32], const Ortho
 		for (int j = 0; j < 16; ++j) x[j] = b + j < n ? w[(b + j) * m.ld_w] : 0.0f;
 #pragma unroll
 		for (int j = 0; j < 16; ++j)
-			if (b + j < n) o[(b + j) * m.ld_w] = fmaf(-m.lr, v[b + j], keep * x[j]);
+			if (b + j < n)
+			{
+				const float y = fmaf(-m.lr, v[b + j], keep * x[j]);
+				finite = finite && isfinite(y);
+				o[(b + j) * m.ld_w] = y;
+			}
 	}
+	if (bad && !finite) atomicOr(bad, 1);
 }
 
 // What the epilogue needs of an operation and its matrix, asked for before the products are awaited: the parameters lie in
@@ -374,7 +382,7 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, int mat, const O
 		if (!M.tall) transpose(v, area, lane);
 		// a wide matrix: lane = column, v = rows r0 ..; a tall one is transposed already: lane = its column, v = its rows c0 ..
 		const int r = M.tall ? c0 : r0, c = (M.tall ? r0 : c0) + lane;
-		if (P.step) update_weights(v, M.m, P.decay, r, c);
+		if (P.step) update_weights(v, M.m, P.decay, P.bad, r, c);
 		else if (P.type == GL_F32) store_result<GL_F32>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
 		else if (P.type == GL_BF16) store_result<GL_BF16>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
 		else store_result<GL_F16>(v, M.m.out, M.m.ld_out, r, c, M.m.rows, M.m.cols);
@@ -1135,6 +1143,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.mu = a.mu;
 	P.decay = a.decay;
 	P.eps = a.eps;
+	P.bad = a.bad;
 	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
 	for (int i = 0; i < count; ++i)
 	{

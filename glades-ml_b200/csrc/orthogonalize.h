@@ -6,6 +6,8 @@ namespace glb {
 
 constexpr int ORTHO_MAX_MATRICES = GL_MAX_WEIGHT_LAYERS;  // of one launch
 constexpr int ORTHO_MAX_STEPS = 16;
+constexpr float ORTHO_QUINTIC[3] = {3.4445f, -4.7750f, 2.0315f};  // the usual coefficients
+constexpr float ORTHO_EPS = 1e-7f;
 
 // One row-major matrix.  Orthogonalisation: out = O(grad).  Update step: mom_out = mu mom + grad,
 // w_out = (1 - lr decay) w - lr O(u) with u = grad + mu mom_out (nesterov) or mom_out.
@@ -30,6 +32,7 @@ struct OrthoArgs
 	int count, steps, type, step, nesterov;
 	float mu, decay, eps;
 	float coef[ORTHO_MAX_STEPS][3];
+	int* bad;     // device word whose bit 0 a new weight that is not finite sets, or NULL
 	int* status;  // device word that a wait that runs out raises, or NULL: the workspace's
 };
 // false where the coefficients let a singular value of [0, 1] (or an eigenvalue on the way) leave the range that the parts are

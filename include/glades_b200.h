@@ -300,6 +300,23 @@ const char* gl_matmul_static_error(void);
 int gl_snapshot_submit(gl_net* net);
 int gl_snapshot_collect(gl_net* net, float* w, float* bias, float* preact, int32_t wait);
 
+/* ---- normalised layers and orthogonalised updates (batched mode, one GPU) ---------------- */
+/* Neither has a counterpart in the reference.  A network that uses them trains and answers layer by layer (never on the
+ * fused whole-network and whole-window kernels, so not with GL_GEMM_GRID_FUSED); it cannot join a data-parallel group.
+ *
+ * gl_set_layer_norm: W_layer reads the layer norm of hidden layer `layer`'s (1..H) activations (see gl_layer_norm) instead of
+ * the activations themselves, in training and in inference.  Gain and shift start at one and zero and are updated after every
+ * window by plain SGD, g -= lr[layer] * dg / rows.  eps < 0 takes the norm out again.  gl_get_activations still gives the
+ * activations; gl_snapshot_submit is refused. */
+int gl_set_layer_norm(gl_net* net, int32_t layer, float eps);
+int gl_set_norm_weights(gl_net* net, int32_t layer, const float* gain, const float* shift);
+int gl_get_norm_weights(gl_net* net, int32_t layer, float* gain, float* shift);
+/* gl_set_muon: weight layer `layer` (0..H) is updated by gl_muon_step on the window's mean gradient, with learning rate
+ * lr[layer] * sqrt(max(1, n_out / n_in)) and the usual coefficients, instead of SGD.  The descriptor's momentum and weight
+ * decay of that layer must be 0.  The momentum starts at zero and again with gl_set_weights; steps == 0 goes back to SGD.
+ * gl_save_state / gl_load_state carry gains, shifts and momenta between networks that are set up alike. */
+int gl_set_muon(gl_net* net, int32_t layer, float momentum, int32_t nesterov, float weight_decay, int32_t steps);
+
 /* Replaces NNetwork::stop (network.cpp:99-102): async-signal-safe; the flag is looked at between
  * epochs of gl_train_epochs. */
 void gl_stop(gl_net* net);
