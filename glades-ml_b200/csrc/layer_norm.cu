@@ -5,44 +5,17 @@
 // A row is held in registers by a group of lanes, so that its statistics cost no second read: the variance is the mean of
 // (x - mu)^2, not a difference of two large sums.  Everything between the loads and the stores is fp32, each result is
 // rounded to the tensors' type once.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <algorithm>
 
-#include "common.cuh"
-#include "internal.h"
+#include "layer_norm.cuh"
 
 namespace glb {
 namespace {
 
-constexpr int LN_SMS = 148;
 constexpr int LN_THREADS = 256;     // threads of a CTA that holds several groups
-constexpr int LN_GROUP_MAX = 512;   // lanes of the largest group
-constexpr int LN_ELEMS = 16;        // values of a row that a lane holds
-constexpr int LN_ELEMS_LONG = 32;   // forward, rows too long for 512 lanes of 16
-
-// VEC neighbouring values of type T as one load or store
-template <int BYTES> struct Word;
-template <> struct Word<2> { typedef unsigned short type; };
-template <> struct Word<4> { typedef unsigned type; };
-template <> struct Word<16> { typedef uint4 type; };
-
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <class T, int VEC>
-struct Pack
-{
-	typename Word<sizeof(T) * VEC>::type w;
-	__device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const decltype(w)*>(p); }
-	__device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(w)*>(p) = w; }
-	__device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T*>(&w)[i]); }
-	__device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&w)[i] = from_float<T>(v); }
-};
+constexpr int LN_GROUP_MAX = 512;   // lanes of the largest group (forward: LN_THREADS)
+constexpr int LN_SLICES = 32;       // of the backward pass's partial rows, added side by side
+constexpr int LN_ELEMS = 16;        // values of a row that a lane holds in the backward pass
 
 // The lanes that share a row.  Groups of at most 32 lanes (a power of two) lie in one warp; larger ones are whole warps of one
 // CTA and meet at a barrier of their own (number 1 + group), their sums in `slot`.
@@ -57,7 +30,30 @@ struct Group
 		lane = (int)threadIdx.x - index * size;
 		slot = shared + index * 2 * ((size + 31) / 32);
 	}
-	// the two sums over the group, on every lane, added in the same order whatever lane asks
+	// the sum over the group, on every lane
+	template <bool WIDE>
+	__device__ __forceinline__ float sum(float a)
+	{
+		if constexpr (!WIDE)
+		{
+			for (int o = size >> 1; o > 0; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+			return a;
+		}
+		else
+		{
+			a = warp_sum(a);
+			const int warps = size >> 5;
+			float* s = reinterpret_cast<float*>(slot + turn * warps);
+			turn ^= 1;
+			if ((lane & 31) == 0) s[lane >> 5] = a;
+			asm volatile("bar.sync %0, %1;" ::"r"(1 + index), "r"(size) : "memory");
+			a = (lane & 15) < warps ? s[lane & 15] : 0.0f;  // at most 16 warps: both half warps add them
+#pragma unroll
+			for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+			return a;
+		}
+	}
+	// two sums over the group
 	template <bool WIDE>
 	__device__ __forceinline__ float2 sum(float a, float b)
 	{
@@ -98,40 +94,131 @@ struct Group
 };
 
 // ---- forward -------------------------------------------------------------------------------------------------
-// Groups walk the rows; a row's values are asked for before the row in front is worked on (the loads of one row alone leave
-// HBM idle for as long as its sums take).  Gain and shift stay in registers.
-template <class T, int VEC, int ELEMS, bool WIDE>
-__global__ void __launch_bounds__(LN_GROUP_MAX) norm_kernel(const LayerNormArgs p, int group)
+// How a row is read: 16 bytes at a time; words of two 16-bit values, for rows that begin on any boundary (the row's whole words are then
+// its elements 2 w + odd and 2 w + odd + 1, odd = 1 where the row begins in the middle of a word; the one or two values beside them are
+// `edge`s of the group's first two lanes); value by value, two values that lie a group apart then make a pair.
+enum { BY_QUADS = 0, BY_WORDS = 1, BY_VALUES = 2 };
+
+// elements of an access
+template <class T> __host__ __device__ constexpr int access_elems(int mode) { return mode == BY_QUADS ? 16 / (int)sizeof(T) : 2; }
+// A lane's accesses to a row: `first` element of the first one; the others lie multiples of group * VEC further; a pair's second
+// element lies `second` behind its first.  all(k): the access that lies k further is the row's; one(k): its first value alone is.
+template <class T, int MODE>
+struct RowPlace
 {
-	constexpr int V = ELEMS / VEC;
-	constexpr bool KEEP = ELEMS == LN_ELEMS;
+	static constexpr int VEC = access_elems<T>(MODE);
+	int first, n, second, edge;
+	__device__ __forceinline__ RowPlace(const void* x, long long ldx, long long rows, int width, long long row, const Group& g)
+	{
+		const int odd = MODE == BY_WORDS ? (int)(((uintptr_t)x >> 1) + row * ldx) & 1 : 0;
+		first = MODE == BY_VALUES ? g.lane : g.lane * VEC + odd;
+		second = MODE == BY_VALUES ? g.size : 1;
+		n = row < rows ? width : 0;
+		edge = -1;
+		if (MODE == BY_WORDS && n > 0)
+		{
+			if (g.lane == 0 && odd) edge = 0;
+			if (g.lane == 1 && ((n - odd) & 1)) edge = n - 1;
+		}
+	}
+	__device__ __forceinline__ bool all(int k) const { return first + k + (MODE == BY_QUADS ? 0 : second) < n; }
+	__device__ __forceinline__ bool one(int k) const { return MODE == BY_VALUES && first + k < n && !all(k); }
+	// the access that lies k further of the row that begins at `row`; what is not the row's becomes zero
+	__device__ __forceinline__ void load(const T* row, int k, Pack<T, VEC>& a) const
+	{
+		const T* x = row + first + k;
+		a.clear();
+		if constexpr (MODE != BY_VALUES)
+		{
+			if (all(k)) a.load(x);
+		}
+		else
+		{
+			if (first + k < n) a.put(0, x[0]);
+			if (all(k)) a.put(1, x[second]);
+		}
+	}
+	__device__ __forceinline__ void store(T* row, int k, f32x2 const (&y)[VEC / 2]) const
+	{
+		T* x = row + first + k;
+		if constexpr (MODE != BY_VALUES)
+		{
+			Pack<T, VEC> o;
+#pragma unroll
+			for (int i = 0; i < VEC / 2; ++i) o.set_pair(i, y[i]);
+			if (all(k)) o.store(x);
+		}
+		else
+		{
+			float lo, hi;
+			unpair2(y[0], lo, hi);
+			if (first + k < n) x[0] = from_float<T>(lo);
+			if (all(k)) x[second] = from_float<T>(hi);
+		}
+	}
+	// a pair of differences without what is not the row's
+	__device__ __forceinline__ f32x2 mask(f32x2 d, int k) const
+	{
+		if (all(k)) return d;
+		if (!one(k)) return pair2(0.0f, 0.0f);
+		float lo, hi;
+		unpair2(d, lo, hi);
+		return pair2(lo, 0.0f);
+	}
+	__device__ __forceinline__ T load_edge(const T* row) const { return edge >= 0 ? row[edge] : from_float<T>(0.0f); }
+	// elements e and e + second of a vector of the row's columns, or `none` where there is no vector
+	__device__ __forceinline__ f32x2 columns(const float* v, int e, float none) const
+	{
+		return pair2(v && e < n ? v[e] : none, v && e + second < n ? v[e + second] : none);
+	}
+};
+
+// Groups walk the rows; a row is asked for before the row in front is worked on.  Beside HBM its instructions bound the kernel: two
+// elements are worked on in one (f32x2), and gain and shift of 16-bit types stay in registers (a group only sees rows that begin on
+// the same half of a word); fp32 rows have half the elements per byte, and the registers serve them better as loads under way.
+//   fp32 8192 x 4096: 47 to 49 us, 5.5 to 5.7 TB/s (gain and shift in registers 54; 32 elements per lane 52)
+//   bf16 8192 x 4096: 33 us; each further 8192 rows 24, of which the copy of as many bytes takes 20.5 (one value per instruction 50;
+//                     32 elements per lane, gain and shift from L1, 36; a warp per row, or rows through shared memory, 43 to 50)
+//   bf16 10007 x 1025: 21 us (words with a branch for the halves 31; one value at a time 42)
+template <class T, int MODE, int ELEMS, bool WIDE>
+__global__ void __launch_bounds__(LN_THREADS, ELEMS == 16 ? 3 : 2) norm_kernel(const LayerNormArgs p, int group)
+{
+	constexpr int VEC = access_elems<T>(MODE), V = ELEMS / VEC, PAIRS = VEC / 2;  // elements of an access, accesses of a lane
 	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
 	Group gr(group, slots);
 	const int groups = blockDim.x / group;
 	const long long step = (long long)gridDim.x * groups;
-	const T* X = static_cast<const T*>(p.x);
-	T* Y = static_cast<T*>(p.y);
 	const float inv_n = 1.0f / (float)p.n;
-	float gain[KEEP ? ELEMS : 1], shift[KEEP ? ELEMS : 1];
-	if (KEEP)
+	const bool quads = MODE == BY_QUADS && (((uintptr_t)p.gain | (uintptr_t)p.shift) & 15) == 0 && p.gain && p.shift;
+	typedef RowPlace<T, MODE> Place;
+	constexpr bool KEEP = ELEMS == 16 && sizeof(T) == 2, EDGE = MODE == BY_WORDS;
+	float gain_e = 1.0f, shift_e = 0.0f;
+	T edge = from_float<T>(0.0f);
+	f32x2 gain[KEEP ? V : 1][PAIRS], shift[KEEP ? V : 1][PAIRS];
+	if (KEEP || EDGE)
 	{
+		const Place at(p.x, p.ldx, p.rows, p.n, (long long)blockIdx.x * groups + gr.index, gr);
+		if (EDGE && at.edge >= 0)
+		{
+			if (p.gain) gain_e = p.gain[at.edge];
+			if (p.shift) shift_e = p.shift[at.edge];
+		}
 #pragma unroll
-		for (int v = 0; v < V; ++v)
+		for (int v = 0; v < (KEEP ? V : 0); ++v)
 #pragma unroll
-			for (int i = 0; i < VEC; ++i)
+			for (int i = 0; i < PAIRS; ++i)
 			{
-				const int c = (v * group + gr.lane) * VEC + i;
-				gain[v * VEC + i] = p.gain && c < p.n ? p.gain[c] : 1.0f;
-				shift[v * VEC + i] = p.shift && c < p.n ? p.shift[c] : 0.0f;
+				const int e = at.first + v * group * VEC + 2 * i;
+				gain[KEEP ? v : 0][i] = at.columns(p.gain, e, 1.0f);
+				shift[KEEP ? v : 0][i] = at.columns(p.shift, e, 0.0f);
 			}
 	}
 	auto fetch = [&](long long row, Pack<T, VEC>(&a)[V]) {
+		const Place at(p.x, p.ldx, p.rows, p.n, row, gr);
+		const T* x = static_cast<const T*>(p.x) + row * p.ldx;
 #pragma unroll
-		for (int v = 0; v < V; ++v)
-		{
-			const int c = (v * group + gr.lane) * VEC;
-			if (row < p.rows && c < p.n) a[v].load(X + row * p.ldx + c);
-		}
+		for (int v = 0; v < V; ++v) at.load(x, v * group * VEC, a[v]);
+		if (EDGE) edge = at.load_edge(x);
 	};
 	long long row = (long long)blockIdx.x * groups + gr.index;
 	Pack<T, VEC> next[V];
@@ -140,47 +227,79 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_kernel(const LayerNormArgs 
 	const long long walk = WIDE ? row : (long long)blockIdx.x * groups + ((int)threadIdx.x & ~31) / group;
 	for (long long first = walk; first < p.rows; first += step, row += step)
 	{
-		float x[ELEMS];
-		float s = 0.0f;
+		const Place at(p.x, p.ldx, p.rows, p.n, row, gr);
+		f32x2 x[V][PAIRS];
+		f32x2 s0 = pair2(0.0f, 0.0f), s1 = s0;
 #pragma unroll
 		for (int v = 0; v < V; ++v)
 #pragma unroll
-			for (int i = 0; i < VEC; ++i)
+			for (int i = 0; i < PAIRS; ++i)
 			{
-				const bool in = row < p.rows && (v * group + gr.lane) * VEC < p.n;
-				x[v * VEC + i] = in ? next[v].get(i) : 0.0f;
-				s += x[v * VEC + i];
+				x[v][i] = next[v].pair(i);
+				if ((v + i) & 1) s1 = add2(s1, x[v][i]);
+				else s0 = add2(s0, x[v][i]);
 			}
+		float a, b, xe = to_float(edge);
 		fetch(row + step, next);
-		const float mean = gr.sum<WIDE>(s, 0.0f).x / (float)p.n;  // (a division: a row of equal values keeps its mean)
-		float q = 0.0f;
-#pragma unroll
-		for (int v = 0; v < V; ++v)
-#pragma unroll
-			for (int i = 0; i < VEC; ++i)
-				if ((v * group + gr.lane) * VEC < p.n)
-				{
-					const float d = x[v * VEC + i] - mean;
-					q = fmaf(d, d, q);
-				}
-		const float rstd = 1.0f / sqrtf(gr.sum<WIDE>(q, 0.0f).x * inv_n + p.eps);
-		if (row >= p.rows) continue;
+		unpair2(add2(s0, s1), a, b);
+		if (EDGE) a += xe;
+		// s / n, with the quotient's remainder: a row of equal values keeps its mean
+		const float sum = gr.sum<WIDE>(a + b);
+		float mean = sum * inv_n;
+		if (fabsf(sum) <= 3.0e38f) mean = fmaf(fmaf(-mean, (float)p.n, sum), inv_n, mean);
+		const f32x2 minus = pair2(-mean, -mean);
+		s0 = s1 = pair2(0.0f, 0.0f);
 #pragma unroll
 		for (int v = 0; v < V; ++v)
 		{
-			const int c = (v * group + gr.lane) * VEC;
-			if (c >= p.n) continue;
-			Pack<T, VEC> o;
+			const int k = v * group * VEC;
 #pragma unroll
-			for (int i = 0; i < VEC; ++i)
+			for (int i = 0; i < PAIRS; ++i)
 			{
-				const float ga = KEEP ? gain[KEEP ? v * VEC + i : 0] : (p.gain ? p.gain[c + i] : 1.0f);
-				const float sh = KEEP ? shift[KEEP ? v * VEC + i : 0] : (p.shift ? p.shift[c + i] : 0.0f);
-				o.set(i, fmaf((x[v * VEC + i] - mean) * rstd, ga, sh));
+				x[v][i] = add2(x[v][i], minus);
+				const f32x2 d = at.mask(x[v][i], k);
+				if ((v + i) & 1) s1 = fma2(d, d, s1);
+				else s0 = fma2(d, d, s0);
 			}
-			o.store(Y + row * p.ldy + c);
 		}
-		if (gr.lane == 0)
+		unpair2(add2(s0, s1), a, b);
+		if (EDGE)
+		{
+			xe = at.edge >= 0 ? xe - mean : 0.0f;
+			a = fmaf(xe, xe, a);
+		}
+		const float rstd = inverse_root(fmaf(gr.sum<WIDE>(a + b), inv_n, p.eps));
+		const f32x2 scale = pair2(rstd, rstd);
+		T* y = static_cast<T*>(p.y) + row * p.ldy;
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+		{
+			const int k = v * group * VEC, c = at.first + k;
+			f32x2 o[PAIRS];
+			if (KEEP)
+			{
+#pragma unroll
+				for (int i = 0; i < PAIRS; ++i) o[i] = fma2(mul2(x[v][i], scale), gain[KEEP ? v : 0][i], shift[KEEP ? v : 0][i]);
+			}
+			else if (quads && at.all(k))
+			{
+#pragma unroll
+				for (int i = 0; i + 1 < PAIRS; i += 2)
+				{
+					const float4 ga = *reinterpret_cast<const float4*>(p.gain + c + 2 * i), sh = *reinterpret_cast<const float4*>(p.shift + c + 2 * i);
+					o[i] = fma2(mul2(x[v][i], scale), pair2(ga.x, ga.y), pair2(sh.x, sh.y));
+					o[i + 1 < PAIRS ? i + 1 : i] = fma2(mul2(x[v][i + 1 < PAIRS ? i + 1 : i], scale), pair2(ga.z, ga.w), pair2(sh.z, sh.w));
+				}
+			}
+			else
+			{
+#pragma unroll
+				for (int i = 0; i < PAIRS; ++i) o[i] = fma2(mul2(x[v][i], scale), at.columns(p.gain, c + 2 * i, 1.0f), at.columns(p.shift, c + 2 * i, 0.0f));
+			}
+			at.store(y, k, o);
+		}
+		if (EDGE && at.edge >= 0) y[at.edge] = from_float<T>(fmaf(xe * rstd, gain_e, shift_e));
+		if (gr.lane == 0 && at.n > 0)
 		{
 			if (p.mean) p.mean[row] = mean;
 			if (p.rstd) p.rstd[row] = rstd;
@@ -188,29 +307,87 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_kernel(const LayerNormArgs 
 	}
 }
 
-// Rows too long for a group's registers: one CTA per row reads it three times (the second and third time from L2).
-template <class T>
+// Rows too long for a group's registers: one CTA per row reads it three times (the second and third time from L2), 16 bytes at a time
+// where every row allows it.  bf16, 800 x 40000: 44 us; value by value 69.
+template <class T, int VEC>
+__device__ __forceinline__ void load_values(const T* p, float (&f)[VEC])
+{
+	if constexpr (VEC == 1) f[0] = to_float(p[0]);
+	else
+	{
+		Pack<T, VEC> a;
+		a.load(p);
+#pragma unroll
+		for (int i = 0; i < VEC / 2; ++i) unpair2(a.pair(i), f[2 * i], f[2 * i + 1]);
+	}
+}
+// VEC values of a vector of the columns, or `none` where there is no vector
+template <int VEC>
+__device__ __forceinline__ void load_columns(const float* p, long long c, float none, float (&f)[VEC])
+{
+	if constexpr (VEC == 1) f[0] = p ? p[c] : none;
+	else
+	{
+#pragma unroll
+		for (int i = 0; i < VEC; i += 4)
+		{
+			const float4 v = p ? *reinterpret_cast<const float4*>(p + c + i) : make_float4(none, none, none, none);
+			f[i] = v.x; f[i + 1] = v.y; f[i + 2] = v.z; f[i + 3] = v.w;
+		}
+	}
+}
+template <class T, int VEC>
+__device__ __forceinline__ void store_values(T* p, const float (&f)[VEC])
+{
+	if constexpr (VEC == 1) p[0] = from_float<T>(f[0]);
+	else
+	{
+		Pack<T, VEC> a;
+#pragma unroll
+		for (int i = 0; i < VEC / 2; ++i) a.set_pair(i, pair2(f[2 * i], f[2 * i + 1]));
+		a.store(p);
+	}
+}
+template <class T, int VEC>
 __global__ void __launch_bounds__(LN_GROUP_MAX) norm_long_kernel(const LayerNormArgs p)
 {
 	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
 	Group gr(LN_GROUP_MAX, slots);
 	const float inv_n = 1.0f / (float)p.n;
+	const int from = threadIdx.x * VEC, step = LN_GROUP_MAX * VEC;
 	for (long long row = blockIdx.x; row < p.rows; row += gridDim.x)
 	{
 		const T* x = static_cast<const T*>(p.x) + row * p.ldx;
 		T* y = static_cast<T*>(p.y) + row * p.ldy;
-		float s = 0.0f;
-		for (long long c = threadIdx.x; c < p.n; c += LN_GROUP_MAX) s += to_float(x[c]);
-		const float mean = gr.sum<true>(s, 0.0f).x / (float)p.n;
-		float q = 0.0f;
-		for (long long c = threadIdx.x; c < p.n; c += LN_GROUP_MAX)
+		float s = 0.0f, f[VEC];
+#pragma unroll 4
+		for (long long c = from; c < p.n; c += step)
 		{
-			const float d = to_float(x[c]) - mean;
-			q = fmaf(d, d, q);
+			load_values<T, VEC>(x + c, f);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i) s += f[i];
 		}
-		const float rstd = 1.0f / sqrtf(gr.sum<true>(q, 0.0f).x * inv_n + p.eps);
-		for (long long c = threadIdx.x; c < p.n; c += LN_GROUP_MAX)
-			y[c] = from_float<T>(fmaf((to_float(x[c]) - mean) * rstd, p.gain ? p.gain[c] : 1.0f, p.shift ? p.shift[c] : 0.0f));
+		const float mean = gr.sum<true>(s) / (float)p.n;
+		float q = 0.0f;
+#pragma unroll 4
+		for (long long c = from; c < p.n; c += step)
+		{
+			load_values<T, VEC>(x + c, f);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i) q = fmaf(f[i] - mean, f[i] - mean, q);
+		}
+		const float rstd = 1.0f / sqrtf(gr.sum<true>(q) * inv_n + p.eps);
+#pragma unroll 4
+		for (long long c = from; c < p.n; c += step)
+		{
+			float gain[VEC], shift[VEC];
+			load_values<T, VEC>(x + c, f);
+			load_columns<VEC>(p.gain, c, 1.0f, gain);
+			load_columns<VEC>(p.shift, c, 0.0f, shift);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i) f[i] = fmaf((f[i] - mean) * rstd, gain[i], shift[i]);
+			store_values<T, VEC>(y + c, f);
+		}
 		if (threadIdx.x == 0)
 		{
 			if (p.mean) p.mean[row] = mean;
@@ -220,117 +397,46 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_long_kernel(const LayerNorm
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------
-// The same groups; both row sums in one exchange.  A lane keeps the same columns for all its rows and adds their dgain and
+// The same groups; both row sums in one exchange.  bf16 10007 x 1025: 35 us (one value at a time 164).  A lane keeps the same columns for all its rows and adds their dgain and
 // dshift up in registers; a CTA's groups are added in a fixed order and leave as one partial row, which norm_columns_kernel
-// adds up: no atomics, two runs give the same bits.
-template <class T, int VEC, bool WIDE>
-__global__ void __launch_bounds__(LN_GROUP_MAX) norm_backward_kernel(const LayerNormArgs p, int group)
+// adds up: no atomics, two runs give the same bits.  With d = x - mu, g = gain dy:  dx = r g - r sum(g) / n - d r^3 sum(g d) / n.
+// A CTA's sums of the columns: its groups' are added in a fixed order in `sums`, [groups or (in-warp groups) warps][n], and leave as
+// one partial row.  A lane's access v begins at column first + v * group * VEC.
+template <bool APART, bool WIDE, int V, int PAIRS>
+__device__ __forceinline__ void leave_columns(const LayerNormArgs& p, const Group& gr, int first, f32x2 (&dg)[V][PAIRS], f32x2 (&ds)[V][PAIRS], int edge, float2 dedge, float2* sums)
 {
-	constexpr int ELEMS = LN_ELEMS, V = ELEMS / VEC;
-	extern __shared__ float2 sums[];  // [groups or (in-warp groups) warps][n]
-	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
-	Group gr(group, slots);
-	const int groups = blockDim.x / group;
-	const long long step = (long long)gridDim.x * groups;
-	const T* X = static_cast<const T*>(p.x);
-	const T* DY = static_cast<const T*>(p.dy);
-	T* DX = static_cast<T*>(p.dx);
-	const float inv_n = 1.0f / (float)p.n;
-	float gain[ELEMS], dg[ELEMS], ds[ELEMS];
-#pragma unroll
-	for (int v = 0; v < V; ++v)
-#pragma unroll
-		for (int i = 0; i < VEC; ++i)
-		{
-			const int c = (v * group + gr.lane) * VEC + i;
-			gain[v * VEC + i] = p.gain && c < p.n ? p.gain[c] : 1.0f;
-			dg[v * VEC + i] = ds[v * VEC + i] = 0.0f;
-		}
-	Pack<T, VEC> xn[V], dn[V];
-	float mean_n = 0.0f, rstd_n = 0.0f;
-	auto fetch = [&](long long row) {
-		if (row >= p.rows) return;
-		mean_n = p.mean[row];
-		rstd_n = p.rstd[row];
-#pragma unroll
-		for (int v = 0; v < V; ++v)
-		{
-			const int c = (v * group + gr.lane) * VEC;
-			if (c < p.n)
-			{
-				xn[v].load(X + row * p.ldx + c);
-				dn[v].load(DY + row * p.lddy + c);
-			}
-		}
-	};
-	long long row = (long long)blockIdx.x * groups + gr.index;
-	fetch(row);
-	const long long walk = WIDE ? row : (long long)blockIdx.x * groups + ((int)threadIdx.x & ~31) / group;
-	for (long long first = walk; first < p.rows; first += step, row += step)
-	{
-		float xh[ELEMS], dy[ELEMS];
-		const float mean = mean_n, rstd = rstd_n;
-		float a = 0.0f, b = 0.0f;
-#pragma unroll
-		for (int v = 0; v < V; ++v)
-#pragma unroll
-			for (int i = 0; i < VEC; ++i)
-			{
-				const int e = v * VEC + i;
-				const bool in = row < p.rows && (v * group + gr.lane) * VEC < p.n;
-				xh[e] = in ? (xn[v].get(i) - mean) * rstd : 0.0f;
-				dy[e] = in ? dn[v].get(i) : 0.0f;
-				const float g = dy[e] * gain[e];
-				a += g;
-				b = fmaf(g, xh[e], b);
-				dg[e] = fmaf(dy[e], xh[e], dg[e]);
-				ds[e] += dy[e];
-			}
-		fetch(row + step);
-		const float2 s = gr.sum<WIDE>(a, b);
-		const float ma = s.x * inv_n, mb = s.y * inv_n;
-		if (!DX || row >= p.rows) continue;
-#pragma unroll
-		for (int v = 0; v < V; ++v)
-		{
-			const int c = (v * group + gr.lane) * VEC;
-			if (c >= p.n) continue;
-			Pack<T, VEC> o;
-#pragma unroll
-			for (int i = 0; i < VEC; ++i)
-			{
-				const int e = v * VEC + i;
-				o.set(i, rstd * (fmaf(dy[e], gain[e], -ma) - xh[e] * mb));
-			}
-			o.store(DX + row * p.lddx + c);
-		}
-	}
-	if (!p.part) return;
+	const int group = gr.size, second = APART ? group : 1;
 	if (!WIDE)
 	{
 		// the warp's groups hold the same columns on lanes that are a group apart
 #pragma unroll
-		for (int e = 0; e < ELEMS; ++e)
-			for (int o = group; o < 32; o <<= 1)
-			{
-				dg[e] += __shfl_xor_sync(0xFFFFFFFFu, dg[e], o);
-				ds[e] += __shfl_xor_sync(0xFFFFFFFFu, ds[e], o);
-			}
+		for (int v = 0; v < V; ++v)
+#pragma unroll
+			for (int i = 0; i < PAIRS; ++i)
+				for (int o = group; o < 32; o <<= 1)
+				{
+					dg[v][i] = add2(dg[v][i], __shfl_xor_sync(0xFFFFFFFFu, dg[v][i], o));
+					ds[v][i] = add2(ds[v][i], __shfl_xor_sync(0xFFFFFFFFu, ds[v][i], o));
+				}
 	}
-	const int parts = WIDE ? groups : (int)blockDim.x / 32;
+	const int parts = WIDE ? (int)blockDim.x / group : (int)blockDim.x / 32;
 	const int part = WIDE ? gr.index : (int)threadIdx.x / 32;
+	float2* out = parts == 1 ? p.part + (long long)blockIdx.x * p.n : sums + (long long)part * p.n;
 	if (WIDE || (int)(threadIdx.x & 31) < group)
 	{
 #pragma unroll
 		for (int v = 0; v < V; ++v)
 #pragma unroll
-			for (int i = 0; i < VEC; ++i)
+			for (int i = 0; i < PAIRS; ++i)
 			{
-				const int c = (v * group + gr.lane) * VEC + i;
-				if (c >= p.n) continue;
-				if (parts == 1) p.part[(long long)blockIdx.x * p.n + c] = make_float2(dg[v * VEC + i], ds[v * VEC + i]);
-				else sums[(long long)part * p.n + c] = make_float2(dg[v * VEC + i], ds[v * VEC + i]);
+				const int e = first + v * group * 2 * PAIRS + 2 * i, f = e + second;
+				float g0, g1, s0, s1;
+				unpair2(dg[v][i], g0, g1);
+				unpair2(ds[v][i], s0, s1);
+				if ((APART ? e : f) < p.n) out[e] = make_float2(g0, s0);
+				if (f < p.n) out[f] = make_float2(g1, s1);
 			}
+		if (edge >= 0) out[edge] = dedge;
 	}
 	if (parts == 1) return;
 	__syncthreads();
@@ -346,62 +452,307 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_backward_kernel(const Layer
 	}
 }
 
+template <class T, int MODE, bool WIDE>
+__global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const LayerNormArgs p, int group)
+{
+	constexpr int VEC = access_elems<T>(MODE), V = LN_ELEMS / VEC, PAIRS = VEC / 2;
+	extern __shared__ float2 sums[];  // [groups or (in-warp groups) warps][n]
+	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
+	Group gr(group, slots);
+	const int groups = blockDim.x / group;
+	const long long step = (long long)gridDim.x * groups;
+	typedef RowPlace<T, MODE> Place;
+	const float inv_n = 1.0f / (float)p.n;
+	const f32x2 zero = pair2(0.0f, 0.0f);
+	cudaTriggerProgrammaticLaunchCompletion();
+	f32x2 gain[V][PAIRS], dg[V][PAIRS], ds[V][PAIRS];
+	long long row = (long long)blockIdx.x * groups + gr.index;
+	const Place column(p.x, p.ldx, row + 1, p.n, row, gr);  // (of a group without rows too: it leaves zeros)
+#pragma unroll
+	for (int v = 0; v < V; ++v)
+#pragma unroll
+		for (int i = 0; i < PAIRS; ++i)
+		{
+			gain[v][i] = column.columns(p.gain, column.first + v * group * VEC + 2 * i, 1.0f);
+			dg[v][i] = ds[v][i] = zero;
+		}
+	constexpr bool EDGE = MODE == BY_WORDS;
+	const float gain_e = EDGE && p.gain && column.edge >= 0 ? p.gain[column.edge] : 1.0f;
+	float dg_e = 0.0f, ds_e = 0.0f;
+	T xe_n = from_float<T>(0.0f), de_n = xe_n;
+	Pack<T, VEC> xn[V], dn[V];
+	float mean_n = 0.0f, rstd_n = 0.0f;
+	auto fetch = [&](long long row) {
+		const Place at(p.x, p.ldx, p.rows, p.n, row, gr);
+		if (row < p.rows)
+		{
+			mean_n = p.mean[row];
+			rstd_n = p.rstd[row];
+		}
+		const T *x = static_cast<const T*>(p.x) + row * p.ldx, *dy = static_cast<const T*>(p.dy) + row * p.lddy;
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+		{
+			at.load(x, v * group * VEC, xn[v]);
+			at.load(dy, v * group * VEC, dn[v]);
+		}
+		if (EDGE)
+		{
+			xe_n = at.load_edge(x);
+			de_n = at.load_edge(dy);
+		}
+	};
+	fetch(row);
+	const long long walk = WIDE ? row : (long long)blockIdx.x * groups + ((int)threadIdx.x & ~31) / group;
+	for (long long first = walk; first < p.rows; first += step, row += step)
+	{
+		const Place at(p.x, p.ldx, p.rows, p.n, row, gr);
+		const f32x2 minus = pair2(-mean_n, -mean_n), scale = pair2(rstd_n, rstd_n);
+		const float rstd = rstd_n;
+		f32x2 d[V][PAIRS], g[V][PAIRS];
+		f32x2 a2 = zero, b2 = zero;
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+#pragma unroll
+			for (int i = 0; i < PAIRS; ++i)
+			{
+				// (what is not the row's has a dy of zero, and a difference that means nothing)
+				const f32x2 dy = dn[v].pair(i);
+				d[v][i] = at.mask(add2(xn[v].pair(i), minus), v * group * VEC);
+				g[v][i] = mul2(dy, gain[v][i]);
+				a2 = add2(a2, g[v][i]);
+				b2 = fma2(g[v][i], d[v][i], b2);
+				dg[v][i] = fma2(mul2(dy, scale), d[v][i], dg[v][i]);
+				ds[v][i] = add2(ds[v][i], dy);
+			}
+		float a, b, c, e, de = 0.0f, ge = 0.0f;
+		unpair2(a2, a, c);
+		unpair2(b2, b, e);
+		if (EDGE && at.edge >= 0)
+		{
+			const float dy = to_float(de_n);
+			de = to_float(xe_n) - mean_n;
+			ge = dy * gain_e;
+			a += ge;
+			b = fmaf(ge, de, b);
+			dg_e = fmaf(dy * rstd, de, dg_e);
+			ds_e += dy;
+		}
+		fetch(row + step);
+		if (!p.dx) continue;
+		const float2 s = gr.sum<WIDE>(a + c, b + e);
+		if (at.n == 0) continue;
+		const float ma = -s.x * inv_n * rstd, mb = -s.y * inv_n * rstd * rstd * rstd;
+		const f32x2 ma2 = pair2(ma, ma), mb2 = pair2(mb, mb);
+		T* dx = static_cast<T*>(p.dx) + row * p.lddx;
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+		{
+			f32x2 o[PAIRS];
+#pragma unroll
+			for (int i = 0; i < PAIRS; ++i) o[i] = fma2(g[v][i], scale, fma2(d[v][i], mb2, ma2));
+			at.store(dx, v * group * VEC, o);
+		}
+		if (EDGE && at.edge >= 0) dx[at.edge] = from_float<T>(fmaf(ge, rstd, fmaf(de, mb, ma)));
+	}
+	if (p.part) leave_columns<MODE == BY_VALUES, WIDE>(p, gr, column.first, dg, ds, column.edge, make_float2(dg_e, ds_e), sums);
+}
+
+// Rows that 16-byte accesses can read: they are copied to shared memory several rows ahead, each lane its own accesses, and read
+// there twice, so that a lane's registers hold only what outlives a row.  One CTA of 512 threads per SM: 768, with 80 registers each, spill.
+//   fp32 8192 x 4096: 72 us, 5.6 TB/s (one row ahead in registers 110);  bf16: 50 us, each further 8192 rows 31: as the copy of as
+//   many bytes.  What is above that is the start, the CTAs' sums and the columns' kernel.
+template <class T> __host__ __device__ constexpr int quads_stages() { return 208 * 1024 / (LN_GROUP_MAX * 2 * LN_ELEMS * (int)sizeof(T)); }
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(const LayerNormArgs p, int group)
+{
+	constexpr int VEC = access_elems<T>(BY_QUADS), V = LN_ELEMS / VEC, PAIRS = VEC / 2, STAGES = quads_stages<T>();
+	extern __shared__ uint4 ahead[];  // [STAGES][x, dy][V][threads]; at the end the columns' sums
+	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
+	Group gr(group, slots);
+	const int groups = blockDim.x / group;
+	const long long step = (long long)gridDim.x * groups;
+	const float inv_n = 1.0f / (float)p.n;
+	const f32x2 zero = pair2(0.0f, 0.0f);
+	cudaTriggerProgrammaticLaunchCompletion();
+	const int first_c = gr.lane * VEC, hop = group * VEC;
+	uint4* const mine = ahead + threadIdx.x;
+	f32x2 gain[V][PAIRS], dg[V][PAIRS], ds[V][PAIRS];
+#pragma unroll
+	for (int v = 0; v < V; ++v)
+#pragma unroll
+		for (int i = 0; i < PAIRS; ++i)
+		{
+			const int e = first_c + v * hop + 2 * i;
+			gain[v][i] = p.gain && e < p.n ? pair2(p.gain[e], p.gain[e + 1]) : pair2(1.0f, 1.0f);
+			dg[v][i] = ds[v][i] = zero;
+		}
+	float mean_n = 0.0f, rstd_n = 0.0f;
+	auto fetch = [&](long long row, int stage) {
+		const bool is = row < p.rows;
+		const T *x = static_cast<const T*>(p.x) + (is ? row * p.ldx : 0), *dy = static_cast<const T*>(p.dy) + (is ? row * p.lddy : 0);
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+		{
+			const int c = first_c + v * hop;
+			const bool in = is && c < p.n;
+			copy_ahead(mine + (2 * stage * V + v) * (int)blockDim.x, x + (in ? c : 0), in);
+			copy_ahead(mine + ((2 * stage + 1) * V + v) * (int)blockDim.x, dy + (in ? c : 0), in);
+		}
+		asm volatile("cp.async.commit_group;" ::: "memory");
+	};
+	auto fetch_statistics = [&](long long row) {
+		if (row >= p.rows) return;
+		mean_n = p.mean[row];
+		rstd_n = p.rstd[row];
+	};
+	long long row = (long long)blockIdx.x * groups + gr.index;
+	for (int i = 0; i < STAGES; ++i) fetch(row + i * step, i);
+	fetch_statistics(row);
+	int stage = 0;
+	const long long walk = WIDE ? row : (long long)blockIdx.x * groups + ((int)threadIdx.x & ~31) / group;
+	for (long long first = walk; first < p.rows; first += step, row += step)
+	{
+		const f32x2 minus = pair2(-mean_n, -mean_n), scale = pair2(rstd_n, rstd_n);
+		const float rstd = rstd_n;
+		f32x2 a2 = zero, b2 = zero;
+		asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+		fetch_statistics(row + step);
+		const uint4 *xs = mine + 2 * stage * V * (int)blockDim.x, *dys = xs + V * (int)blockDim.x;
+#pragma unroll
+		for (int v = 0; v < V; ++v)
+		{
+			Pack<T, VEC> xv, dv;  // (what is not the row's has a dy of zero, and a difference that means nothing)
+			xv.set(xs[v * (int)blockDim.x]);
+			dv.set(dys[v * (int)blockDim.x]);
+#pragma unroll
+			for (int i = 0; i < PAIRS; ++i)
+			{
+				const f32x2 dy = dv.pair(i), d = add2(xv.pair(i), minus), g = mul2(dy, gain[v][i]);
+				a2 = add2(a2, g);
+				b2 = fma2(g, d, b2);
+				dg[v][i] = fma2(mul2(dy, scale), d, dg[v][i]);
+				ds[v][i] = add2(ds[v][i], dy);
+			}
+		}
+		if (p.dx)
+		{
+			float a, b, c, e;
+			unpair2(a2, a, c);
+			unpair2(b2, b, e);
+			const float2 s = gr.sum<WIDE>(a + c, b + e);
+			const float ma = -s.x * inv_n * rstd, mb = -s.y * inv_n * rstd * rstd * rstd;
+			const f32x2 ma2 = pair2(ma, ma), mb2 = pair2(mb, mb);
+			T* dx = static_cast<T*>(p.dx) + row * p.lddx + first_c;
+			if (row < p.rows)
+			{
+#pragma unroll
+				for (int v = 0; v < V; ++v)
+				{
+					Pack<T, VEC> xv, dv, o;
+					xv.set(xs[v * (int)blockDim.x]);
+					dv.set(dys[v * (int)blockDim.x]);
+#pragma unroll
+					for (int i = 0; i < PAIRS; ++i)
+						o.set_pair(i, fma2(mul2(dv.pair(i), gain[v][i]), scale, fma2(add2(xv.pair(i), minus), mb2, ma2)));
+					if (first_c + v * hop < p.n) o.store(dx + v * hop);
+				}
+			}
+		}
+		fetch(row + STAGES * step, stage);
+		stage = stage + 1 == STAGES ? 0 : stage + 1;
+	}
+	asm volatile("cp.async.wait_all;" ::: "memory");
+	__syncthreads();
+	if (p.part) leave_columns<false, WIDE>(p, gr, first_c, dg, ds, -1, make_float2(0.0f, 0.0f), reinterpret_cast<float2*>(ahead));
+}
+
 // Long rows: dx by a CTA per row in two passes ...
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(LN_GROUP_MAX) norm_backward_long_kernel(const LayerNormArgs p)
 {
 	__shared__ float2 slots[2 * LN_GROUP_MAX / 32];
 	Group gr(LN_GROUP_MAX, slots);
 	const float inv_n = 1.0f / (float)p.n;
+	const int from = threadIdx.x * VEC, step = LN_GROUP_MAX * VEC;
 	for (long long row = blockIdx.x; row < p.rows; row += gridDim.x)
 	{
 		const T* x = static_cast<const T*>(p.x) + row * p.ldx;
 		const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
 		T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 		const float mean = p.mean[row], rstd = p.rstd[row];
-		float a = 0.0f, b = 0.0f;
-		for (long long c = threadIdx.x; c < p.n; c += LN_GROUP_MAX)
+		float a = 0.0f, b = 0.0f, f[VEC], d[VEC], gain[VEC];
+#pragma unroll 2
+		for (long long c = from; c < p.n; c += step)
 		{
-			const float g = to_float(dy[c]) * (p.gain ? p.gain[c] : 1.0f);
-			a += g;
-			b = fmaf(g, (to_float(x[c]) - mean) * rstd, b);
+			load_values<T, VEC>(x + c, f);
+			load_values<T, VEC>(dy + c, d);
+			load_columns<VEC>(p.gain, c, 1.0f, gain);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i)
+			{
+				const float g = d[i] * gain[i];
+				a += g;
+				b = fmaf(g, (f[i] - mean) * rstd, b);
+			}
 		}
 		const float2 s = gr.sum<true>(a, b);
 		const float ma = s.x * inv_n, mb = s.y * inv_n;
-		for (long long c = threadIdx.x; c < p.n; c += LN_GROUP_MAX)
-			dx[c] = from_float<T>(rstd * (fmaf(to_float(dy[c]), p.gain ? p.gain[c] : 1.0f, -ma) - (to_float(x[c]) - mean) * rstd * mb));
+#pragma unroll 2
+		for (long long c = from; c < p.n; c += step)
+		{
+			load_values<T, VEC>(x + c, f);
+			load_values<T, VEC>(dy + c, d);
+			load_columns<VEC>(p.gain, c, 1.0f, gain);
+#pragma unroll
+			for (int i = 0; i < VEC; ++i) f[i] = rstd * (fmaf(d[i], gain[i], -ma) - (f[i] - mean) * rstd * mb);
+			store_values<T, VEC>(dx + c, f);
+		}
 	}
 }
 // ... and the columns' sums over a slice of the rows
-template <class T>
+template <class T, int VEC>
 __global__ void __launch_bounds__(LN_THREADS) norm_slices_kernel(const LayerNormArgs p, int slices)
 {
-	const long long c = (long long)blockIdx.x * LN_THREADS + threadIdx.x;
+	const long long c = ((long long)blockIdx.x * LN_THREADS + threadIdx.x) * VEC;
 	if (c >= p.n) return;
-	const T* x = static_cast<const T*>(p.x);
-	const T* dy = static_cast<const T*>(p.dy);
-	float2 t = make_float2(0.0f, 0.0f);
+	const T* x = static_cast<const T*>(p.x) + c;
+	const T* dy = static_cast<const T*>(p.dy) + c;
+	float2 t[VEC];
+#pragma unroll
+	for (int i = 0; i < VEC; ++i) t[i] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
 	for (long long row = blockIdx.y; row < p.rows; row += slices)
 	{
-		const float d = to_float(dy[row * p.lddy + c]);
-		t.x = fmaf(d, (to_float(x[row * p.ldx + c]) - p.mean[row]) * p.rstd[row], t.x);
-		t.y += d;
+		float f[VEC], d[VEC];
+		load_values<T, VEC>(x + row * p.ldx, f);
+		load_values<T, VEC>(dy + row * p.lddy, d);
+		const float mean = p.mean[row], rstd = p.rstd[row];
+#pragma unroll
+		for (int i = 0; i < VEC; ++i)
+		{
+			t[i].x = fmaf(d[i], (f[i] - mean) * rstd, t[i].x);
+			t[i].y += d[i];
+		}
 	}
-	p.part[(long long)blockIdx.y * p.n + c] = t;
+#pragma unroll
+	for (int i = 0; i < VEC; ++i)
+		if (VEC == 1) p.part[(long long)blockIdx.y * p.n + c] = t[i];
+		else if (i % 2 == 0) reinterpret_cast<float4*>(p.part + (long long)blockIdx.y * p.n + c)[i / 2] = make_float4(t[i].x, t[i].y, t[i + 1 < VEC ? i + 1 : i].x, t[i + 1 < VEC ? i + 1 : i].y);
 }
 
-// dgain | dshift from `parts` partial rows: 32 columns per CTA, eight slices of the partials, added in a fixed order
-__global__ void __launch_bounds__(LN_THREADS) norm_columns_kernel(const float2* part, int parts, int n, float* dgain, float* dshift)
+// dgain | dshift from `parts` partial rows: 32 columns per CTA, LN_SLICES slices of the partials, added in a fixed order
+__global__ void __launch_bounds__(32 * LN_SLICES) norm_columns_kernel(const float2* part, int parts, int n, float* dgain, float* dshift)
 {
-	__shared__ float2 sums[8][33];
+	__shared__ float2 sums[LN_SLICES][33];
 	const int k = threadIdx.x & 31, slice = threadIdx.x >> 5;
 	const long long c = (long long)blockIdx.x * 32 + k;
 	cudaGridDependencySynchronize();
 	float2 t = make_float2(0.0f, 0.0f);
 	if (c < n)
 	{
-#pragma unroll 4
-		for (int r = slice; r < parts; r += 8)
+#pragma unroll 5
+		for (int r = slice; r < parts; r += LN_SLICES)
 		{
 			const float2 v = part[(long long)r * n + c];
 			t.x += v.x;
@@ -412,7 +763,7 @@ __global__ void __launch_bounds__(LN_THREADS) norm_columns_kernel(const float2* 
 	__syncthreads();
 	if (slice != 0 || c >= n) return;
 #pragma unroll
-	for (int s = 1; s < 8; ++s)
+	for (int s = 1; s < LN_SLICES; ++s)
 	{
 		t.x += sums[s][k].x;
 		t.y += sums[s][k].y;
@@ -448,65 +799,103 @@ int group_lanes(int n, int elems)
 }
 int group_threads(int group) { return group <= LN_THREADS ? group * (LN_THREADS / group) : group; }
 
-// The widest access that every row of every tensor allows: 16 bytes, 4 bytes (16-bit types), one value.
+// Do all rows of all tensors consist of whole pieces of so many bytes?
 bool aligned(const LayerNormArgs& a, int size, int bytes)
 {
 	auto ok = [&](const void* p, long long ld) { return !p || ((uintptr_t)p % bytes == 0 && (ld * size) % bytes == 0); };
 	return ((long long)a.n * size) % bytes == 0 && ok(a.x, a.ldx) && ok(a.y, a.ldy) && ok(a.dy, a.lddy) && ok(a.dx, a.lddx);
 }
 
-// CTAs of the backward kernel, each of which leaves one partial row
-int backward_ctas(long long rows, int n)
+// and the same of the vectors of columns, which long rows read 16 bytes at a time
+bool columns_aligned(const LayerNormArgs& a) { return (((uintptr_t)a.gain | (uintptr_t)a.shift) & 15) == 0; }
+
+// Threads and CTAs of the backward kernel, each CTA of which leaves one partial row: one CTA per SM, with two or more groups where
+// a row is short enough; but smaller ones where there would be fewer than SMs (1024 x 256 in fp32 runs on 128 SMs, not on 32).
+void backward_shape(long long rows, int group, int* threads, int* ctas)
 {
-	const int group = group_lanes(n, LN_ELEMS);
-	const int groups = group_threads(group) / group;
-	const long long want = (rows + groups - 1) / groups;
-	const long long most = LN_SMS * 2;
-	return (int)(want < most ? want : most);
+	int t = LN_GROUP_MAX;
+	while (t > 64 && t / 2 >= group && (rows + t / group - 1) / (t / group) < LN_SMS) t /= 2;
+	*threads = group <= t ? group * (t / group) : group;
+	const int groups = *threads / group;
+	*ctas = (int)std::min<long long>(LN_SMS, (rows + groups - 1) / groups);
 }
 bool backward_long(int n) { return n > LN_GROUP_MAX * LN_ELEMS; }
+// Lanes of a row of whole words and their edges, which take two.
+int mode_lanes(int n, int elems, int mode) { return mode == BY_WORDS ? std::max(2, group_lanes(n / 2 * 2, elems)) : group_lanes(n, elems); }
 int backward_slices(long long rows) { return (int)(rows < 32 ? rows : 32); }
 
-template <class T, int VEC>
-cudaError_t forward_vec(const LayerNormArgs& a, cudaStream_t s)
+template <class T, int MODE, int ELEMS>
+cudaError_t forward_elems(const LayerNormArgs& a, cudaStream_t s)
 {
-	const bool lengthy = a.n > LN_GROUP_MAX * LN_ELEMS;
-	const int group = group_lanes(a.n, lengthy ? LN_ELEMS_LONG : LN_ELEMS);
+	const int group = mode_lanes(a.n, ELEMS, MODE);
 	const int threads = group_threads(group);
-	const long long want = (a.rows + threads / group - 1) / (threads / group);
-	const long long most = (long long)LN_SMS * (2048 / threads);
+	const int groups = threads / group;
+	const long long want = (a.rows + groups - 1) / groups;
+	// (LN_SMS is even: a group that walks sees rows of one kind only, where every other row begins in the middle of a word)
+	const long long most = (long long)LN_SMS * std::max(1, (ELEMS == 16 ? 768 : 512) / threads);
 	const unsigned grid = (unsigned)(want < most ? want : most);
-	if (lengthy) norm_kernel<T, VEC, LN_ELEMS_LONG, true><<<grid, threads, 0, s>>>(a, group);
-	else if (group > 32) norm_kernel<T, VEC, LN_ELEMS, true><<<grid, threads, 0, s>>>(a, group);
-	else norm_kernel<T, VEC, LN_ELEMS, false><<<grid, threads, 0, s>>>(a, group);
+	if (group > 32) norm_kernel<T, MODE, ELEMS, true><<<grid, threads, 0, s>>>(a, group);
+	else norm_kernel<T, MODE, ELEMS, false><<<grid, threads, 0, s>>>(a, group);
 	return cudaGetLastError();
 }
 
-template <class T, int VEC>
-cudaError_t backward_vec(const LayerNormArgs& a, cudaStream_t s)
+template <class T, int MODE>
+cudaError_t forward_mode(const LayerNormArgs& a, cudaStream_t s)
 {
-	const int group = group_lanes(a.n, LN_ELEMS);
-	const int threads = group_threads(group);
-	const int parts = group > 32 ? threads / group : threads / 32;
-	const size_t smem = parts > 1 ? (size_t)parts * a.n * sizeof(float2) : 0;
-	const int grid = backward_ctas(a.rows, a.n);
-	if (group > 32) norm_backward_kernel<T, VEC, true><<<grid, threads, smem, s>>>(a, group);
-	else norm_backward_kernel<T, VEC, false><<<grid, threads, smem, s>>>(a, group);
-	return cudaGetLastError();
+	if (a.n <= LN_THREADS * 16) return forward_elems<T, MODE, 16>(a, s);
+	return a.n <= LN_THREADS * 32 ? forward_elems<T, MODE, 32>(a, s) : forward_elems<T, MODE, 64>(a, s);
 }
+
+template <class T, int MODE>
+cudaError_t backward_mode(const LayerNormArgs& a, int* ctas, cudaStream_t s)
+{
+	const int group = mode_lanes(a.n, LN_ELEMS, MODE);
+	int threads, grid;
+	backward_shape(a.rows, group, &threads, &grid);
+	*ctas = grid;
+	const int parts = group > 32 ? threads / group : threads / 32;
+	size_t smem = parts > 1 ? (size_t)parts * a.n * sizeof(float2) : 0;
+	auto go = [&](void (*kernel)(LayerNormArgs, int)) {
+		if (smem > 47 * 1024)  // (48 KB without being asked for, the sums' slots among them)
+			if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+		kernel<<<grid, threads, smem, s>>>(a, group);
+		return cudaGetLastError();
+	};
+	if constexpr (MODE == BY_QUADS)
+	{
+		smem = std::max(smem, (size_t)threads * 2 * LN_ELEMS * sizeof(T) * quads_stages<T>());
+		return group > 32 ? go(norm_backward_quads_kernel<T, true>) : go(norm_backward_quads_kernel<T, false>);
+	}
+	else if constexpr (MODE == BY_WORDS) return go(norm_backward_kernel<T, MODE, true>);
+	else return group > 32 ? go(norm_backward_kernel<T, MODE, true>) : go(norm_backward_kernel<T, MODE, false>);
+}
+
+// Two tensors whose rows begin on the same half of a word.
+bool alike(const void* x, long long ldx, const void* y, long long ldy) { return (((uintptr_t)x ^ (uintptr_t)y) & 2) == 0 && ((ldx ^ ldy) & 1) == 0; }
 
 template <class T>
 cudaError_t forward_type(const LayerNormArgs& a, cudaStream_t s)
 {
-	if (a.n > LN_GROUP_MAX * LN_ELEMS_LONG)
+	if (a.n > LN_THREADS * 64)
 	{
-		const long long most = LN_SMS * 4;
-		norm_long_kernel<T><<<(unsigned)(a.rows < most ? a.rows : most), LN_GROUP_MAX, 0, s>>>(a);
+		const unsigned grid = (unsigned)std::min<long long>(a.rows, LN_SMS * 4);
+		if (aligned(a, sizeof(T), 16) && columns_aligned(a)) norm_long_kernel<T, 16 / sizeof(T)><<<grid, LN_GROUP_MAX, 0, s>>>(a);
+		else norm_long_kernel<T, 1><<<grid, LN_GROUP_MAX, 0, s>>>(a);
 		return cudaGetLastError();
 	}
-	if (aligned(a, sizeof(T), 16)) return forward_vec<T, 16 / sizeof(T)>(a, s);
-	if (sizeof(T) == 2 && aligned(a, sizeof(T), 4)) return forward_vec<T, 4 / sizeof(T)>(a, s);
-	return forward_vec<T, 1>(a, s);
+	if (aligned(a, sizeof(T), 16)) return forward_mode<T, BY_QUADS>(a, s);
+	if constexpr (sizeof(T) == 2)
+		if (alike(a.x, a.ldx, a.y, a.ldy)) return forward_mode<T, BY_WORDS>(a, s);
+	return forward_mode<T, BY_VALUES>(a, s);
+}
+
+template <class T, int VEC>
+cudaError_t backward_long_rows(const LayerNormArgs& a, int parts, cudaStream_t s)
+{
+	if (a.part) norm_slices_kernel<T, VEC><<<dim3((unsigned)((a.n + LN_THREADS * VEC - 1) / (LN_THREADS * VEC)), (unsigned)parts), LN_THREADS, 0, s>>>(a, parts);
+	if (cudaError_t e = cudaGetLastError()) return e;
+	if (a.dx) norm_backward_long_kernel<T, VEC><<<(unsigned)std::min<long long>(a.rows, LN_SMS * 4), LN_GROUP_MAX, 0, s>>>(a);
+	return cudaGetLastError();
 }
 
 template <class T>
@@ -516,33 +905,24 @@ cudaError_t backward_type(const LayerNormArgs& a, cudaStream_t s)
 	if (backward_long(a.n))
 	{
 		parts = backward_slices(a.rows);
-		if (a.part)
-		{
-			norm_slices_kernel<T><<<dim3((unsigned)((a.n + LN_THREADS - 1) / LN_THREADS), (unsigned)parts), LN_THREADS, 0, s>>>(a, parts);
-			cudaError_t e = cudaGetLastError();
-			if (e != cudaSuccess) return e;
-		}
-		if (a.dx)
-		{
-			const long long most = LN_SMS * 4;
-			norm_backward_long_kernel<T><<<(unsigned)(a.rows < most ? a.rows : most), LN_GROUP_MAX, 0, s>>>(a);
-			cudaError_t e = cudaGetLastError();
-			if (e != cudaSuccess) return e;
-		}
+		const cudaError_t e = aligned(a, sizeof(T), 16) && columns_aligned(a) ? backward_long_rows<T, 16 / sizeof(T)>(a, parts, s) : backward_long_rows<T, 1>(a, parts, s);
+		if (e != cudaSuccess) return e;
 	}
 	else
 	{
-		parts = backward_ctas(a.rows, a.n);
-		cudaError_t e;
-		if (aligned(a, sizeof(T), 16)) e = backward_vec<T, 16 / sizeof(T)>(a, s);
-		else if (sizeof(T) == 2 && aligned(a, sizeof(T), 4)) e = backward_vec<T, 4 / sizeof(T)>(a, s);
-		else e = backward_vec<T, 1>(a, s);
+		cudaError_t e = cudaErrorInvalidValue;
+		// by words: in a warp of several groups the columns' sums would lie on different lanes
+		const bool words = sizeof(T) == 2 && mode_lanes(a.n, LN_ELEMS, BY_WORDS) > 32 && alike(a.x, a.ldx, a.dy, a.lddy) &&
+		                   (!a.dx || alike(a.x, a.ldx, a.dx, a.lddx));
+		if (aligned(a, sizeof(T), 16)) e = backward_mode<T, BY_QUADS>(a, &parts, s);
+		else if (!words) e = backward_mode<T, BY_VALUES>(a, &parts, s);
+		else if constexpr (sizeof(T) == 2) e = backward_mode<T, BY_WORDS>(a, &parts, s);
 		if (e != cudaSuccess) return e;
 	}
 	if (!a.part) return cudaSuccess;
 	cudaLaunchConfig_t cfg = {};
 	cfg.gridDim = dim3((unsigned)((a.n + 31) / 32));
-	cfg.blockDim = dim3(LN_THREADS);
+	cfg.blockDim = dim3(32 * LN_SLICES);
 	cfg.stream = s;
 	cudaLaunchAttribute at[1];
 	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -557,7 +937,8 @@ cudaError_t backward_type(const LayerNormArgs& a, cudaStream_t s)
 size_t layer_norm_partial_rows(long long rows, int n)
 {
 	if (rows < 1) return 0;
-	return (size_t)(backward_long(n) ? backward_slices(rows) : backward_ctas(rows, n));
+	if (backward_long(n)) return (size_t)backward_slices(rows);
+	return (size_t)std::min<long long>(rows, LN_SMS);
 }
 
 cudaError_t launch_layer_norm(const LayerNormArgs& a, int type, cudaStream_t s)

@@ -151,7 +151,7 @@ extern "C" int gl_layer_norm(const void* d_x, int64_t ldx, const float* d_gain, 
 extern "C" int64_t gl_layer_norm_backward_workspace(int64_t rows, int32_t n)
 {
 	if (rows < 0 || n < 1 || n > MAX_DIM) return report_error(GL_ERR_INVALID, "gl_layer_norm_backward_workspace: bad size");
-	return (int64_t)(layer_norm_partial_rows(rows, n) * (size_t)n * sizeof(float2) + 8);
+	return (int64_t)(layer_norm_partial_rows(rows, n) * (size_t)n * sizeof(float2) + 15);
 }
 
 extern "C" int gl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int64_t ldx, const float* d_gain, const float* d_mean,
@@ -193,7 +193,7 @@ extern "C" int gl_layer_norm_backward(const void* d_dy, int64_t lddy, const void
 	a.gain = d_gain;
 	a.mean = const_cast<float*>(d_mean);
 	a.rstd = const_cast<float*>(d_rstd);
-	a.part = sums ? reinterpret_cast<float2*>(((uintptr_t)d_work + 7) / 8 * 8) : nullptr;
+	a.part = sums ? reinterpret_cast<float2*>(((uintptr_t)d_work + 15) / 16 * 16) : nullptr;
 	a.dgain = d_dgain; a.dshift = d_dshift;
 	a.rows = rows; a.n = n;
 	return finish(name, launch_layer_norm_backward(a, type, s));

@@ -135,12 +135,21 @@ def test_layer_norm_many_rows(g, n):
     check_norm(g, 30011, n, "bf16", n, n, 0, "relu", plain=True)
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,n,pad", [(700, 4096, 0), (593, 4096, 8), (5001, 1025, 0), (6007, 500, 0), (20011, 257, 0), (601, 9001, 0),
+                                        (1203, 2050, 0), (4099, 1000, 0), (30001, 264, 0), (9000, 255, 0)])
+def test_layer_norm_walks(g, t, rows, n, pad):
+    """More rows than lanes hold at a time: rows of whole 16-byte pieces, rows that begin anywhere, a last turn that is cut."""
+    check_norm(g, rows, n, t, n + pad, n + 2 * pad, 0, "relu", seed=rows)
+    check_norm(g, rows, n, t, n + pad, n + pad, 0, "offset", seed=n, plain=True)
+
+
 def test_layer_norm_in_place_and_without_statistics(g):
-    for n, t in ((300, "f32"), (4096, "bf16"), (20000, "f16")):
-        _, x, gain, shift, _ = norm_inputs(50, n, t, n, 0, 3, "plain")
+    for n, t, rows in ((300, "f32", 50), (4096, "bf16", 50), (20000, "f16", 50), (4096, "f32", 700), (1025, "bf16", 5000)):
+        _, x, gain, shift, _ = norm_inputs(rows, n, t, n, 0, 3, "plain")
         y = torch.empty_like(x)
         run_norm(g, x, gain, shift, y, t)
-        g.layer_norm(x.data_ptr(), n, gain.data_ptr(), shift.data_ptr(), x.data_ptr(), n, None, None, 50, n, dtype=code(g, t),
+        g.layer_norm(x.data_ptr(), n, gain.data_ptr(), shift.data_ptr(), x.data_ptr(), n, None, None, rows, n, dtype=code(g, t),
                      stream=stream())
         assert torch.equal(x, y)
 
