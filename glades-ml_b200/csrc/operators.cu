@@ -2,7 +2,10 @@
 // their work is queued on the caller's stream.  Nothing is allocated, nothing waits, no state is kept between calls.
 #include <math.h>
 
+#include <algorithm>
+#include <atomic>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "internal.h"
@@ -32,7 +35,7 @@ struct OnDevice
 // GL_OK for an sm_100 device; its attributes are asked for once
 int check_device(int device)
 {
-	static int known[64];  // 1: sm_100, written with the same value by whoever comes first
+	static std::atomic<int> known[64];  // 1: sm_100
 	if (device < 0 || device >= 64) return report_error(GL_ERR_INVALID, "device %d: no such device", device);
 	if (known[device] == 1) return GL_OK;
 	int n = 0, major = 0;
@@ -84,6 +87,27 @@ int check_steps(const char* name, OrthoArgs& a, const float* coefficients, int s
 }
 
 bool shape_ok(int rows, int cols) { return rows >= 1 && cols >= 1 && rows <= MAX_DIM && cols <= MAX_DIM; }
+
+// The arguments of a list of matrices, each input with the number of the output that may take its place (-1: none may).
+struct Arguments
+{
+	std::vector<std::pair<uintptr_t, int>> in, out;
+	void read(const void* p, int output) { in.push_back({(uintptr_t)p, output}); }
+	void write(const void* p, int output) { out.push_back({(uintptr_t)p, output}); }
+	// No output begins where another one does, or where an input of another one's does: the matrices are worked on at once.
+	bool apart()
+	{
+		std::sort(out.begin(), out.end());
+		for (size_t i = 1; i < out.size(); ++i)
+			if (out[i].first == out[i - 1].first) return false;
+		for (const auto& a : in)
+		{
+			const auto o = std::lower_bound(out.begin(), out.end(), std::make_pair(a.first, -1));
+			if (o != out.end() && o->first == a.first && o->second != a.second) return false;
+		}
+		return true;
+	}
+};
 
 template <class ITEM>
 int64_t workspace(const char* name, const ITEM* items, int count)
@@ -217,6 +241,7 @@ extern "C" int gl_orthogonalize(const gl_ortho_item* items, int32_t count, const
 	try
 	{
 		std::vector<OrthoMatrix> m(count);
+		Arguments all;
 		for (int i = 0; i < count; ++i)
 		{
 			const gl_ortho_item& t = items[i];
@@ -226,7 +251,10 @@ extern "C" int gl_orthogonalize(const gl_ortho_item* items, int32_t count, const
 			m[i].rows = t.rows; m[i].cols = t.cols;
 			m[i].grad = t.d_in; m[i].ld_grad = t.ld_in;
 			m[i].out = t.d_out; m[i].ld_out = t.ld_out;
+			all.read(t.d_in, i);
+			all.write(t.d_out, i);
 		}
+		if (!all.apart()) return report_error(GL_ERR_INVALID, "%s: an output is listed twice, or is another matrix's input", name);
 		return run_ortho(name, a, m, d_work, work_bytes, stream, device);
 	}
 	catch (const std::bad_alloc&)
@@ -252,6 +280,7 @@ extern "C" int gl_muon_step(const gl_muon_item* items, int32_t count, float mome
 	try
 	{
 		std::vector<OrthoMatrix> m(count);
+		Arguments all;
 		for (int i = 0; i < count; ++i)
 		{
 			const gl_muon_item& t = items[i];
@@ -266,7 +295,13 @@ extern "C" int gl_muon_step(const gl_muon_item* items, int32_t count, float mome
 			m[i].mom = t.d_momentum; m[i].mom_out = t.d_momentum_out; m[i].ld_mom = t.ld_momentum;
 			m[i].w = t.d_weight; m[i].w_out = t.d_weight_out; m[i].ld_w = t.ld_weight;
 			m[i].lr = t.lr;
+			all.read(t.d_grad, -1);
+			all.read(t.d_momentum, 2 * i);
+			all.read(t.d_weight, 2 * i + 1);
+			all.write(t.d_momentum_out, 2 * i);
+			all.write(t.d_weight_out, 2 * i + 1);
 		}
+		if (!all.apart()) return report_error(GL_ERR_INVALID, "%s: an output is listed twice, or is another argument than its own input", name);
 		return run_ortho(name, a, m, d_work, work_bytes, stream, device);
 	}
 	catch (const std::bad_alloc&)

@@ -409,7 +409,8 @@ int gl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int6
  * Coefficients under which a singular value of [0, 1] could grow beyond 16 are refused (GL_ERR_INVALID).  Every product is
  * fp32-faithful (three fp16 products on tensor cores), the result is rounded to the output's type once.  A zero matrix
  * gives zeros; a matrix with a NaN or an infinity gives NaN.  In and out are row-major of `type`, pitches in elements; out may
- * be in.  (A column-major matrix is the transposed one row-major: its result comes out transposed too.) */
+ * be in.  The matrices are worked on at once: an output that is listed twice, or is another matrix's input, is refused.
+ * (A column-major matrix is the transposed one row-major: its result comes out transposed too.) */
 typedef struct gl_ortho_item {
 	int32_t rows, cols;
 	const void* d_in;
@@ -424,7 +425,7 @@ int gl_orthogonalize(const gl_ortho_item* items, int32_t count, const float* coe
 /* Momentum update of a list of weight matrices whose direction is orthogonalised, O() as above:
  *     M' = momentum * M + G;   U = G + momentum * M' (nesterov) or M';   W' = (1 - lr * weight_decay) W - lr O(U)
  * G is of `type`, M and W are fp32, each with its own pitch; M' and W' go to d_momentum_out and d_weight_out, which may be
- * d_momentum and d_weight.  lr is the matrix's own: users scale it with sqrt(max(1, rows / cols)) or the like. */
+ * d_momentum and d_weight, but no other argument of the list (refused).  lr is the matrix's own: users scale it with sqrt(max(1, rows / cols)) or the like. */
 typedef struct gl_muon_item {
 	int32_t rows, cols;
 	float lr;

@@ -18,6 +18,12 @@ def status(g, call):
     return 0
 
 
+def last(g, call):
+    with pytest.raises(g.GladesError) as e:
+        call()
+    return str(e.value)
+
+
 def norm(g, **over):
     a = dict(d_x=P, ldx=8, d_gain=P, d_shift=P, d_y=P + 4096, ldy=8, d_mean=P, d_rstd=P, rows=4, n=8)
     a.update(over)
@@ -54,8 +60,8 @@ def ortho_item(**over):
 
 
 def muon_item(**over):
-    a = dict(rows=4, cols=8, lr=0.1, d_grad=P, ld_grad=8, d_momentum=P, d_momentum_out=P, ld_momentum=8, d_weight=P, d_weight_out=P,
-             ld_weight=8)
+    a = dict(rows=4, cols=8, lr=0.1, d_grad=P, ld_grad=8, d_momentum=P + 4096, d_momentum_out=P + 4096, ld_momentum=8, d_weight=P + 8192,
+             d_weight_out=P + 8192, ld_weight=8)
     a.update(over)
     return a
 
@@ -64,7 +70,7 @@ def muon_item(**over):
     dict(rows=0), dict(cols=0), dict(rows=-3), dict(d_in=None), dict(d_out=None), dict(ld_in=7), dict(ld_out=7), dict(d_in=P + 2),
     dict(rows=1 << 30, cols=(1 << 30) + 1)])
 def test_orthogonalize_refuses_matrices(g, over):
-    items = g.ortho_items([ortho_item(), ortho_item(**over)])
+    items = g.ortho_items([ortho_item(d_out=P + 12288), ortho_item(**over)])
     assert status(g, lambda: g.orthogonalize(items, P, 1 << 40)) == INVALID
 
 
@@ -74,6 +80,32 @@ def test_orthogonalize_refuses_matrices(g, over):
 def test_muon_refuses_matrices(g, over):
     items = g.muon_items([muon_item(**over)])
     assert status(g, lambda: g.muon_step(items, P, 1 << 40)) == INVALID
+
+
+def test_orthogonalize_refuses_an_output_twice(g):
+    one = ortho_item()
+    free = dict(d_work=P, work_bytes=1 << 30)
+    for other in (ortho_item(), ortho_item(d_in=P + 12288), ortho_item(d_in=P + 4096, d_out=P + 8192), ortho_item(d_in=P + 12288, d_out=P)):
+        for items in ((one, other), (other, one)):
+            assert status(g, lambda: g.orthogonalize(g.ortho_items(items), **free)) == INVALID
+    # one input for two outputs, and every output in its input's place, are taken: only the device is missing, if that
+    for items in ((one, ortho_item(d_out=P + 8192)), (ortho_item(d_out=P), ortho_item(d_in=P + 4096))):
+        assert status(g, lambda: g.orthogonalize(g.ortho_items(items), P, 100)) == INVALID
+        assert "workspace" in last(g, lambda: g.orthogonalize(g.ortho_items(items), P, 100))
+
+
+@pytest.mark.parametrize("over", [
+    dict(d_weight_out=P + 4096), dict(d_momentum_out=P), dict(d_weight_out=P), dict(d_momentum_out=P + 8192), dict(d_momentum=P + 8192)])
+def test_muon_refuses_an_output_that_is_another_argument(g, over):
+    free = dict(d_work=P, work_bytes=1 << 30)
+    assert status(g, lambda: g.muon_step(g.muon_items([muon_item(**over)]), **free)) == INVALID
+    assert "output" in last(g, lambda: g.muon_step(g.muon_items([muon_item(**over)]), P, 100))
+
+
+def test_muon_refuses_a_matrix_twice(g):
+    assert "output" in last(g, lambda: g.muon_step(g.muon_items([muon_item(), muon_item()]), P, 100))
+    other = muon_item(d_momentum=P + 16384, d_momentum_out=P + 20480, d_weight=P + 24576, d_weight_out=P + 28672)
+    assert "workspace" in last(g, lambda: g.muon_step(g.muon_items([muon_item(), other]), P, 100))
 
 
 @pytest.mark.parametrize("over", [
