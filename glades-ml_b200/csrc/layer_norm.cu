@@ -418,6 +418,11 @@ __device__ __forceinline__ void leave_columns(const LayerNormArgs& p, const Grou
 					dg[v][i] = add2(dg[v][i], __shfl_xor_sync(0xFFFFFFFFu, dg[v][i], o));
 					ds[v][i] = add2(ds[v][i], __shfl_xor_sync(0xFFFFFFFFu, ds[v][i], o));
 				}
+		for (int o = group; o < 32; o <<= 1)
+		{
+			dedge.x += __shfl_xor_sync(0xFFFFFFFFu, dedge.x, o);
+			dedge.y += __shfl_xor_sync(0xFFFFFFFFu, dedge.y, o);
+		}
 	}
 	const int parts = WIDE ? (int)blockDim.x / group : (int)blockDim.x / 32;
 	const int part = WIDE ? gr.index : (int)threadIdx.x / 32;
@@ -866,7 +871,6 @@ cudaError_t backward_mode(const LayerNormArgs& a, int* ctas, cudaStream_t s)
 		smem = std::max(smem, (size_t)threads * 2 * LN_ELEMS * sizeof(T) * quads_stages<T>());
 		return group > 32 ? go(norm_backward_quads_kernel<T, true>) : go(norm_backward_quads_kernel<T, false>);
 	}
-	else if constexpr (MODE == BY_WORDS) return go(norm_backward_kernel<T, MODE, true>);
 	else return group > 32 ? go(norm_backward_kernel<T, MODE, true>) : go(norm_backward_kernel<T, MODE, false>);
 }
 
@@ -911,8 +915,8 @@ cudaError_t backward_type(const LayerNormArgs& a, cudaStream_t s)
 	else
 	{
 		cudaError_t e = cudaErrorInvalidValue;
-		// by words: in a warp of several groups the columns' sums would lie on different lanes
-		const bool words = sizeof(T) == 2 && mode_lanes(a.n, LN_ELEMS, BY_WORDS) > 32 && alike(a.x, a.ldx, a.dy, a.lddy) &&
+		// by words: in a warp of several groups the columns' sums must lie on the same lanes of each
+		const bool words = sizeof(T) == 2 && (mode_lanes(a.n, LN_ELEMS, BY_WORDS) > 32 || (a.ldx & 1) == 0) && alike(a.x, a.ldx, a.dy, a.lddy) &&
 		                   (!a.dx || alike(a.x, a.ldx, a.dx, a.lddx));
 		if (aligned(a, sizeof(T), 16)) e = backward_mode<T, BY_QUADS>(a, &parts, s);
 		else if (!words) e = backward_mode<T, BY_VALUES>(a, &parts, s);

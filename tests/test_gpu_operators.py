@@ -255,6 +255,15 @@ def test_layer_norm_backward_many_rows(g, n):
     check_back(g, 9001, n, "bf16", n, n, n, 0, kind="offset")
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("n,ld,offset", [(1, 2, 0), (1, 2, 1), (2, 2, 1), (3, 4, 0), (17, 18, 1), (50, 50, 0), (100, 100, 0), (101, 102, 3),
+                                         (255, 258, 1), (511, 512, 1), (1025, 1025, 0), (2050, 2050, 1), (8191, 8191, 0)])
+def test_layer_norm_backward_of_rows_of_words(g, t, n, ld, offset):
+    """16-bit rows that begin on an even or an odd element, several or one of them per warp, more of them than groups."""
+    for rows in (3, 149, 9001 if n < 600 else 701):
+        check_back(g, rows, n, t, ld, ld, ld, offset, seed=rows + n)
+
+
 def test_layer_norm_backward_in_place(g):
     for n, t in ((300, "f32"), (4096, "bf16"), (20000, "f16")):
         rows = 33
