@@ -99,6 +99,7 @@ struct OrParams
 	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
 	int* bad;
+	unsigned* arrived;  // CTAs at the rounds' barriers
 	double* sums;  // [matrix][grid] sums of squares
 	float4* part;  // parts of split tiles
 };
@@ -423,6 +424,34 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32])
 	    : "memory");
 }
 
+// The grid barrier: CTAs count themselves without waiting for the count, and then watch it (the cooperative launch has
+// them all resident; against the runtime's barrier it saves a way to L2 and back: 256 x 256, 15 rounds, 110 -> 106 us).  Bounded:
+// false where a CTA has not come.
+constexpr int MEETING_LOST = 2;
+__device__ __forceinline__ bool meet(unsigned* arrived, unsigned all, volatile int* abort_flag, int* err_flag)
+{
+	__syncthreads();
+	if (threadIdx.x == 0)
+	{
+		asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrived) : "memory");
+		const long long t0 = clock64();
+		for (;;)
+		{
+			unsigned v;
+			asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(arrived) : "memory");
+			if (v >= all) break;
+			if (clock64() - t0 > 8 * TC_WAIT_CYCLES)  // (a CTA may have to sit out its own waits)
+			{
+				*abort_flag = MEETING_LOST;
+				atomicExch(err_flag, 5);
+				break;
+			}
+		}
+	}
+	__syncthreads();
+	return *abort_flag != MEETING_LOST;
+}
+
 template <int BN>
 __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __grid_constant__ OrParams P)
 {
@@ -461,7 +490,9 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		mbar_init(bar_given_up, 1);
 		*abort_flag = 0;
 		asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-		if (blockIdx.x == 0 && P.reset) *P.status = 0;  // (nothing can raise it before the first grid barrier)
+		// (nothing can raise the one before the first grid barrier, which is the runtime's, nor count on the other)
+		if (blockIdx.x == 0 && P.reset) *P.status = 0;
+		if (blockIdx.x == 0) *P.arrived = 0;
 	}
 	if (warp == 1)
 	{
@@ -619,7 +650,8 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			}
 		}
 	}
-	grid.sync();
+	unsigned meeting = gridDim.x;
+	const bool met = meet(P.arrived, meeting, abort_flag, P.status);
 
 	// ---- the products
 	int s = 0;             // producer, MMA warp: next stage, and how often (mod 2) the ring has been walked
@@ -630,14 +662,15 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	bool ok = true;
 	OrItem t;              // copying and multiplying warps: a round's first item is looked up in front of the barrier before it
 	if (warp < 2 && (int)blockIdx.x < P.items[0]) find_item<BN>(P, 0, blockIdx.x, t);
-	for (int round = 0; round < P.rounds; ++round)
+	for (int round = 0; met && round < P.rounds; ++round)
 	{
 		const int items = P.items[round];
 		if (warp == 0)
 		{
 			// ------------------------------------------------ TMA producer
-			// (the copies read through another proxy what ordinary stores of all CTAs have written in front of the grid barrier)
-			asm volatile("fence.proxy.async;" ::: "memory");
+			// (the copies read through another proxy what ordinary stores of all CTAs have written to global memory in front of the grid
+			// barrier; a fence for all state spaces costs 0.45 us more in every round)
+			asm volatile("fence.proxy.async.global;" ::: "memory");
 			const bool leader = elect_one();
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
@@ -807,7 +840,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		}
 		if (P.reduce >> round & 1)
 		{
-			grid.sync();
+			if (!meet(P.arrived, meeting += gridDim.x, abort_flag, P.status)) break;
 			if (warp >= S::FIRST)
 			{
 				const uint32_t area = staging0 + (uint32_t)(warp - S::FIRST) * 4096u;
@@ -846,7 +879,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		if (round + 1 < P.rounds)
 		{
 			if (warp < 2 && (int)blockIdx.x < P.items[round + 1]) find_item<BN>(P, round + 1, blockIdx.x, t);
-			grid.sync();
+			if (!meet(P.arrived, meeting += gridDim.x, abort_flag, P.status)) break;
 		}
 	}
 	if (*abort_flag)
@@ -865,7 +898,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
-constexpr size_t OR_HEADER = 256;  // status word
+constexpr size_t OR_HEADER = 256;  // status word; half of it further the barriers' count
 constexpr size_t OR_SUMS = (size_t)ORTHO_MAX_MATRICES * OR_SMS * sizeof(double);
 size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 
@@ -1295,6 +1328,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 		P.status = status;
 		P.reset = first == 0 && !a.status;
 		at += OR_HEADER;
+		P.arrived = reinterpret_cast<unsigned*>(at - OR_HEADER / 2);
 		P.sums = reinterpret_cast<double*>(at);
 		at += round_up(OR_SUMS, 256);
 		P.part = reinterpret_cast<float4*>(at);
