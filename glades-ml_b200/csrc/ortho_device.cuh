@@ -1,6 +1,8 @@
 // What the kernels of the orthogonalisation share: programs of products, the caller's elements, parts, waits and MMAs of a
 // warp that stays together (orthogonalize.cu, ortho_small.cu).
 #pragma once
+#include <algorithm>
+
 #include <cuda_bf16.h>
 
 #include "orthogonalize.h"
@@ -22,6 +24,17 @@ struct OrOp
 	signed char round;
 	float f, w1, w2, so;
 };
+// The factor of an operation's products.  Tensor cores cut off what a sum cannot hold, so that sums of products come out too small:
+// measured on orthogonal rows, by 2.1e-7 where an accumulator takes eight 16-k steps, by up to 5e-7 on the diagonal of A A, where one product is
+// far larger than the others; by nothing where there is one product.  The polynomial multiplies such an error of all
+// singular values by up to 15, so it is taken back here (64 x 512: 3.0e-6 -> 1.8e-6; fp32 products 1.6e-6).
+inline float product_factor(const OrOp& o, int p, int q, int additions)
+{
+	const int k = o.a >= ID_X ? q : p;
+	const double cut = 2.1e-7 * std::min(1.0, k / (o.a >= ID_X ? 128.0 : 32.0)) * std::max(1.0, std::min(additions, k / 16) / 8.0) +
+	                   (o.a == ID_A && o.b == ID_A ? 3.2e-7 * std::min(1.0, p / 96.0) : 0.0);
+	return (float)(o.f * (1.0 + cut));
+}
 struct OrProgram
 {
 	OrOp op[OR_MAX_OPS];

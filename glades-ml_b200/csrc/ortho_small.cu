@@ -20,7 +20,7 @@ namespace {
 
 constexpr int SM_WARPS = 16;                        // epilogue warps: four for each quarter of tensor memory's lanes
 constexpr int SM_THREADS = 32 * (SM_WARPS + 1);     // and one that multiplies
-constexpr int SM_K = 24;                            // 16-k steps that an accumulator takes before it is drained (24 additions)
+constexpr int SM_K = 8;                             // 16-k steps that an accumulator takes before it is drained
 constexpr int SM_TMEM = 512, SM_BUFFER = 256;       // columns: all, and of one of the two accumulators
 constexpr int SM_SMEM = 227 * 1024;
 
@@ -34,6 +34,7 @@ struct SmParams
 {
 	OrProgram prog;
 	SmMat mat[ORTHO_MAX_MATRICES];
+	float factor[ORTHO_MAX_MATRICES][OR_MAX_OPS];  // product_factor
 	int count, type, step, nesterov, reset;
 	float mu, decay, eps, s0;
 	int* status;
@@ -60,7 +61,11 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 	const SmMat& M = P.mat[blockIdx.x];
 	const OrthoMatrix& m = M.m;
 	const int count = P.prog.count;
-	for (int i = threadIdx.x; i < count; i += SM_THREADS) ops[i] = P.prog.op[i];
+	for (int i = threadIdx.x; i < count; i += SM_THREADS)
+	{
+		ops[i] = P.prog.op[i];
+		ops[i].f = P.factor[blockIdx.x][i];
+	}
 	const uint32_t raw = smem_u32(smem_raw);
 	const uint32_t base = (raw + 1023u) & ~1023u;
 	uint8_t* gen = smem_raw + (base - raw);
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 #pragma unroll
 						for (int u = 0; u < 2; ++u)
 #pragma unroll
-							for (int i = 0; i < 8; ++i) acc[u0 + u][i] += __uint_as_float(x[u][i]) + __uint_as_float(h[u][i]);
+							for (int i = 0; i < 8; ++i) acc[u0 + u][i] = fmaf(o.f, __uint_as_float(h[u][i]), fmaf(o.f, __uint_as_float(x[u][i]), acc[u0 + u][i]));
 					}
 				}
 				asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -336,12 +341,11 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 						add(o.e2, o.w2);
 						if (o.out != ID_NONE)
 						{
-							const float f = o.f * o.so;
 							uint4 h4, l4;
-							split_pair(v[0], v[1], f, h4.x, l4.x);
-							split_pair(v[2], v[3], f, h4.y, l4.y);
-							split_pair(v[4], v[5], f, h4.z, l4.z);
-							split_pair(v[6], v[7], f, h4.w, l4.w);
+							split_pair(v[0], v[1], o.so, h4.x, l4.x);
+							split_pair(v[2], v[3], o.so, h4.y, l4.y);
+							split_pair(v[4], v[5], o.so, h4.z, l4.z);
+							split_pair(v[6], v[7], o.so, h4.w, l4.w);
 							uint8_t* e = gen + (at(o.out) - base) + off;
 							*reinterpret_cast<uint4*>(e) = h4;
 							*reinterpret_cast<uint4*>(e + part) = l4;
@@ -353,7 +357,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 #pragma unroll
 							for (int i = 0; i < 4; ++i)
 							{
-								const uint32_t b0 = __float_as_uint(v[2 * i] * o.f), b1 = __float_as_uint(v[2 * i + 1] * o.f);
+								const uint32_t b0 = __float_as_uint(v[2 * i]), b1 = __float_as_uint(v[2 * i + 1]);
 								hw[i] = __byte_perm(b0, b1, 0x7632);
 								lw[i] = __byte_perm(b0, b1, 0x5410);
 							}
@@ -488,6 +492,7 @@ cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float 
 		M.tall = M.m.rows > M.m.cols;
 		M.rows = (M.p + 15) / 16 * 16;
 		M.chunks = (M.q + 63) / 64;
+		for (int k = 0; k < prog.count; ++k) P.factor[i][k] = product_factor(prog.op[k], M.p, M.q, SM_K);
 		smem = std::max(smem, small_bytes(M.p, M.q));
 	}
 	static_assert(sizeof(SmParams) < 32764, "kernel parameters");

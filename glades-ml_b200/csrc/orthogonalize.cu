@@ -20,8 +20,8 @@
 // (Tiles of 256 columns, which only fit with one accumulator for all three products, lost: their epilogue holds 128 sums per
 // thread, spills, and the MMAs wait for it.  4096 x 4096, a step: 769 us against 655.)
 // a X (b A, a T, ..) is where the epilogue's registers start from, loaded while the first chunk is computed: inside the accumulator
-// it would be truncated with every addition, which doubles the error of the result (3.3e-6 against 1.3e-6 of a 256 x 256
-// matrix, fp32 products: 2.5e-6).
+// it would be truncated with every addition, which doubles the error of the result.  The products are multiplied by their own
+// coefficient as they are added, so that every coefficient is used as it is given.
 // A, R, T and Q are symmetric: tiles above the diagonal are left out, an element below it is stored at both places.
 //
 // One cooperative launch walks all steps of all matrices: norm, scaling, then rounds of products that do not depend on one
@@ -48,14 +48,18 @@ constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_PROGRAMS = 3;
 constexpr int OR_SMS = 148;
+constexpr int OR_CHUNK = 2;    // stages whose products an accumulator takes before it is drained
 constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 
 template <int BN>
 struct OrSmem
 {
-	// Stages whose products an accumulator takes before it is drained: the tensor core truncates as it adds, so a chain of n
-	// additions drifts by up to n * 2^-24 towards zero; 6 stages are 24 additions of full size.
-	static constexpr int CHUNK = 6;
+	// The tensor core truncates as it adds, so a chain of n additions drifts by up to n * 2^-24 towards zero; two stages are eight
+	// additions of full size, and what they still lose on average is taken back (product_factor).  Errors of random matrices against
+	// 64 bits, six stages -> two and the factor (fp32 products): 256 x 1000 6.0e-6 -> 2.3e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 4.0e-6
+	// (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  It costs the epilogue 0 to 15 % of the time: 256 x 256 103 -> 105 us, 2048 x 2048
+	// 482 -> 510, 1024 x 8192 361 -> 425.
+	static constexpr int CHUNK = OR_CHUNK;
 	static constexpr int COLUMNS = 2 * BN;                   // of an accumulator
 	static constexpr int STAGES = BN == 128 ? 3 : 4;
 	static constexpr int EC = BN / 2;                        // columns per epilogue warp
@@ -92,6 +96,7 @@ struct OrParams
 	OrMat mat[ORTHO_MAX_MATRICES];
 	OrProgram prog[OR_PROGRAMS];  // step by step; in groups of two; with three steps in the first
 	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
+	float factor[ORTHO_MAX_MATRICES][OR_MAX_OPS];  // product_factor
 	unsigned long long reduce;  // rounds with split tiles
 	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
 	int count, rounds, units;
@@ -359,7 +364,6 @@ struct OrTarget
 	long long plane, ld;
 	__device__ __forceinline__ OrTarget(const OrMat& M, const OrOp& o)
 	{
-		f = o.f;
 		so = o.so;
 		p = M.p;
 		q = M.q;
@@ -377,8 +381,6 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, int mat, const O
 {
 	if (T.kind == 0)
 	{
-#pragma unroll
-		for (int i = 0; i < 32; ++i) v[i] *= T.f;
 		const OrMat& M = P.mat[mat];
 		if (!M.tall) transpose(v, area, lane);
 		// a wide matrix: lane = column, v = rows r0 ..; a tall one is transposed already: lane = its column, v = its rows c0 ..
@@ -400,7 +402,7 @@ __device__ __forceinline__ void finish_piece(const OrParams& P, int mat, const O
 		for (int j = 0; j < 32; ++j)
 			if (j > lane) v[j] = square_get(area, j, lane);
 	}
-	stage_parts(v, T.f * T.so, area, lane);
+	stage_parts(v, T.so, area, lane);
 	store_staged(T.D + (long long)r0 * T.ld + c0, T.plane, T.ld, area, lane);
 	if (T.kind == 1 && c0 != r0)
 	{
@@ -777,6 +779,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				const OrMat& M = P.mat[t.mat];
 				const OrOp& o = P.prog[M.program].op[t.op];
 				const OrTarget target(M, o);
+				const float f = P.factor[t.mat][t.op];
 				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
 				float acc[EC];
 #pragma unroll
@@ -809,7 +812,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 							tmem_ld32(taddr + (uint32_t)(h * BN + c * 32), r);
 							asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-							for (int e = 0; e < 32; ++e) acc[c * 32 + e] += __uint_as_float(r[e]);
+							for (int e = 0; e < 32; ++e) acc[c * 32 + e] = fmaf(f, __uint_as_float(r[e]), acc[c * 32 + e]);
 						}
 					asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
 					__syncwarp();
@@ -995,11 +998,10 @@ void make_program(OrProgram& g, const float (*coef)[3], const Bounds& b, const i
 		OrOp& o = g.op[g.count++];
 		o.a = (signed char)a; o.b = (signed char)bb; o.e1 = (signed char)e1; o.e2 = (signed char)e2; o.out = (signed char)out;
 		o.round = (signed char)round;
-		// (a factor of zero: so small a one that nothing of the product is left beside w1 E1)
-		const double factor = (fabs(f) < 0x1p-40 ? 0x1p-40 : f) / scale[a] / scale[bb];
-		o.f = (float)factor;
-		o.w1 = e1 == ID_NONE ? 0.0f : (float)(w1 / scale[e1] / factor);
-		o.w2 = e2 == ID_NONE ? 0.0f : (float)(w2 / scale[e2] / factor);
+		// (the scales are powers of two: the coefficients stay as they are)
+		o.f = (float)(f / scale[a] / scale[bb]);
+		o.w1 = e1 == ID_NONE ? 0.0f : (float)(w1 / scale[e1]);
+		o.w2 = e2 == ID_NONE ? 0.0f : (float)(w2 / scale[e2]);
 		o.so = out == ID_NONE ? 1.0f : scale_under(bound);
 	};
 	for (int i = 0; i < groups; ++i)
@@ -1203,6 +1205,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
 		P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
 		bytes += matrix_bytes(M, g.planes);
+		for (int k = 0; k < g.count; ++k) P.factor[i][k] = product_factor(g.op[k], M.p, M.q, OR_CHUNK * OR_BK / 16);
 	}
 	long long best = -1;
 	for (int bn : {128, 64})
