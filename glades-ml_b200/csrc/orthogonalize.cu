@@ -48,18 +48,18 @@ constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_PROGRAMS = 3;
 constexpr int OR_SMS = 148;
-constexpr int OR_CHUNK = 2;    // stages whose products an accumulator takes before it is drained
+// Stages whose products an accumulator takes before it is drained.  The tensor core truncates as it adds, so a chain of n additions
+// drifts by up to n * 2^-24 towards zero; two stages are eight additions of full size, and what they still lose on average is taken
+// back (product_factor).  Errors of random matrices against 64 bits, with six stages and no factor -> with two and the factor (fp32
+// products): 256 x 1000 6.0e-6 -> 2.2e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 3.9e-6 (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  It costs
+// 0 to 15 % of the time (256 x 256 103 -> 105 us, 2048 x 2048 482 -> 510, 1024 x 8192 361 -> 425), which results of 16 bits, off by
+// 5e-4 or more anyway, need not pay.
+constexpr int OR_CHUNK = 2, OR_CHUNK_16 = 6;
 constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 
 template <int BN>
 struct OrSmem
 {
-	// The tensor core truncates as it adds, so a chain of n additions drifts by up to n * 2^-24 towards zero; two stages are eight
-	// additions of full size, and what they still lose on average is taken back (product_factor).  Errors of random matrices against
-	// 64 bits, six stages -> two and the factor (fp32 products): 256 x 1000 6.0e-6 -> 2.3e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 4.0e-6
-	// (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  It costs the epilogue 0 to 15 % of the time: 256 x 256 103 -> 105 us, 2048 x 2048
-	// 482 -> 510, 1024 x 8192 361 -> 425.
-	static constexpr int CHUNK = OR_CHUNK;
 	static constexpr int COLUMNS = 2 * BN;                   // of an accumulator
 	static constexpr int STAGES = BN == 128 ? 3 : 4;
 	static constexpr int EC = BN / 2;                        // columns per epilogue warp
@@ -100,6 +100,7 @@ struct OrParams
 	unsigned long long reduce;  // rounds with split tiles
 	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
 	int count, rounds, units;
+	int chunk;  // stages whose products an accumulator takes before it is drained
 	int type, step, nesterov, reset;
 	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
@@ -740,7 +741,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 					const uint32_t off = (uint32_t)s * (S::STAGE_BYTES >> 4);
 					const uint32_t a0 = a_low + off, b0 = b_low + off;
 					const uint32_t d = tmem_base + (uint32_t)(buf * S::COLUMNS);
-					const bool ends = in + 1 == S::CHUNK || left == 1;
+					const bool ends = in + 1 == P.chunk || left == 1;
 					if (leader)
 					{
 #pragma unroll
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 							add_parts(acc + pc * 32, o.w2, o.e2, M, r0 + lane, c00 + pc * 32);
 						}
 				}
-				for (int done = t.kb0; done < t.kb1; done += S::CHUNK)
+				for (int done = t.kb0; done < t.kb1; done += P.chunk)
 				{
 					if (!warp_wait(bar_acc_full + 8 * buf, aph, abort_flag, P.status, 3))
 					{
@@ -1179,6 +1180,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.decay = a.decay;
 	P.eps = a.eps;
 	P.bad = a.bad;
+	P.chunk = !a.step && a.type != GL_F32 ? OR_CHUNK_16 : OR_CHUNK;
 	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
 	for (int i = 0; i < count; ++i)
 	{
@@ -1205,7 +1207,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
 		P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
 		bytes += matrix_bytes(M, g.planes);
-		for (int k = 0; k < g.count; ++k) P.factor[i][k] = product_factor(g.op[k], M.p, M.q, OR_CHUNK * OR_BK / 16);
+		for (int k = 0; k < g.count; ++k) P.factor[i][k] = product_factor(g.op[k], M.p, M.q, P.chunk * OR_BK / 16);
 	}
 	long long best = -1;
 	for (int bn : {128, 64})
