@@ -144,8 +144,10 @@ __device__ __forceinline__ void mma(bool first, uint32_t d, uint32_t a, uint32_t
 	    : "memory");
 }
 
-// small matrices (ortho_small.cu): whether one is, and the launch for a.mat[first] .. [first + count - 1], which all are
+// small matrices (ortho_small.cu): whether one is, whether one is a single row or column, and the launch for m[0] .. [count - 1], each of
+// which is one or the other
 bool ortho_small(int rows, int cols);
-cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, int first, int count, int* status, bool reset, cudaStream_t s);
+bool ortho_vector(const OrthoMatrix& m);
+cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, cudaStream_t s);
 
 }  // namespace glb

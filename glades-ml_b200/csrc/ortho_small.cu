@@ -11,6 +11,8 @@
 // accumulator that nobody reads.
 // X <- q X + Q X and R <- b A + c A^2 are written over what they are made of: the MMAs that read a chunk are done when it is written,
 // and every element's own old value is read by the thread that writes it.
+#include <string.h>
+
 #include <algorithm>
 
 #include "ortho_device.cuh"
@@ -27,7 +29,7 @@ constexpr int SM_SMEM = 227 * 1024;
 struct SmMat
 {
 	OrthoMatrix m;
-	int p, q, tall;
+	int p, q, tall, vector;
 	int rows, chunks;  // rows of a chunk, chunks of X
 };
 struct SmParams
@@ -35,7 +37,8 @@ struct SmParams
 	OrProgram prog;
 	SmMat mat[ORTHO_MAX_MATRICES];
 	float factor[ORTHO_MAX_MATRICES][OR_MAX_OPS];  // product_factor
-	int count, type, step, nesterov, reset;
+	float coef[ORTHO_MAX_STEPS][3];
+	int count, steps, type, step, nesterov, reset;
 	float mu, decay, eps, s0;
 	int* status;
 	int* bad;
@@ -50,6 +53,62 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
 	             : "r"(taddr));
 }
 
+// A single row or column: X stays U times a number, A = X X^T is a number, and so are the steps: they are done in double, and the result
+// is rounded once (three fp16 products: 1 to 2e-6 off, since every step multiplies the one number's rounding).
+__device__ __noinline__ void orthogonalize_vector(const SmParams& P, const SmMat& M, double* warp_sums)
+{
+	const OrthoMatrix& m = M.m;
+	auto at = [&](int e, long long ld) { return m.cols == 1 ? e * ld : (long long)e; };
+	double sum = 0.0;
+	for (int e = threadIdx.x; e < M.q; e += SM_THREADS)
+	{
+		float u = load_typed(m.grad, at(e, m.ld_grad), P.type);
+		if (P.step)
+		{
+			const float v = fmaf(P.mu, m.mom[at(e, m.ld_mom)], u);
+			m.mom_out[at(e, m.ld_mom)] = v;
+			u = P.nesterov ? fmaf(P.mu, v, u) : v;
+		}
+		sum = fma((double)u, (double)u, sum);
+	}
+#pragma unroll
+	for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+	if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x / 32] = sum;
+	__syncthreads();
+	sum = 0.0;
+	for (int w = 0; w < SM_THREADS / 32; ++w) sum += warp_sums[w];
+	const double inv = 1.0 / ((double)(float)sqrt(sum) + (double)P.eps);
+	double a = sum * inv * inv, factor = inv;
+	for (int k = 0; k < P.steps; ++k)
+	{
+		const double f = (double)P.coef[k][0] + a * ((double)P.coef[k][1] + a * (double)P.coef[k][2]);
+		factor *= f;
+		a *= f * f;
+	}
+	const float keep = 1.0f - m.lr * P.decay;
+	bool finite = true;
+	for (int e = threadIdx.x; e < M.q; e += SM_THREADS)
+	{
+		float u;
+		if (P.step)
+		{
+			u = m.mom_out[at(e, m.ld_mom)];
+			if (P.nesterov) u = fmaf(P.mu, u, load_typed(m.grad, at(e, m.ld_grad), P.type));
+		}
+		else u = load_typed(m.grad, at(e, m.ld_grad), P.type);
+		const float o = (float)(u * factor);
+		if (!P.step)
+		{
+			store_typed(m.out, at(e, m.ld_out), o, P.type);
+			continue;
+		}
+		const float w = fmaf(-m.lr, o, keep * m.w[at(e, m.ld_w)]);
+		finite = finite && isfinite(w);
+		m.w_out[at(e, m.ld_w)] = w;
+	}
+	if (P.step && P.bad && !finite) atomicOr(P.bad, 1);
+}
+
 __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid_constant__ SmParams P)
 {
 	extern __shared__ uint8_t smem_raw[];
@@ -60,6 +119,12 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 	__shared__ OrOp ops[OR_MAX_OPS];  // (from constant memory every operation would cost a miss on the way)
 	const SmMat& M = P.mat[blockIdx.x];
 	const OrthoMatrix& m = M.m;
+	if (M.vector)
+	{
+		if (blockIdx.x == 0 && threadIdx.x == 0 && P.reset) *P.status = 0;
+		orthogonalize_vector(P, M, warp_sums);
+		return;
+	}
 	const int count = P.prog.count;
 	for (int i = threadIdx.x; i < count; i += SM_THREADS)
 	{
@@ -467,7 +532,13 @@ bool ortho_small(int rows, int cols)
 	return p <= 128 && q <= 512 && small_bytes(p, q) <= SM_SMEM - 2048;
 }
 
-cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, int first, int count, int* status, bool reset, cudaStream_t s)
+// (up to 1 << 17 elements: 240 of one thread.  Columns that move within their own memory are left to the kernels that read all first.)
+bool ortho_vector(const OrthoMatrix& m)
+{
+	return std::min(m.rows, m.cols) == 1 && std::max(m.rows, m.cols) <= 1 << 17 && !(m.cols == 1 && m.out && m.out == m.grad && m.ld_out != m.ld_grad);
+}
+
+cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, cudaStream_t s)
 {
 	SmParams& P = t_small;
 	P.prog = prog;
@@ -482,18 +553,21 @@ cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float 
 	P.bad = a.bad;
 	P.s0 = s0;
 	P.status = status;
+	P.steps = a.steps;
+	memcpy(P.coef, a.coef, sizeof P.coef);
 	size_t smem = 0;
 	for (int i = 0; i < count; ++i)
 	{
 		SmMat& M = P.mat[i];
-		M.m = a.mat[first + i];
+		M.m = m[i];
+		M.vector = ortho_vector(m[i]);
 		M.p = std::min(M.m.rows, M.m.cols);
 		M.q = std::max(M.m.rows, M.m.cols);
 		M.tall = M.m.rows > M.m.cols;
 		M.rows = (M.p + 15) / 16 * 16;
 		M.chunks = (M.q + 63) / 64;
 		for (int k = 0; k < prog.count; ++k) P.factor[i][k] = product_factor(prog.op[k], M.p, M.q, SM_K);
-		smem = std::max(smem, small_bytes(M.p, M.q));
+		if (!M.vector) smem = std::max(smem, small_bytes(M.p, M.q));
 	}
 	static_assert(sizeof(SmParams) < 32764, "kernel parameters");
 	int sms = 0;

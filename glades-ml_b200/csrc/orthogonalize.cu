@@ -1314,24 +1314,39 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 	OrParams& P = t_params;
 	for (int first = 0; first < a.count; first += ORTHO_MAX_MATRICES)
 	{
-		// A list of small matrices only goes to one CTA for each of them; beside larger ones they ride along.
-		const int count = std::min(ORTHO_MAX_MATRICES, a.count - first);
+		// A list of small matrices only goes to one CTA for each of them; beside larger ones they ride along, but single rows and
+		// columns, which go to one CTA each behind the others.
+		const int all = std::min(ORTHO_MAX_MATRICES, a.count - first);
 		int* const status = a.status ? a.status : ortho_status(work);
+		const bool reset = first == 0 && !a.status;
+		OrthoMatrix m[ORTHO_MAX_MATRICES], vectors[ORTHO_MAX_MATRICES];
+		int count = 0, n = 0;
 		bool small = true;
-		for (int i = first; i < first + count && small; ++i) small = ortho_small(a.mat[i].rows, a.mat[i].cols);
+		for (int i = first; i < first + all; ++i)
+		{
+			const OrthoMatrix& x = a.mat[i];
+			if (ortho_vector(x)) vectors[n++] = x;
+			else
+			{
+				small = small && ortho_small(x.rows, x.cols);
+				m[count++] = x;
+			}
+		}
+		if (small)
+			while (n > 0) m[count++] = vectors[--n];
 		if (small)
 		{
 			const float s0 = make_programs(P.prog, 1, a);
-			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, first, count, status, first == 0 && !a.status, s);
+			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, m, count, status, reset, s);
 			if (e != cudaSuccess) return e;
 			continue;
 		}
 		Plan plan;
-		const size_t need = make_plan(P, a, a.mat + first, count, plan);
+		const size_t need = make_plan(P, a, m, count, plan);
 		if (need + 256 > work_bytes) return cudaErrorInvalidValue;
 		char* at = reinterpret_cast<char*>(ortho_status(work));
 		P.status = status;
-		P.reset = first == 0 && !a.status;
+		P.reset = reset;
 		at += OR_HEADER;
 		P.arrived = reinterpret_cast<unsigned*>(at - OR_HEADER / 2);
 		P.sums = reinterpret_cast<double*>(at);
@@ -1345,7 +1360,8 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			M.S = M.X + 4 * M.planex;
 			at += matrix_bytes(M, P.prog[M.program].planes);
 		}
-		const cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
+		cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
+		if (e == cudaSuccess && n > 0) e = launch_ortho_small(a, P.prog[0], P.s0, vectors, n, status, false, s);
 		if (e != cudaSuccess) return e;
 	}
 	return cudaSuccess;

@@ -469,6 +469,57 @@ def test_orthogonalize_in_place_and_repeatable(g):
         assert torch.equal(a, b)
 
 
+def vector_exact(u, steps=5, off=0.0):
+    """O of a single row or column with the coefficients as fp32 holds them; off: its norm's relative error."""
+    u = u.double()
+    norm = u.norm() * (1.0 + off)
+    x = u / (norm + 1e-7)
+    factor, gram = 1.0, (x * x).sum()
+    for a, b, c in coefs(steps):
+        a, b, c = (float(torch.tensor(v, dtype=torch.float32)) for v in (a, b, c))
+        f = a + gram * (b + gram * c)
+        factor, gram = factor * f, gram * f * f
+    return x * factor
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("beside", [None, (40, 30), (300, 260)])
+def test_orthogonalize_single_rows_and_columns(g, t, beside):
+    """The only roundings are the norm's (half a step of fp32, and what the steps make of it) and the result's two."""
+    ins, outs, bufs = [], [], []
+    for i, (m, n, pad) in enumerate([(1, 1, 0), (1, 256, 0), (256, 1, 0), (256, 1, 6), (1, 545, 3), (40001, 1, 2), (1, 131072, 0)]):
+        _, a = matrix(m, n, n + pad, t, i % 2)
+        a.copy_(torch.randn(m, n, generator=gen(i), device=DEV))
+        buf, b = matrix(m, n, n + 2 * pad, t, i % 3, fill=3.0)
+        ins.append(a), outs.append(b), bufs.append(buf)
+    ins[4][0, 7] = float("nan")
+    if beside:
+        ins.append(gradient(*beside, 9).to(TYPES[t])), outs.append(torch.empty_like(ins[-1]))
+    run_ortho(g, ins, outs, t)
+    for a, b, buf in zip(ins, outs, bufs):
+        assert untouched(buf, b, 3.0)
+        if a is ins[4]:
+            assert bool(torch.isnan(b).all())
+            continue
+        exact = vector_exact(a)
+        tol = sum((vector_exact(a, off=o) - exact).abs() for o in (1.01 * U, -1.01 * U)) + 1e-12 * exact.abs()
+        tol = tol + (U + HALF[t]) * exact.abs() * 1.01 + TINY[t]
+        assert bool(((b.double() - exact).abs() <= tol).all()), (tuple(a.shape), float(((b.double() - exact).abs() / tol).max()))
+
+
+def test_orthogonalize_long_and_moving_single_columns(g):
+    """Those that the kernels of matrices take: beyond 131072 elements, and a column whose result has another pitch in its place."""
+    check_ortho(g, [(1, 131073), (140000, 1)])
+    buf = torch.zeros(3 * 500, device=DEV)
+    a = buf.view(500, 3)[:, :1]
+    a.copy_(torch.randn(500, 1, generator=gen(4), device=DEV))
+    u = a.clone()
+    out = buf[:1000].view(500, 2)[:, :1]
+    run_ortho(g, [a], [out], "f32")
+    exact = iterate(u.double(), 5, coefs(5), 1e-7, torch.float64)
+    assert bool(((out.double() - exact).abs() <= ortho_tolerance(u, 5, coefs(5), 1e-7, exact)).all())
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("nesterov", [False, True])
 def test_muon_step(g, t, nesterov):
