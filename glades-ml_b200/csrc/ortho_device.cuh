@@ -145,9 +145,9 @@ __device__ __forceinline__ void mma(bool first, uint32_t d, uint32_t a, uint32_t
 }
 
 // small matrices (ortho_small.cu): whether one is, whether one is a single row or column, and the launch for m[0] .. [count - 1], each of
-// which is one or the other
+// which is one or the other (beside: single rows and columns only, which may run beside the kernel in front of them on the stream)
 bool ortho_small(int rows, int cols);
 bool ortho_vector(const OrthoMatrix& m);
-cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, cudaStream_t s);
+cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, bool beside, cudaStream_t s);
 
 }  // namespace glb

@@ -60,6 +60,7 @@ __device__ __noinline__ void orthogonalize_vector(const SmParams& P, const SmMat
 	const OrthoMatrix& m = M.m;
 	auto at = [&](int e, long long ld) { return m.cols == 1 ? e * ld : (long long)e; };
 	double sum = 0.0;
+#pragma unroll 4
 	for (int e = threadIdx.x; e < M.q; e += SM_THREADS)
 	{
 		float u = load_typed(m.grad, at(e, m.ld_grad), P.type);
@@ -87,6 +88,7 @@ __device__ __noinline__ void orthogonalize_vector(const SmParams& P, const SmMat
 	}
 	const float keep = 1.0f - m.lr * P.decay;
 	bool finite = true;
+#pragma unroll 4
 	for (int e = threadIdx.x; e < M.q; e += SM_THREADS)
 	{
 		float u;
@@ -123,6 +125,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 	{
 		if (blockIdx.x == 0 && threadIdx.x == 0 && P.reset) *P.status = 0;
 		orthogonalize_vector(P, M, warp_sums);
+		cudaGridDependencySynchronize();  // (it may have been let in beside the kernel in front, which the stream's next work waits for too)
 		return;
 	}
 	const int count = P.prog.count;
@@ -532,13 +535,14 @@ bool ortho_small(int rows, int cols)
 	return p <= 128 && q <= 512 && small_bytes(p, q) <= SM_SMEM - 2048;
 }
 
-// (up to 1 << 17 elements: 240 of one thread.  Columns that move within their own memory are left to the kernels that read all first.)
+// (up to 1 << 17 elements, which take one CTA 130 us; 1 x 20000 in rounds of products takes 300.  Columns that move within their own
+// memory are left to the kernels that read all of it first.)
 bool ortho_vector(const OrthoMatrix& m)
 {
 	return std::min(m.rows, m.cols) == 1 && std::max(m.rows, m.cols) <= 1 << 17 && !(m.cols == 1 && m.out && m.out == m.grad && m.ld_out != m.ld_grad);
 }
 
-cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, cudaStream_t s)
+cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float s0, const OrthoMatrix* m, int count, int* status, bool reset, bool beside, cudaStream_t s)
 {
 	SmParams& P = t_small;
 	P.prog = prog;
@@ -572,8 +576,17 @@ cudaError_t launch_ortho_small(const OrthoArgs& a, const OrProgram& prog, float 
 	static_assert(sizeof(SmParams) < 32764, "kernel parameters");
 	int sms = 0;
 	if (cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(&ortho_small_kernel), SM_SMEM - 2048, &sms)) return e;
-	ortho_small_kernel<<<(unsigned)count, SM_THREADS, smem, s>>>(P);
-	return cudaGetLastError();
+	cudaLaunchConfig_t cfg = {};
+	cfg.gridDim = dim3((unsigned)count);
+	cfg.blockDim = dim3(SM_THREADS);
+	cfg.dynamicSmemBytes = smem;
+	cfg.stream = s;
+	cudaLaunchAttribute at[1];
+	at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+	at[0].val.programmaticStreamSerializationAllowed = 1;
+	cfg.attrs = at;
+	cfg.numAttrs = beside ? 1 : 0;
+	return cudaLaunchKernelEx(&cfg, ortho_small_kernel, (const SmParams)P);
 }
 
 }  // namespace glb

@@ -476,6 +476,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	double* warp_sums = reinterpret_cast<double*>(tail + 8);  // 10 at most
 
 	cg::grid_group grid = cg::this_grid();
+	cudaTriggerProgrammaticLaunchCompletion();  // (single rows and columns have nothing to wait for)
 	const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
 	if (threadIdx.x == 0)
@@ -1337,7 +1338,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 		if (small)
 		{
 			const float s0 = make_programs(P.prog, 1, a);
-			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, m, count, status, reset, s);
+			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, m, count, status, reset, false, s);
 			if (e != cudaSuccess) return e;
 			continue;
 		}
@@ -1361,7 +1362,7 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			at += matrix_bytes(M, P.prog[M.program].planes);
 		}
 		cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
-		if (e == cudaSuccess && n > 0) e = launch_ortho_small(a, P.prog[0], P.s0, vectors, n, status, false, s);
+		if (e == cudaSuccess && n > 0) e = launch_ortho_small(a, P.prog[0], P.s0, vectors, n, status, false, true, s);
 		if (e != cudaSuccess) return e;
 	}
 	return cudaSuccess;

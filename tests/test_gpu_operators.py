@@ -507,6 +507,49 @@ def test_orthogonalize_single_rows_and_columns(g, t, beside):
         assert bool(((b.double() - exact).abs() <= tol).all()), (tuple(a.shape), float(((b.double() - exact).abs() / tol).max()))
 
 
+def test_single_rows_beside_a_matrix_in_order_and_in_a_graph(g):
+    """What comes before and behind the call on the stream sees it as one: the row's input is made in front of it, its output
+    and the matrix's are used behind it, eager and replayed."""
+    big, row = gradient(400, 300, 1), torch.randn(1, 300, generator=gen(2), device=DEV)
+    src, out = [torch.empty_like(big), torch.empty_like(row)], [torch.empty_like(big), torch.empty_like(row)]
+    items = g.ortho_items([dict(rows=a.shape[0], cols=a.shape[1], d_in=a.data_ptr(), ld_in=a.shape[1], d_out=b.data_ptr(), ld_out=a.shape[1])
+                           for a, b in zip(src, out)])
+    bytes_ = g.orthogonalize_workspace(items)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=DEV)
+    got = [torch.empty_like(big), torch.empty_like(row)]
+
+    def call():
+        for a, b in zip(src, (big, row)):
+            a.copy_(b)
+        g.orthogonalize(items, work.data_ptr(), bytes_, stream=stream())
+        for a, b in zip(got, out):
+            a.copy_(b)
+        for a in src + out:
+            a.fill_(float("nan"))
+
+    call()
+    want = [a.clone() for a in got]
+    assert bool(((want[1].double() - vector_exact(row)).abs() <= 1e-6).all()) and bool(torch.isfinite(want[0]).all())
+    for _ in range(20):
+        call()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        call()
+    for _ in range(20):
+        for a in got:
+            a.zero_()
+        graph.replay()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_orthogonalize_long_and_moving_single_columns(g):
     """Those that the kernels of matrices take: beyond 131072 elements, and a column whose result has another pitch in its place."""
     check_ortho(g, [(1, 131073), (140000, 1)])
