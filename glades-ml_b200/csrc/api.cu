@@ -17,6 +17,9 @@
 #include <string>
 #include <vector>
 
+#include <memory>
+#include <new>
+
 #include "host_copy.h"
 #include "internal.h"
 #include "orthogonalize.h"
@@ -954,9 +957,10 @@ extern "C" int gl_set_layer_norm(gl_net* n, int32_t layer, float eps)
 	{
 		const size_t w = (size_t)n->d.sizes[layer];
 		if (!t.param) CU(cudaMalloc(&t.param, 4 * w * sizeof(float)));
-		std::vector<float> p(4 * w, 0.0f);
-		std::fill(p.begin(), p.begin() + w, 1.0f);
-		CU(cudaMemcpyAsync(t.param, p.data(), p.size() * sizeof(float), cudaMemcpyHostToDevice, n->stream));
+		std::unique_ptr<float[]> p(new (std::nothrow) float[4 * w]());
+		if (!p) return fail(GL_ERR_INVALID, "gl_set_layer_norm: no host memory");
+		std::fill(p.get(), p.get() + w, 1.0f);
+		CU(cudaMemcpyAsync(t.param, p.get(), 4 * w * sizeof(float), cudaMemcpyHostToDevice, n->stream));
 		CU(cudaStreamSynchronize(n->stream));
 	}
 	t.on = eps >= 0.0f;
@@ -2044,7 +2048,8 @@ static int grid_fused_launch(gl_net* n, const float* X, const float* Y, int64_t 
 // The updates that no gradient's epilogue makes: gains and shifts of normalised layers, orthogonalised weight updates.
 static int special_updates(gl_net* n, int rows, int64_t* launches)
 {
-	std::vector<OrthoMatrix> m;
+	OrthoMatrix m[GL_MAX_WEIGHT_LAYERS];  // of the layers that have one
+	bool done[GL_MAX_WEIGHT_LAYERS] = {false};
 	for (int l = 0; l <= n->H; ++l)
 	{
 		if (n->norm[l].on)
@@ -2061,30 +2066,25 @@ static int special_updates(gl_net* n, int rows, int64_t* launches)
 		t.w = t.w_out = n->dW + n->woff[l];
 		t.ld_grad = t.ld_mom = t.ld_w = t.cols;
 		t.lr = n->d.lr[l] * sqrtf(std::max(1.0f, (float)t.rows / (float)t.cols));
-		m.push_back(t);
+		m[l] = t;
 	}
 	// layers of one setting in one call
-	std::vector<bool> done(m.size(), false);
-	for (int l = 0, i = 0; l <= n->H; ++l)
+	for (int l = 0; l <= n->H; ++l)
 	{
-		if (!n->muon[l].on) continue;
 		const gl_net::Muon& k = n->muon[l];
-		if (done[i++]) continue;
-		std::vector<OrthoMatrix> same;
-		for (int j = l, q = i - 1; j <= n->H; ++j)
+		if (!k.on || done[l]) continue;
+		OrthoMatrix same[GL_MAX_WEIGHT_LAYERS];
+		int count = 0;
+		for (int j = l; j <= n->H; ++j)
 		{
 			const gl_net::Muon& o = n->muon[j];
-			if (!o.on) continue;
-			if (!done[q] && o.momentum == k.momentum && o.decay == k.decay && o.nesterov == k.nesterov && o.steps == k.steps)
-			{
-				done[q] = true;
-				same.push_back(m[q]);
-			}
-			++q;
+			if (!o.on || done[j] || o.momentum != k.momentum || o.decay != k.decay || o.nesterov != k.nesterov || o.steps != k.steps) continue;
+			done[j] = true;
+			same[count++] = m[j];
 		}
 		OrthoArgs a = {};
-		a.mat = same.data();
-		a.count = (int)same.size();
+		a.mat = same;
+		a.count = count;
 		a.steps = k.steps;
 		a.type = GL_F32;
 		a.step = 1;

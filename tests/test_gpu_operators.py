@@ -550,6 +550,12 @@ def test_single_rows_beside_a_matrix_in_order_and_in_a_graph(g):
             assert torch.equal(a, b)
 
 
+def test_orthogonalize_lists_of_several_launches_of_all_kinds(g):
+    check_ortho(g, [(1, 50), (200, 150), (70, 1)] + [(20, 30 + i) for i in range(14)] + [(1, 90), (12, 12), (1, 1)])
+    check_ortho(g, [(1, 60 + i) for i in range(17)] + [(3, 9)])
+    check_ortho(g, [(1, 60 + i) for i in range(17)] + [(300, 140), (9, 1)], "bf16")
+
+
 def test_orthogonalize_long_and_moving_single_columns(g):
     """Those that the kernels of matrices take: beyond 131072 elements, and a column whose result has another pitch in its place."""
     check_ortho(g, [(1, 131073), (140000, 1)])
