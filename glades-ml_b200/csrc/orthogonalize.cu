@@ -51,10 +51,9 @@ constexpr int OR_SMS = 148;
 // Stages whose products an accumulator takes before it is drained.  The tensor core truncates as it adds, so a chain of n additions
 // drifts by up to n * 2^-24 towards zero; two stages are eight additions of full size, and what they still lose on average is taken
 // back (product_factor).  Errors of random matrices against 64 bits, with six stages and no factor -> with two and the factor (fp32
-// products): 256 x 1000 6.0e-6 -> 2.2e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 3.9e-6 (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  It costs
-// 0 to 15 % of the time (256 x 256 103 -> 105 us, 2048 x 2048 482 -> 510, 1024 x 8192 361 -> 425), which results of 16 bits, off by
-// 5e-4 or more anyway, need not pay.
-constexpr int OR_CHUNK = 2, OR_CHUNK_16 = 6;
+// products): 256 x 1000 6.0e-6 -> 2.2e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 3.9e-6 (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  Results of
+// 16 bits take the same products: theirs are the fp32 results, rounded.
+constexpr int OR_CHUNK = 2;
 constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 
 template <int BN>
@@ -1181,7 +1180,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.decay = a.decay;
 	P.eps = a.eps;
 	P.bad = a.bad;
-	P.chunk = !a.step && a.type != GL_F32 ? OR_CHUNK_16 : OR_CHUNK;
+	P.chunk = OR_CHUNK;
 	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
 	for (int i = 0; i < count; ++i)
 	{
