@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "layer_norm.cuh"
+#include "tc_gemm.h"
 
 namespace glb {
 namespace {
@@ -568,6 +569,9 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const La
 //   fp32 8192 x 4096: 72 us, 5.6 TB/s (one row ahead in registers 110);  bf16: 50 us, each further 8192 rows 31: as the copy of as
 //   many bytes.  What is above that is the start, the CTAs' sums and the columns' kernel.
 template <class T> __host__ __device__ constexpr int quads_stages() { return 208 * 1024 / (LN_GROUP_MAX * 2 * LN_ELEMS * (int)sizeof(T)); }
+template <class T> constexpr size_t quads_bytes(int threads) { return (size_t)threads * 2 * LN_ELEMS * sizeof(T) * quads_stages<T>(); }
+// the columns' sums of a CTA's groups, or of the warps that hold several: at most 16 rows of 512 columns, or as many values in fewer, longer rows
+constexpr size_t sums_bytes = (size_t)LN_GROUP_MAX * LN_ELEMS * sizeof(float2);
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(const LayerNormArgs p, int group)
 {
@@ -860,15 +864,19 @@ cudaError_t backward_mode(const LayerNormArgs& a, int* ctas, cudaStream_t s)
 	*ctas = grid;
 	const int parts = group > 32 ? threads / group : threads / 32;
 	size_t smem = parts > 1 ? (size_t)parts * a.n * sizeof(float2) : 0;
+	// The limit of a kernel's shared memory is the context's, not the call's, and can be lowered: it is set once, to the most that
+	// any shape needs, so that threads with other shapes at the same time take nothing away from one another.
+	constexpr size_t most = MODE == BY_QUADS ? quads_bytes<T>(LN_GROUP_MAX) : sums_bytes;
 	auto go = [&](void (*kernel)(LayerNormArgs, int)) {
-		if (smem > 47 * 1024)  // (48 KB without being asked for, the sums' slots among them)
-			if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+		int sms = 0;
+		if (smem > most) return cudaErrorInvalidValue;
+		if (cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(kernel), (int)most, &sms)) return e;
 		kernel<<<grid, threads, smem, s>>>(a, group);
 		return cudaGetLastError();
 	};
 	if constexpr (MODE == BY_QUADS)
 	{
-		smem = std::max(smem, (size_t)threads * 2 * LN_ELEMS * sizeof(T) * quads_stages<T>());
+		smem = std::max(smem, quads_bytes<T>(threads));
 		return group > 32 ? go(norm_backward_quads_kernel<T, true>) : go(norm_backward_quads_kernel<T, false>);
 	}
 	else return group > 32 ? go(norm_backward_kernel<T, MODE, true>) : go(norm_backward_kernel<T, MODE, false>);

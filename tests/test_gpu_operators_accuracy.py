@@ -1,9 +1,11 @@
 """What the operators' results are off by, and where they must be the same bits."""
+import threading
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_operators import DEV, TYPES, gradient, run_ortho  # noqa: E402
+from test_gpu_operators import DEV, TYPES, gen, gradient, norm_exact, run_ortho, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +21,43 @@ def test_orthogonalised_16_bit_matrices_are_the_fp32_results_rounded(g, t, shape
     run_ortho(g, [a.float() for a in ins], wide, "f32")
     for a, b in zip(outs, wide):
         assert torch.equal(a, b.to(TYPES[t]))
+
+
+def test_layer_norm_backward_from_several_threads_at_once(g):
+    """Two shapes that need different amounts of shared memory, each from two host threads with a stream each: no call fails, and every
+    one gives the bits that it gives alone."""
+    calls, errors = [], []
+    for i, (rows, n) in enumerate([(2000, 256), (8192, 256)] * 2):
+        r = gen(i)
+        x, dy = torch.randn(rows, n, generator=r, device=DEV), torch.randn(rows, n, generator=r, device=DEV)
+        _, em, er = norm_exact(x, None, None, 1e-5)
+        keep = (x, dy, em[:, 0].float(), er[:, 0].float(), torch.empty(rows, n, device=DEV), torch.empty(n, device=DEV), torch.empty(n, device=DEV),
+                torch.empty(g.layer_norm_backward_workspace(rows, n), dtype=torch.uint8, device=DEV))
+
+        def call(s, keep=keep, rows=rows, n=n):
+            x, dy, mean, rstd, dx, dg, ds, work = keep
+            g.layer_norm_backward(dy.data_ptr(), n, x.data_ptr(), n, None, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), n, dg.data_ptr(),
+                                  ds.data_ptr(), rows, n, work.data_ptr(), work.numel(), stream=s)
+        call(stream())
+        torch.cuda.synchronize()
+        calls.append((call, keep[4:7], [a.clone() for a in keep[4:7]], torch.cuda.Stream()))
+        for a in keep[4:7]:
+            a.zero_()
+    torch.cuda.synchronize()
+
+    def work(call, s):
+        try:
+            for _ in range(20000):
+                call(s.cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(c, s)) for c, _, _, s in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for _, got, want, _ in calls:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
