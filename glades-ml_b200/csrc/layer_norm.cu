@@ -570,8 +570,9 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const La
 //   many bytes.  What is above that is the start, the CTAs' sums and the columns' kernel.
 template <class T> __host__ __device__ constexpr int quads_stages() { return 208 * 1024 / (LN_GROUP_MAX * 2 * LN_ELEMS * (int)sizeof(T)); }
 template <class T> constexpr size_t quads_bytes(int threads) { return (size_t)threads * 2 * LN_ELEMS * sizeof(T) * quads_stages<T>(); }
-// the columns' sums of a CTA's groups, or of the warps that hold several: at most 16 rows of 512 columns, or as many values in fewer, longer rows
-constexpr size_t sums_bytes = (size_t)LN_GROUP_MAX * LN_ELEMS * sizeof(float2);
+// the columns' sums of a CTA's groups, or of the warps that hold several: at most 16 rows of 512 columns, or as many values in fewer, longer
+// rows; rows of words have a column more
+constexpr size_t sums_bytes = (size_t)(LN_GROUP_MAX * LN_ELEMS + LN_GROUP_MAX / 32) * sizeof(float2);
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(const LayerNormArgs p, int group)
 {

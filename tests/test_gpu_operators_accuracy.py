@@ -5,7 +5,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_operators import DEV, TYPES, gen, gradient, norm_exact, run_ortho, stream  # noqa: E402
+from test_gpu_operators import DEV, TYPES, check_back, gen, gradient, norm_exact, run_ortho, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,13 @@ def test_layer_norm_backward_from_several_threads_at_once(g):
     for _, got, want, _ in calls:
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [15, 16, 17, 257, 512, 513, 1025, 1537, 2049, 4097, 8191, 8192])
+def test_layer_norm_backward_of_full_blocks(g, t, n):
+    """As many groups per block as there can be, and rows of one value more than their lanes hold: the most shared memory that the
+    columns' sums take."""
+    rows = 148 * 2 * max(1, 512 // max(1, n // 16)) + 3
+    check_back(g, rows, n, t, n, n, n, 0, seed=n)
+    check_back(g, rows, n, t, n, n, n, 1, seed=n, plain=True)
