@@ -398,9 +398,11 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_long_kernel(const LayerNorm
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------
-// The same groups; both row sums in one exchange.  bf16 10007 x 1025: 35 us (one value at a time 164).  A lane keeps the same columns for all its rows and adds their dgain and
-// dshift up in registers; a CTA's groups are added in a fixed order and leave as one partial row, which norm_columns_kernel
-// adds up: no atomics, two runs give the same bits.  With d = x - mu, g = gain dy:  dx = r g - r sum(g) / n - d r^3 sum(g d) / n.
+// The same groups; both row sums in one exchange.  A lane keeps the same columns for all its rows and adds their dgain and dshift up in
+// registers; a CTA's groups are added in a fixed order and leave as one partial row, which norm_columns_kernel adds up: no atomics, two
+// runs give the same bits.  Every difference is scaled as it is taken, xh = (x - mu) r: sums of g (x - mu) and powers of r beside
+// them would leave fp32's range where activations are very large or very small.
+//   bf16 10007 x 1025: 35 us (one value at a time 164)
 // A CTA's sums of the columns: its groups' are added in a fixed order in `sums`, [groups or (in-warp groups) warps][n], and leave as
 // one partial row.  A lane's access v begins at column first + v * group * VEC.
 template <bool APART, bool WIDE, int V, int PAIRS>
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const La
 		const Place at(p.x, p.ldx, p.rows, p.n, row, gr);
 		const f32x2 minus = pair2(-mean_n, -mean_n), scale = pair2(rstd_n, rstd_n);
 		const float rstd = rstd_n;
-		f32x2 d[V][PAIRS], g[V][PAIRS];
+		f32x2 xh[V][PAIRS], g[V][PAIRS];
 		f32x2 a2 = zero, b2 = zero;
 #pragma unroll
 		for (int v = 0; v < V; ++v)
@@ -524,31 +526,31 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const La
 			{
 				// (what is not the row's has a dy of zero, and a difference that means nothing)
 				const f32x2 dy = dn[v].pair(i);
-				d[v][i] = at.mask(add2(xn[v].pair(i), minus), v * group * VEC);
+				xh[v][i] = mul2(at.mask(add2(xn[v].pair(i), minus), v * group * VEC), scale);
 				g[v][i] = mul2(dy, gain[v][i]);
 				a2 = add2(a2, g[v][i]);
-				b2 = fma2(g[v][i], d[v][i], b2);
-				dg[v][i] = fma2(mul2(dy, scale), d[v][i], dg[v][i]);
+				b2 = fma2(g[v][i], xh[v][i], b2);
+				dg[v][i] = fma2(dy, xh[v][i], dg[v][i]);
 				ds[v][i] = add2(ds[v][i], dy);
 			}
-		float a, b, c, e, de = 0.0f, ge = 0.0f;
+		float a, b, c, e, xhe = 0.0f, ge = 0.0f;
 		unpair2(a2, a, c);
 		unpair2(b2, b, e);
 		if (EDGE && at.edge >= 0)
 		{
 			const float dy = to_float(de_n);
-			de = to_float(xe_n) - mean_n;
+			xhe = (to_float(xe_n) - mean_n) * rstd;
 			ge = dy * gain_e;
 			a += ge;
-			b = fmaf(ge, de, b);
-			dg_e = fmaf(dy * rstd, de, dg_e);
+			b = fmaf(ge, xhe, b);
+			dg_e = fmaf(dy, xhe, dg_e);
 			ds_e += dy;
 		}
 		fetch(row + step);
 		if (!p.dx) continue;
 		const float2 s = gr.sum<WIDE>(a + c, b + e);
 		if (at.n == 0) continue;
-		const float ma = -s.x * inv_n * rstd, mb = -s.y * inv_n * rstd * rstd * rstd;
+		const float ma = -s.x * inv_n * rstd, mb = -s.y * inv_n * rstd;
 		const f32x2 ma2 = pair2(ma, ma), mb2 = pair2(mb, mb);
 		T* dx = static_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
@@ -556,10 +558,10 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_kernel(const La
 		{
 			f32x2 o[PAIRS];
 #pragma unroll
-			for (int i = 0; i < PAIRS; ++i) o[i] = fma2(g[v][i], scale, fma2(d[v][i], mb2, ma2));
+			for (int i = 0; i < PAIRS; ++i) o[i] = fma2(g[v][i], scale, fma2(xh[v][i], mb2, ma2));
 			at.store(dx, v * group * VEC, o);
 		}
-		if (EDGE && at.edge >= 0) dx[at.edge] = from_float<T>(fmaf(ge, rstd, fmaf(de, mb, ma)));
+		if (EDGE && at.edge >= 0) dx[at.edge] = from_float<T>(fmaf(ge, rstd, fmaf(xhe, mb, ma)));
 	}
 	if (p.part) leave_columns<MODE == BY_VALUES, WIDE>(p, gr, column.first, dg, ds, column.edge, make_float2(dg_e, ds_e), sums);
 }
@@ -638,10 +640,10 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(co
 #pragma unroll
 			for (int i = 0; i < PAIRS; ++i)
 			{
-				const f32x2 dy = dv.pair(i), d = add2(xv.pair(i), minus), g = mul2(dy, gain[v][i]);
+				const f32x2 dy = dv.pair(i), xh = mul2(add2(xv.pair(i), minus), scale), g = mul2(dy, gain[v][i]);
 				a2 = add2(a2, g);
-				b2 = fma2(g, d, b2);
-				dg[v][i] = fma2(mul2(dy, scale), d, dg[v][i]);
+				b2 = fma2(g, xh, b2);
+				dg[v][i] = fma2(dy, xh, dg[v][i]);
 				ds[v][i] = add2(ds[v][i], dy);
 			}
 		}
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(co
 			unpair2(a2, a, c);
 			unpair2(b2, b, e);
 			const float2 s = gr.sum<WIDE>(a + c, b + e);
-			const float ma = -s.x * inv_n * rstd, mb = -s.y * inv_n * rstd * rstd * rstd;
+			const float ma = -s.x * inv_n, mb = -s.y * inv_n * rstd;
 			const f32x2 ma2 = pair2(ma, ma), mb2 = pair2(mb, mb);
 			T* dx = static_cast<T*>(p.dx) + row * p.lddx + first_c;
 			if (row < p.rows)
@@ -664,7 +666,7 @@ __global__ void __launch_bounds__(LN_GROUP_MAX, 1) norm_backward_quads_kernel(co
 					dv.set(dys[v * (int)blockDim.x]);
 #pragma unroll
 					for (int i = 0; i < PAIRS; ++i)
-						o.set_pair(i, fma2(mul2(dv.pair(i), gain[v][i]), scale, fma2(add2(xv.pair(i), minus), mb2, ma2)));
+						o.set_pair(i, mul2(fma2(dv.pair(i), gain[v][i], fma2(add2(xv.pair(i), minus), mb2, ma2)), scale));
 					if (first_c + v * hop < p.n) o.store(dx + v * hop);
 				}
 			}

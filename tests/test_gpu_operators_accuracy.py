@@ -5,7 +5,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_operators import DEV, TYPES, check_back, gen, gradient, norm_exact, run_ortho, stream  # noqa: E402
+from test_gpu_operators import (DEV, HALF, TINY, TYPES, U, back_exact, chain, check_back, code, gen, gradient, norm_exact, run_ortho,  # noqa: E402
+                                stream)
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,32 @@ def test_layer_norm_backward_of_full_blocks(g, t, n):
     rows = 148 * 2 * max(1, 512 // max(1, n // 16)) + 3
     check_back(g, rows, n, t, n, n, n, 0, seed=n)
     check_back(g, rows, n, t, n, n, n, 1, seed=n, plain=True)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(70, 256), (70, 4096), (70, 1000), (33, 257), (41, 4097), (9, 8192), (9, 8193), (7, 20000)])
+@pytest.mark.parametrize("size", [1e18, 1e-18])
+def test_layer_norm_backward_of_very_large_and_very_small_activations(g, t, rows, n, size):
+    """No factor on the way leaves fp32's range, whichever kernel a row's length leads to: the gradient is as exact as for activations of 1."""
+    r = gen(n)
+    x = (size * torch.randn(rows, n, generator=r, device=DEV)).to(TYPES[t])
+    dy = (1e-4 * torch.randn(rows, n, generator=r, device=DEV)).to(TYPES[t])
+    gain = 1.0 + 0.3 * torch.randn(n, generator=r, device=DEV)
+    _, em, er = norm_exact(x, None, None, 0.0)
+    mean, rstd = em[:, 0].float(), er[:, 0].float()
+    dx, dgain, dshift = torch.empty(rows, n, device=DEV, dtype=TYPES[t]), torch.empty(n, device=DEV), torch.empty(n, device=DEV)
+    bytes_ = g.layer_norm_backward_workspace(rows, n)
+    work = torch.empty(bytes_, dtype=torch.uint8, device=DEV)
+    g.layer_norm_backward(dy.data_ptr(), n, x.data_ptr(), n, gain.data_ptr(), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), n,
+                          dgain.data_ptr(), dshift.data_ptr(), rows, n, work.data_ptr(), bytes_, dtype=code(g, t), stream=stream())
+    ex, eg, _ = back_exact(dy, x, gain, mean, rstd)
+    # a sum of n terms: at most chain(n) additions; every other factor one rounding
+    rd = rstd.double()[:, None]
+    xh = ((x.double() - mean.double()[:, None]) * rd).abs()
+    v = (dy.double() * gain.double()).abs()
+    a, b = v.mean(1, keepdim=True), (v * xh).mean(1, keepdim=True)
+    tol = 1.01 * rd * U * ((chain(n) + 4) * (a + xh * b) + 2 * xh * b + 6 * (v + a + xh * b))
+    tol = tol + HALF[t] * (ex.abs() + tol) + TINY[t]
+    assert bool(((dx.double() - ex).abs() <= tol).all()), float(((dx.double() - ex).abs() / tol).max())
+    tol = 1.01 * U * ((rows + 23) * (dy.double().abs() * xh).sum(0)) + TINY["f32"]
+    assert bool(((dgain.double() - eg).abs() <= tol).all())
