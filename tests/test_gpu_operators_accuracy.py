@@ -5,8 +5,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_operators import (DEV, HALF, TINY, TYPES, U, back_exact, chain, check_back, code, gen, gradient, norm_exact, run_ortho,  # noqa: E402
-                                stream)
+from test_gpu_operators import (DEV, HALF, TINY, TYPES, U, back_exact, chain, check_back, code, coefs, gen, gradient, iterate,  # noqa: E402
+                                norm_exact, ortho_tolerance, run_ortho, stream)
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,21 @@ def test_layer_norm_backward_of_very_large_and_very_small_activations(g, t, rows
     assert bool(((dx.double() - ex).abs() <= tol).all()), float(((dx.double() - ex).abs() / tol).max())
     tol = 1.01 * U * ((rows + 23) * (dy.double().abs() * xh).sum(0)) + TINY["f32"]
     assert bool(((dgain.double() - eg).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_orthogonalize_matrices_whose_norm_is_beyond_fp32(g, t):
+    """Finite elements of up to 3e38: the norm is taken and used in 64 bits."""
+    for list_ in ([(1, 9), (600, 1)], [(2, 2), (16, 40), (100, 30), (1, 7)], [(200, 260), (1, 80), (90, 1)]):
+        ins = [((2 * torch.rand(m, n, generator=gen(m + n), device=DEV) - 1) * 3e38).to(TYPES[t]) for m, n in list_]
+        ins[0].fill_(3e38)
+        ins[0][0, 0] = -2e38
+        outs = [torch.empty_like(a) for a in ins]
+        assert sum(float(a.double().norm()) > 3.5e38 for a in ins) >= 2  # (a short row's need not be)
+        run_ortho(g, ins, outs, t)
+        for a, b in zip(ins, outs):
+            u = a.double() * 2.0 ** -100  # (the same matrix to the operator: eps is 1e-16 of its norm)
+            exact = iterate(u, 5, coefs(5), 1e-7, torch.float64)
+            tol = ortho_tolerance(u.float(), 5, coefs(5), 1e-7, exact)
+            tol = tol + HALF[t] * (exact.abs() + tol)
+            assert bool(((b.double() - exact).abs() <= tol).all()), tuple(a.shape)
