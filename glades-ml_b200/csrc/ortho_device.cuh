@@ -42,6 +42,14 @@ struct OrProgram
 	unsigned char first[OR_MAX_ROUNDS + 1];  // operations first[r] .. first[r + 1] - 1 are round r's
 };
 
+// What X_0 is U times, from the sum of U's squares: in 64 bits throughout, since finite elements may have a norm beyond fp32's range.
+// A zero matrix without an eps stays zero.
+__device__ __forceinline__ double inverse_norm(double sum, float eps)
+{
+	const double norm = sqrt(sum) + (double)eps;
+	return norm == 0.0 ? 0.0 : 1.0 / norm;
+}
+
 // ---- elements of the caller's matrices, four neighbours at a time ------------------------------------------------
 __device__ __forceinline__ float load_typed(const void* p, long long i, int type)
 {

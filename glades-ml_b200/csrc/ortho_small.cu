@@ -78,7 +78,7 @@ __device__ __noinline__ void orthogonalize_vector(const SmParams& P, const SmMat
 	__syncthreads();
 	sum = 0.0;
 	for (int w = 0; w < SM_THREADS / 32; ++w) sum += warp_sums[w];
-	const double inv = 1.0 / (sqrt(sum) + (double)P.eps);
+	const double inv = inverse_norm(sum, P.eps);
 	double a = sum * inv * inv, factor = inv;
 	for (int k = 0; k < P.steps; ++k)
 	{
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 	const uint32_t tmem_base = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 	sum = 0.0;
 	for (int w = 0; w <= SM_WARPS; ++w) sum += warp_sums[w];
-	const double inv = 1.0 / (sqrt(sum) + (double)P.eps);
+	const double inv = inverse_norm(sum, P.eps);
 
 	// ---- X_0: scaled, split, the short side as rows (every thread visits the elements that it has visited before)
 	for (unsigned e0 = threadIdx.x; e0 < total; e0 += 4 * SM_THREADS)

@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			if (lane == 0) warp_sums[0] = t;
 		}
 		__syncthreads();
-		const double inv = 1.0 / (sqrt(warp_sums[0]) + (double)P.eps);  // (finite elements may have a norm beyond fp32's range)
+		const double inv = inverse_norm(warp_sums[0], P.eps);
 		const float s = P.s0;
 		__syncthreads();
 		for (int u = first; u < units; u += gridDim.x)

@@ -119,3 +119,18 @@ def test_orthogonalize_matrices_whose_norm_is_beyond_fp32(g, t):
             tol = ortho_tolerance(u.float(), 5, coefs(5), 1e-7, exact)
             tol = tol + HALF[t] * (exact.abs() + tol)
             assert bool(((b.double() - exact).abs() <= tol).all()), tuple(a.shape)
+
+
+@pytest.mark.parametrize("shapes", [[(1, 9), (70, 1)], [(16, 40), (100, 30), (1, 7)], [(200, 260), (1, 80)]])
+def test_zero_matrices_give_zeros_without_eps_too(g, shapes):
+    ins = [torch.zeros(m, n, device=DEV) for m, n in shapes]
+    outs = [torch.full((m, n), 7.0, device=DEV) for m, n in shapes]
+    run_ortho(g, ins, outs, "f32", eps=0.0)
+    for a in outs:
+        assert not a.any() and not torch.isnan(a).any()
+    # and a gradient without eps is what it is with a negligible one
+    ins = [gradient(m, n, 5) for m, n in shapes]
+    run_ortho(g, ins, outs, "f32", eps=0.0)
+    for a, b in zip(ins, outs):
+        exact = iterate(a.double(), 5, coefs(5), 0.0, torch.float64)
+        assert bool(((b.double() - exact).abs() <= ortho_tolerance(a, 5, coefs(5), 0.0, exact)).all())
