@@ -24,17 +24,6 @@ struct OrOp
 	signed char round;
 	float f, w1, w2, so;
 };
-// The factor of an operation's products.  Tensor cores cut off what a sum cannot hold, so that sums of products come out too small.
-// Measured with accumulators of eight additions: X X^T by 4.2e-7 (from 128 columns on); products of p x p matrices, whose
-// diagonals hold most of them, by up to 2.1e-7; the diagonal of A A, whose other products are all positive, by 3.5e-7 more.  The polynomial
-// multiplies such an error of all singular values by up to 15, so it is taken back here (64 x 512: 3.0e-6 -> 1.8e-6; fp32 products 1.6e-6).
-inline float product_factor(const OrOp& o, int p, int q, int additions)
-{
-	const bool of_x = o.a >= ID_X;
-	const double cut = of_x ? 4.2e-7 * std::min(1.0, q / 128.0) : 2.1e-7 * std::min(1.0, p / 192.0);
-	const double square = o.a == ID_A && o.b == ID_A ? 3.5e-7 * std::min(1.0, p / 96.0) : 0.0;
-	return (float)(o.f * (1.0 + cut * std::max(1.0, std::min(additions, (of_x ? q : p) / 16) / 8.0) + square));
-}
 struct OrProgram
 {
 	OrOp op[OR_MAX_OPS];

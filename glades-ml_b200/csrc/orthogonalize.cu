@@ -48,12 +48,11 @@ constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_PROGRAMS = 3;
 constexpr int OR_SMS = 148;
-// Stages whose products an accumulator takes before it is drained.  The tensor core truncates as it adds, so a chain of n additions
-// drifts by up to n * 2^-24 towards zero; two stages are eight additions of full size, and what they still lose on average is taken
-// back (product_factor).  Errors of random matrices against 64 bits, with six stages and no factor -> with two and the factor (fp32
-// products): 256 x 1000 6.0e-6 -> 2.2e-6 (2.6e-6), 1000 x 8192 1.1e-5 -> 3.9e-6 (3.9e-6), 10 x 500 1.8e-6 -> 0.6e-6 (0.6e-6).  Results of
-// 16 bits take the same products: theirs are the fp32 results, rounded.
-constexpr int OR_CHUNK = 2;
+// An accumulator takes one stage, four additions, before it is drained.  The tensor core truncates as it adds: a sum of one sign loses
+// half a unit in the last place with every addition, and the polynomial multiplies an error that all singular values share by up to 15.
+// Against 64 bits, relative to the error of fp32 products, with 8 additions -> 4: random 512 x 4096 2.2 -> 1.3, 256 x 256 with near singular
+// values 1.5 -> 1.0.  (What is lost cannot be put back by a factor: sums that cancel, or of few products, lose less.  A factor
+// that made up for it on random matrices left diagonal and block diagonal ones 4 times further off than fp32 products.)
 constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 
 template <int BN>
@@ -95,11 +94,9 @@ struct OrParams
 	OrMat mat[ORTHO_MAX_MATRICES];
 	OrProgram prog[OR_PROGRAMS];  // step by step; in groups of two; with three steps in the first
 	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
-	float factor[ORTHO_MAX_MATRICES][OR_MAX_OPS];  // product_factor
 	unsigned long long reduce;  // rounds with split tiles
 	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
 	int count, rounds, units;
-	int chunk;  // stages whose products an accumulator takes before it is drained
 	int type, step, nesterov, reset;
 	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
@@ -728,39 +725,29 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				const uint32_t a_low = (uint32_t)desc_a, a_high = (uint32_t)(desc_a >> 32), b_low = (uint32_t)desc_b, b_high = (uint32_t)(desc_b >> 32);
 				const uint32_t a_step = 32u >> 4, b_step = b_mn ? 2048u >> 4 : 32u >> 4;
 				constexpr uint32_t A_LO = S::A_BYTES >> 4;
-				int in = 0;
 				for (int left = t.kb1 - t.kb0; left > 0; --left)
 				{
-					if (in == 0)
-					{
-						if (!warp_wait(bar_acc_empty + 8 * buf, aph ^ 1u, abort_flag, P.status, 4)) { ok = false; break; }
-					}
+					if (!warp_wait(bar_acc_empty + 8 * buf, aph ^ 1u, abort_flag, P.status, 4)) { ok = false; break; }
 					const uint32_t full = bar0 + 8 * s;
 					if (!warp_wait(full, ph, abort_flag, P.status, 2)) { ok = false; break; }
 					asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 					const uint32_t off = (uint32_t)s * (S::STAGE_BYTES >> 4);
 					const uint32_t a0 = a_low + off, b0 = b_low + off;
 					const uint32_t d = tmem_base + (uint32_t)(buf * S::COLUMNS);
-					const bool ends = in + 1 == P.chunk || left == 1;
 					if (leader)
 					{
 #pragma unroll
 						for (int k = 0; k < OR_BK / 16; ++k)
 						{
-							mma(k == 0 && in == 0, d, a0 + k * a_step, a_high, b0 + k * b_step, b_high, idesc2);
+							mma(k == 0, d, a0 + k * a_step, a_high, b0 + k * b_step, b_high, idesc2);
 							mma(false, d + BN, a0 + A_LO + k * a_step, a_high, b0 + k * b_step, b_high, idesc);
 						}
 						umma_commit(full + 8 * STAGES);
-						if (ends) umma_commit(bar_acc_full + 8 * buf);
+						umma_commit(bar_acc_full + 8 * buf);
 					}
 					__syncwarp();
-					++in;
-					if (ends)
-					{
-						in = 0;
-						buf ^= 1;
-						aph ^= (uint32_t)(buf == 0);
-					}
+					buf ^= 1;
+					aph ^= (uint32_t)(buf == 0);
 					if (++s == STAGES)
 					{
 						s = 0;
@@ -780,7 +767,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				const OrMat& M = P.mat[t.mat];
 				const OrOp& o = P.prog[M.program].op[t.op];
 				const OrTarget target(M, o);
-				const float f = P.factor[t.mat][t.op];
+				const float f = o.f;
 				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
 				float acc[EC];
 #pragma unroll
@@ -795,7 +782,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 							add_parts(acc + pc * 32, o.w2, o.e2, M, r0 + lane, c00 + pc * 32);
 						}
 				}
-				for (int done = t.kb0; done < t.kb1; done += P.chunk)
+				for (int left = t.kb1 - t.kb0; left > 0; --left)
 				{
 					if (!warp_wait(bar_acc_full + 8 * buf, aph, abort_flag, P.status, 3))
 					{
@@ -1180,7 +1167,6 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.decay = a.decay;
 	P.eps = a.eps;
 	P.bad = a.bad;
-	P.chunk = OR_CHUNK;
 	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
 	for (int i = 0; i < count; ++i)
 	{
@@ -1207,7 +1193,6 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
 		P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
 		bytes += matrix_bytes(M, g.planes);
-		for (int k = 0; k < g.count; ++k) P.factor[i][k] = product_factor(g.op[k], M.p, M.q, P.chunk * OR_BK / 16);
 	}
 	long long best = -1;
 	for (int bn : {128, 64})

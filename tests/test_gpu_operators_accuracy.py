@@ -134,3 +134,83 @@ def test_zero_matrices_give_zeros_without_eps_too(g, shapes):
     for a, b in zip(ins, outs):
         exact = iterate(a.double(), 5, coefs(5), 0.0, torch.float64)
         assert bool(((b.double() - exact).abs() <= ortho_tolerance(a, 5, coefs(5), 0.0, exact)).all())
+
+
+# ---- the orthogonalisation's error beside that of fp32 products ---------------------------------------------------------
+def fp32(coef):
+    """Coefficients as the entry point holds them."""
+    return [tuple(float(torch.tensor(v, dtype=torch.float32)) for v in c) for c in coef]
+
+
+def structured(p, q, seed):
+    """p x q matrices, p <= q, whose products differ in kind: sums of many terms of one sign or of both, of few terms, of one."""
+    r = gen(seed)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=r, device=DEV)
+    eye = torch.zeros(p, q, device=DEV)
+    eye[torch.arange(p), torch.arange(p)] = 1.0
+    blocks = torch.zeros(p, q, device=DEV)
+    for i in range(8):
+        a, b = p * i // 8, p * (i + 1) // 8
+        blocks[a:b, q * i // 8:q * (i + 1) // 8] = randn(b - a, q * (i + 1) // 8 - q * i // 8)
+    signs = torch.ones(q, device=DEV)
+    signs[1::2] = -1.0
+    opposite = randn(p, q)
+    opposite[1::2] = -opposite[0::2][:p // 2]
+    u, v = torch.linalg.qr(randn(p, p).double())[0], torch.linalg.qr(randn(q, p).double())[0]
+    return {
+        "noise": randn(p, q),
+        "near singular values": ((u * torch.linspace(0.5, 1, p, device=DEV, dtype=torch.float64)) @ v.t()).float(),
+        "wide spectrum": ((u * torch.logspace(0, -4, p, device=DEV, dtype=torch.float64)) @ v.t()).float(),
+        "orthogonal rows": v.t().float().contiguous(),
+        "diagonal": eye * torch.exp(randn(p, 1)),
+        "blocks": blocks,
+        "blocks of different size": blocks * torch.logspace(0, -3, p, device=DEV)[:, None],
+        "one strong direction": randn(p, 1) @ randn(1, q) + 1e-3 * randn(p, q),
+        "positive": torch.rand(p, q, generator=r, device=DEV),
+        "columns of alternating sign": randn(p, q).abs() * signs,
+        "rows that cancel": opposite + 1e-3 * randn(p, q),
+        "gradient": gradient(p, q, seed),
+        # products that fp32 holds without a rounding
+        "exact: identity": eye,
+        "exact: permutation": eye[:, torch.randperm(q, generator=r, device=DEV)].contiguous(),
+        "exact: ones": torch.ones(p, q, device=DEV),
+        "exact: ones of alternating sign": torch.ones(p, 1, device=DEV) * signs,
+    }
+
+
+def check_structured(g, p, q, tall=False, steps=5, coefficients=None):
+    """The result's error against 64 bits, root mean square over seeds, relative to the result: at most 2.5 times that of fp32
+    products.  (An accumulator that cuts four additions off loses (1 + 2 + 3 + 4) / 4 half units in the last place of a sum of one sign on
+    average, where a rounded sum is off by up to one.)  Matrices whose products fp32 holds without a rounding may be off by what
+    the parts' roundings make of one step: the terms |a| + |b| + |c| = 10.25 of a result of 0.7 or more, each with four half units."""
+    coef = fp32(coefficients or coefs(steps))
+    error, plain = {}, {}
+    seeds = 4
+    for seed in range(seeds):
+        for kind, u in structured(p, q, seed).items():
+            if tall:
+                u = u.t().contiguous()
+            out = torch.empty_like(u)
+            run_ortho(g, [u], [out], "f32", steps, coefficients)
+            exact = iterate(u.double(), steps, coef, 1e-7, torch.float64)
+            for sums, got in ((error, out), (plain, iterate(u, steps, coef, 1e-7, torch.float32))):
+                sums[kind] = sums.get(kind, 0.0) + float((got.double() - exact).norm() / exact.norm()) ** 2 / seeds
+    off = {}
+    for kind in error:
+        e, f = error[kind] ** 0.5, plain[kind] ** 0.5
+        limit = 2.5 * f + (4 * U * 10.25 / 0.7 if kind.startswith("exact") else 0.0)
+        if e > limit:
+            off[kind] = (e, f)
+    assert not off, off
+
+
+@pytest.mark.parametrize("p,q", [(16, 64), (33, 90), (64, 128), (128, 128), (10, 500), (64, 512), (96, 200), (112, 300)])
+def test_errors_of_small_matrices(g, p, q):
+    check_structured(g, p, q)
+
+
+@pytest.mark.parametrize("p,q", [(192, 192), (256, 256), (256, 1000), (500, 1000), (1000, 784), (1024, 1024), (20, 2048)])
+def test_errors_of_matrices(g, p, q):
+    check_structured(g, min(p, q), max(p, q), tall=p > q)
