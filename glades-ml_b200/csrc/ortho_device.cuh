@@ -11,24 +11,21 @@
 namespace glb {
 using namespace tc;
 
-constexpr int OR_MAX_OPS = 4 * ORTHO_MAX_STEPS;
-constexpr int OR_MAX_ROUNDS = 64;  // at most 55 are needed: step by step three per step, in groups of n 3 n + 1
-constexpr int OR_PLANES = 6;       // p x p matrices of a grouped program
+// Three products a step, one behind the other: A = X X^T, R = b A + c A A, X <- a X + R X.
+constexpr int OR_MAX_OPS = 3 * ORTHO_MAX_STEPS;
 
-// Matrices of parts that an operation names: 0 .. 5 p x p, 6 and 7 the two X.
-enum { ID_A = 0, ID_X = 6, ID_NONE = -1 };
-// out = f (A B^T or A B + w1 E1 + w2 E2); the factors hold the parts' scales
+// Matrices of parts that an operation names: two p x p, and the two X.
+enum { ID_A = 0, ID_R = 1, ID_X = 2, ID_NONE = -1 };
+// out = f (A B^T or A B) + w E; the factors hold the parts' scales
 struct OrOp
 {
-	signed char a, b, e1, e2, out;  // out ID_NONE: the result
-	signed char round;
-	float f, w1, w2, so;
+	signed char a, b, e, out;  // out ID_NONE: the result
+	float f, w, so;
 };
 struct OrProgram
 {
 	OrOp op[OR_MAX_OPS];
-	int count, rounds, planes;
-	unsigned char first[OR_MAX_ROUNDS + 1];  // operations first[r] .. first[r + 1] - 1 are round r's
+	int count;
 };
 
 // What X_0 is U times, from the sum of U's squares: in 64 bits throughout, since finite elements may have a norm beyond fp32's range.

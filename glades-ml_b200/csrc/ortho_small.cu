@@ -1,5 +1,5 @@
 // Orthogonalisation of small matrices: one CTA per matrix, everything in its shared memory (the mathematics: orthogonalize.cu).
-// The step-by-step program on the same tensor-core operands, but no copies, no grid barriers and no symmetry: what bounds
+// The same program on the same tensor-core operands, but no copies, no grid barriers and no symmetry: what bounds
 // a round here is the chain MMAs -> commit -> tensor-memory loads -> parts into shared memory -> block barrier, about a
 // microsecond against six of the cooperative kernel (its barrier alone takes one).
 //
@@ -403,8 +403,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) ortho_small_kernel(const __grid
 								v[2 * i + 1] = fmaf(w, a2.y + b2.y, v[2 * i + 1]);
 							}
 						};
-						add(o.e1, o.w1);
-						add(o.e2, o.w2);
+						add(o.e, o.w);
 						if (o.out != ID_NONE)
 						{
 							uint4 h4, l4;

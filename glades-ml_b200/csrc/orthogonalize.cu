@@ -3,13 +3,10 @@
 // drives the singular values of U towards 1 and keeps its singular vectors.  X is held with its short side p as rows (a tall
 // matrix is transposed on the way in and on the way out), so that A and R are p x p.
 //
-// Several steps on the short side alone ("a group"): P = a + R is a polynomial of A and commutes with it, so the next step's
-// A is P A P, and the group's X is (P_n .. P_1) X.  A group of n steps costs one product with X on both sides (A) and one with X
-// on one side instead of n of each, and 2 (n - 1) + (n - 1) more products of p x p matrices:
-//     T = a A + R A,   A' = a T + T R,   Q' = P Q  as  q' + Qr' = a q + (a Qr + q R + R Qr)
-// 15 p^2 q + 5 p^3 multiply-adds become 6 p^2 q + 14 p^3 for five steps in groups of three and two (symmetric products by half).
-// A's rounding is absolute, so small singular values lose digits with every further step of a group: two steps, and
-// three from the start of a large matrix, whose A has small elements, stay within the error of fp32 products; see groups_allowed.
+// Multiply-adds of a step: p^2 q / 2 (A) + p^3 / 2 (A A), which are symmetric, and p^2 q.
+// (Several steps on the short side alone -- P = a + R commutes with A, so that the next step's A is P A P and X needs one product for
+// all of them -- take half of the multiply-adds of a flat matrix.  But the rounding of A is absolute, and small singular values lose
+// digits with every further step: 512 x 4096 came out up to 5 times further off than with fp32 products.)
 //
 // Bound: tensor cores.  Every product is fp32-faithful on three fp16 products (hi*hi + hi*lo + lo*hi), as the layer products of
 // gemm_tcgen05.cu; unlike there the scales are known beforehand -- all singular values stay below a bound that follows from
@@ -19,13 +16,13 @@
 // twice the columns, [hi*hi | hi*lo], an accumulator for each half: two MMAs per 16 k instead of three, fewer reads of shared memory.
 // (Tiles of 256 columns, which only fit with one accumulator for all three products, lost: their epilogue holds 128 sums per
 // thread, spills, and the MMAs wait for it.  4096 x 4096, a step: 769 us against 655.)
-// a X (b A, a T, ..) is where the epilogue's registers start from, loaded while the first chunk is computed: inside the accumulator
+// a X (or b A) is where the epilogue's registers start from, loaded while the first chunk is computed: inside the accumulator
 // it would be truncated with every addition, which doubles the error of the result.  The products are multiplied by their own
 // coefficient as they are added, so that every coefficient is used as it is given.
-// A, R, T and Q are symmetric: tiles above the diagonal are left out, an element below it is stored at both places.
+// A and R are symmetric: tiles above the diagonal are left out, an element below it is stored at both places.
 //
-// One cooperative launch walks all steps of all matrices: norm, scaling, then rounds of products that do not depend on one
-// another, a grid barrier after each.  Within a round every CTA takes the items cta, cta + grid, ... of all matrices.  Where a
+// One cooperative launch walks all steps of all matrices: norm, scaling, then a round for each product of the program, of all
+// matrices at once, a grid barrier after each.  Within a round every CTA takes the items cta, cta + grid, ... of all matrices.  Where a
 // round has too few tiles for the SMs, its tiles are split along k: the parts go to scratch in fp32, and after one more
 // barrier all warps of the GPU add them up, 32 x 32 elements at a time, in a fixed order.
 #include <cooperative_groups.h>
@@ -46,8 +43,8 @@ namespace {
 // stages of 32 k that bounded both tiles (530 clocks per 32 k on 128 columns, 350 to 400 now).
 constexpr int OR_BK = 64;
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
-constexpr int OR_PROGRAMS = 3;
 constexpr int OR_SMS = 148;
+constexpr int OR_SQUARES = 2;  // p x p matrices of parts: A and R
 // An accumulator takes one stage, four additions, before it is drained.  The tensor core truncates as it adds: a sum of one sign loses
 // half a unit in the last place with every addition, and the polynomial multiplies an error that all singular values share by up to 15.
 // Against 64 bits, relative to the error of fp32 products, with 8 additions -> 4: random 512 x 4096 2.2 -> 1.3, 256 x 256 with near singular
@@ -76,7 +73,7 @@ struct OrSmem
 struct OrMat
 {
 	OrthoMatrix m;
-	int p, q, tall, program;
+	int p, q, tall;
 	long long ldx, planex;  // halfs: row pitch and size of one part of X; parts in the order X0 hi, X0 lo, X1 hi, X1 lo
 	long long lds, planes;  // the same of the p x p matrices
 	__half* X;
@@ -92,11 +89,11 @@ struct OrParams
 {
 	OrMaps maps[ORTHO_MAX_MATRICES];
 	OrMat mat[ORTHO_MAX_MATRICES];
-	OrProgram prog[OR_PROGRAMS];  // step by step; in groups of two; with three steps in the first
+	OrProgram prog;  // operation k is round k's, of every matrix
 	unsigned char split[ORTHO_MAX_MATRICES][OR_MAX_OPS];
 	unsigned long long reduce;  // rounds with split tiles
-	int items[OR_MAX_ROUNDS], splits[OR_MAX_ROUNDS];  // a round's items, and its split tiles
-	int count, rounds, units;
+	int items[OR_MAX_OPS], splits[OR_MAX_OPS];  // a round's items, and its split tiles
+	int count, units;
 	int type, step, nesterov, reset;
 	float mu, decay, eps, s0;  // s0: X_0's scale
 	int* status;
@@ -127,7 +124,7 @@ __host__ __device__ inline int op_tiles(const OrOp& o, int p, int q, int bn)
 
 struct OrItem
 {
-	int mat, op, m0, n0, kb0, kb1, split, slot;  // slot: of a split tile's first part
+	int mat, m0, n0, kb0, kb1, split, slot;  // slot: of a split tile's first part
 };
 // the tile t of operation o
 template <int BN>
@@ -157,59 +154,51 @@ __device__ __forceinline__ void tile_origin(const OrOp& o, int p, int q, int t, 
 template <int BN>
 __device__ __forceinline__ void find_item(const OrParams& P, int round, int t, OrItem& it)
 {
+	const OrOp& o = P.prog.op[round];
 	int slot = 0;
 	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.program];
-		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
+		const int s = P.split[i][round];
+		const int n = op_tiles(o, M.p, M.q, BN) * s;
+		if (t < n)
 		{
-			const int s = P.split[i][k];
-			const int n = op_tiles(g.op[k], M.p, M.q, BN) * s;
-			if (t < n)
-			{
-				const int tile = t / s, part = t - tile * s;
-				const int kb = op_kb(g.op[k], M.p, M.q);
-				it.mat = i;
-				it.op = k;
-				it.split = s;
-				it.kb0 = kb * part / s;
-				it.kb1 = kb * (part + 1) / s;
-				it.slot = slot + t;
-				tile_origin<BN>(g.op[k], M.p, M.q, tile, it.m0, it.n0);
-				return;
-			}
-			t -= n;
-			if (s > 1) slot += n;
+			const int tile = t / s, part = t - tile * s;
+			const int kb = op_kb(o, M.p, M.q);
+			it.mat = i;
+			it.split = s;
+			it.kb0 = kb * part / s;
+			it.kb1 = kb * (part + 1) / s;
+			it.slot = slot + t;
+			tile_origin<BN>(o, M.p, M.q, tile, it.m0, it.n0);
+			return;
 		}
+		t -= n;
+		if (s > 1) slot += n;
 	}
 }
-// tile t < P.splits[round] of a round's split operations
+// tile t < P.splits[round] of a round's split matrices
 template <int BN>
 __device__ __forceinline__ void find_split(const OrParams& P, int round, int t, OrItem& it)
 {
+	const OrOp& o = P.prog.op[round];
 	int slot = 0;
 	for (int i = 0;; ++i)
 	{
 		const OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.program];
-		for (int k = g.first[round]; k < g.first[round + 1]; ++k)
+		const int s = P.split[i][round];
+		if (s < 2) continue;
+		const int n = op_tiles(o, M.p, M.q, BN);
+		if (t < n)
 		{
-			const int s = P.split[i][k];
-			if (s < 2) continue;
-			const int n = op_tiles(g.op[k], M.p, M.q, BN);
-			if (t < n)
-			{
-				it.mat = i;
-				it.op = k;
-				it.split = s;
-				it.slot = slot + t * s;
-				tile_origin<BN>(g.op[k], M.p, M.q, t, it.m0, it.n0);
-				return;
-			}
-			t -= n;
-			slot += n * s;
+			it.mat = i;
+			it.split = s;
+			it.slot = slot + t * s;
+			tile_origin<BN>(o, M.p, M.q, t, it.m0, it.n0);
+			return;
 		}
+		t -= n;
+		slot += n * s;
 	}
 }
 
@@ -662,9 +651,10 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	bool ok = true;
 	OrItem t;              // copying and multiplying warps: a round's first item is looked up in front of the barrier before it
 	if (warp < 2 && (int)blockIdx.x < P.items[0]) find_item<BN>(P, 0, blockIdx.x, t);
-	for (int round = 0; met && round < P.rounds; ++round)
+	for (int round = 0; met && round < P.prog.count; ++round)
 	{
 		const int items = P.items[round];
+		const OrOp& o = P.prog.op[round];
 		if (warp == 0)
 		{
 			// ------------------------------------------------ TMA producer
@@ -676,7 +666,6 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			{
 				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
 				const OrMaps& mp = P.maps[t.mat];
-				const OrOp& o = P.prog[P.mat[t.mat].program].op[t.op];
 				const bool ax = o.a >= ID_X, bx = o.b >= ID_X;
 				const CUtensorMap* ma = ax ? &mp.xa : &mp.sa;
 				const CUtensorMap* mb = ax ? &mp.xb : &mp.sb;
@@ -715,7 +704,6 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
 				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
-				const OrOp& o = P.prog[P.mat[t.mat].program].op[t.op];
 				const uint32_t b_mn = o.b >= ID_X && o.a < ID_X ? 1u : 0u;
 				const uint32_t idesc = (1u << 4) | (b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 				const uint32_t idesc2 = (1u << 4) | (b_mn << 16) | ((uint32_t)(S::COLUMNS >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
@@ -765,7 +753,6 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			{
 				find_item<BN>(P, round, ti, t);
 				const OrMat& M = P.mat[t.mat];
-				const OrOp& o = P.prog[M.program].op[t.op];
 				const OrTarget target(M, o);
 				const float f = o.f;
 				const int r0 = t.m0 + quarter * 32, c00 = t.n0 + half * EC;
@@ -776,11 +763,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				{
 #pragma unroll
 					for (int pc = 0; pc < EC / 32; ++pc)
-						if (target.needs(r0, c00 + pc * 32))
-						{
-							add_parts(acc + pc * 32, o.w1, o.e1, M, r0 + lane, c00 + pc * 32);
-							add_parts(acc + pc * 32, o.w2, o.e2, M, r0 + lane, c00 + pc * 32);
-						}
+						if (target.needs(r0, c00 + pc * 32)) add_parts(acc + pc * 32, o.w, o.e, M, r0 + lane, c00 + pc * 32);
 				}
 				for (int left = t.kb1 - t.kb0; left > 0; --left)
 				{
@@ -840,7 +823,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				for (int k = (warp - S::FIRST) * (int)gridDim.x + (int)blockIdx.x; k < P.splits[round] * S::PIECES; k += warps)
 				{
 					find_split<BN>(P, round, k / S::PIECES, t);
-					const OrTarget target(P.mat[t.mat], P.prog[P.mat[t.mat].program].op[t.op]);
+					const OrTarget target(P.mat[t.mat], o);
 					const int pc = k % S::PIECES;
 					const int r0 = t.m0 + pc / (BN / 32) * 32, c0 = t.n0 + pc % (BN / 32) * 32;
 					if (!target.needs(r0, c0)) continue;
@@ -867,7 +850,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				}
 			}
 		}
-		if (round + 1 < P.rounds)
+		if (round + 1 < P.prog.count)
 		{
 			if (warp < 2 && (int)blockIdx.x < P.items[round + 1]) find_item<BN>(P, round + 1, blockIdx.x, t);
 			if (!meet(P.arrived, meeting += gridDim.x, abort_flag, P.status)) break;
@@ -897,8 +880,7 @@ struct Bounds
 {
 	double sx[ORTHO_MAX_STEPS + 1];  // singular values of X before a step
 	double sa[ORTHO_MAX_STEPS];      // eigenvalues of A,
-	double sr[ORTHO_MAX_STEPS];      // of R = b A + c A^2,
-	double sp[ORTHO_MAX_STEPS];      // of a + R
+	double sr[ORTHO_MAX_STEPS];      // of R = b A + c A^2
 };
 // The largest singular value that a step may find follows from the extrema of its polynomial on [0, largest].
 bool bounds_of(const float (*coef)[3], int steps, Bounds& o)
@@ -912,12 +894,12 @@ bool bounds_of(const float (*coef)[3], int steps, Bounds& o)
 		auto h = [&](double l) { return fabs(a + l * (b + l * c)); };
 		auto e = [&](double l) { return fabs(l * (b + l * c)); };
 		o.sr[k] = e(o.sa[k]);
-		o.sp[k] = std::max(h(0.0), h(o.sa[k]));
+		double sp = std::max(h(0.0), h(o.sa[k]));  // of a + R
 		const double turn = c != 0.0 ? -b / (2 * c) : -1.0;
 		if (turn > 0.0 && turn < o.sa[k])
 		{
 			o.sr[k] = std::max(o.sr[k], e(turn));
-			o.sp[k] = std::max(o.sp[k], h(turn));
+			sp = std::max(sp, h(turn));
 		}
 		double most = h(t * t) * t;
 		// a + 3 b l + 5 c l^2 = 0 with l = s^2
@@ -936,7 +918,7 @@ bool bounds_of(const float (*coef)[3], int steps, Bounds& o)
 		for (int i = 0; i < n; ++i)
 			if (roots[i] > 0.0 && roots[i] < t * t) most = std::max(most, h(roots[i]) * sqrt(roots[i]));
 		o.sx[k + 1] = most * (1.0 + 1e-4);
-		if (!(o.sx[k + 1] <= 16.0) || !(o.sr[k] <= 256.0) || !(o.sp[k] <= 256.0)) return false;
+		if (!(o.sx[k + 1] <= 16.0) || !(o.sr[k] <= 256.0) || !(sp <= 256.0)) return false;
 	}
 	return true;
 }
@@ -949,119 +931,36 @@ float scale_under(double bound)
 	return ldexpf(1.0f, std::max(-40, std::min(15 - e, 40)));
 }
 
-// Steps of the groups.  A group multiplies what its A's rounding does to a small singular value by the product of its steps'
-// slopes at zero.  It may be up to `first` in the first group, whose A has elements of about 1/p, and 16 later (the usual slope is
-// 3.4445: groups of two under a limit of 16, a first one of three under 64).
-int groups_of(const float (*coef)[3], int steps, double first, int* size)
-{
-	int n = 0;
-	for (int k = 0; k < steps; ++n)
-	{
-		double growth = std::max(1.0, (double)fabsf(coef[k][0]));
-		size[n] = 1;
-		for (++k; k < steps && size[n] < 3; ++k, ++size[n])
-		{
-			growth *= std::max(1.0, (double)fabsf(coef[k][0]));
-			if (growth > (n == 0 ? first : 16.0)) break;
-		}
-	}
-	return n;
-}
-// Error of five steps against fp32 products', 2-norms, emulated: groups of 3 and 2 -- p = 256: 1.5e-6 against 2.4e-6, 128: 1.8e-6
-// against 1.7e-6, 64: 2.5e-6 against 1.1e-6; of 2, 2 and 1 -- 128: 1.5e-6, 64: 1.1e-6, 32: 1.5e-6 against 0.9e-6.
-bool groups_allowed(int program, int p) { return program == 0 || p >= (program == 1 ? 64 : 192); }
-
-void make_program(OrProgram& g, const float (*coef)[3], const Bounds& b, const int* size, int groups)
-{
-	bool alone = true;
-	for (int i = 0; i < groups; ++i) alone = alone && size[i] == 1;
-	const int T = 1, R0 = alone ? 1 : 2, Q0 = 4;
-	g.count = 0;
-	g.planes = alone ? 2 : OR_PLANES;
-	float scale[ID_X + 2] = {0};  // of the matrices' present contents
-	scale[ID_X] = scale_under(b.sx[0]);
-	int round = 0, k = 0, x = 0;
-	// out = f A B + w1 E1 + w2 E2
-	auto op = [&](int a, int bb, double f, int e1, double w1, int e2, double w2, int out, double bound) {
-		OrOp& o = g.op[g.count++];
-		o.a = (signed char)a; o.b = (signed char)bb; o.e1 = (signed char)e1; o.e2 = (signed char)e2; o.out = (signed char)out;
-		o.round = (signed char)round;
-		// (the scales are powers of two: the coefficients stay as they are)
-		o.f = (float)(f / scale[a] / scale[bb]);
-		o.w1 = e1 == ID_NONE ? 0.0f : (float)(w1 / scale[e1]);
-		o.w2 = e2 == ID_NONE ? 0.0f : (float)(w2 / scale[e2]);
-		o.so = out == ID_NONE ? 1.0f : scale_under(bound);
-	};
-	for (int i = 0; i < groups; ++i)
-	{
-		op(ID_X + x, ID_X + x, 1.0, ID_NONE, 0, ID_NONE, 0, ID_A, b.sa[k]);
-		scale[ID_A] = g.op[g.count - 1].so;
-		++round;
-		int Q = ID_NONE;
-		double q = 1.0, qbound = 1.0;
-		for (int j = 0; j < size[i]; ++j, ++k)
-		{
-			const double a = coef[k][0];
-			const bool more = j + 1 < size[i];
-			const int R = alone ? R0 : R0 + (j & 1);
-			op(ID_A, ID_A, coef[k][2], ID_A, coef[k][1], ID_NONE, 0, R, b.sr[k]);
-			scale[R] = g.op[g.count - 1].so;
-			++round;
-			qbound *= b.sp[k];
-			int next = R;
-			float next_scale = scale[R];
-			if (j > 0)
-			{
-				next = Q == Q0 ? Q0 + 1 : Q0;
-				op(R, Q, 1.0, Q, a, R, q, next, qbound + fabs(q * a));
-				next_scale = g.op[g.count - 1].so;
-			}
-			float t_scale = 0.0f;
-			if (more)
-			{
-				op(R, ID_A, 1.0, ID_A, a, ID_NONE, 0, T, b.sa[k] * b.sp[k]);
-				t_scale = g.op[g.count - 1].so;
-			}
-			if (j > 0 || more) ++round;
-			scale[next] = next_scale;
-			Q = next;
-			q = j > 0 ? q * a : a;
-			if (more)
-			{
-				scale[T] = t_scale;
-				op(T, R, 1.0, T, a, ID_NONE, 0, ID_A, b.sa[k + 1]);
-				scale[ID_A] = g.op[g.count - 1].so;
-				++round;
-			}
-		}
-		op(Q, ID_X + x, 1.0, ID_X + x, q, ID_NONE, 0, i + 1 < groups ? ID_X + (x ^ 1) : ID_NONE, b.sx[k]);
-		scale[ID_X + (x ^ 1)] = g.op[g.count - 1].so;
-		x ^= 1;
-		++round;
-	}
-	g.rounds = round;
-	int at = 0;
-	for (int r = 0; r <= OR_MAX_ROUNDS; ++r)
-	{
-		while (at < g.count && g.op[at].round < r) ++at;
-		g.first[r] = (unsigned char)at;
-	}
-}
-
-// The first `count` programs; returns X_0's scale.
-float make_programs(OrProgram* prog, int count, const OrthoArgs& a)
+// Returns X_0's scale.
+float make_program(OrProgram& g, const float (*coef)[3], int steps)
 {
 	Bounds b;
-	bounds_of(a.coef, a.steps, b);
-	int size[ORTHO_MAX_STEPS];
-	for (int k = 0; k < a.steps; ++k) size[k] = 1;
-	make_program(prog[0], a.coef, b, size, a.steps);
-	if (count > 1) make_program(prog[1], a.coef, b, size, groups_of(a.coef, a.steps, 16.0, size));
-	if (count > 2) make_program(prog[2], a.coef, b, size, groups_of(a.coef, a.steps, 64.0, size));
-	return scale_under(b.sx[0]);
+	bounds_of(coef, steps, b);
+	const float s0 = scale_under(b.sx[0]);
+	float scale[ID_X + 2] = {0};  // of the matrices' present contents
+	scale[ID_X] = s0;
+	g.count = 0;
+	// out = f A B + w E
+	auto op = [&](int a, int bb, double f, int e, double w, int out, double bound) {
+		OrOp& o = g.op[g.count++];
+		o.a = (signed char)a; o.b = (signed char)bb; o.e = (signed char)e; o.out = (signed char)out;
+		// (the scales are powers of two: the coefficients stay as they are)
+		o.f = (float)(f / scale[a] / scale[bb]);
+		o.w = e == ID_NONE ? 0.0f : (float)(w / scale[e]);
+		o.so = out == ID_NONE ? 1.0f : scale_under(bound);
+		if (out != ID_NONE) scale[out] = o.so;
+	};
+	for (int k = 0; k < steps; ++k)
+	{
+		const int x = ID_X + (k & 1), next = ID_X + (~k & 1);
+		op(x, x, 1.0, ID_NONE, 0.0, ID_A, b.sa[k]);
+		op(ID_A, ID_A, coef[k][2], ID_A, coef[k][1], ID_R, b.sr[k]);
+		op(ID_R, x, 1.0, x, coef[k][0], k + 1 < steps ? next : ID_NONE, b.sx[k + 1]);
+	}
+	return s0;
 }
 
-// A launch's plan: programs, which matrix takes which, the width of the tiles, how far tiles are split.
+// A launch's plan: the width of the tiles, how far they are split.
 struct Plan
 {
 	int bn;
@@ -1079,28 +978,25 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 	long long total = 0;
 	*reduce = 0;
 	*slots = 0;
-	for (int round = 0; round < P.rounds; ++round)
+	for (int round = 0; round < P.prog.count; ++round)
 	{
+		const OrOp& o = P.prog.op[round];
 		int tiles = 0;
 		long long work = 0;
 		auto each = [&](auto&& f) {
-			for (int i = 0; i < P.count; ++i)
-			{
-				const OrProgram& g = P.prog[P.mat[i].program];
-				for (int k = g.first[round]; k < g.first[round + 1]; ++k) f(i, k, op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, bn), op_kb(g.op[k], P.mat[i].p, P.mat[i].q));
-			}
+			for (int i = 0; i < P.count; ++i) f(i, op_tiles(o, P.mat[i].p, P.mat[i].q, bn), op_kb(o, P.mat[i].p, P.mat[i].q));
 		};
-		each([&](int, int, int n, int kb) {
+		each([&](int, int n, int kb) {
 			tiles += n;
 			work += (long long)n * kb;
 		});
-		// whole tiles, or parts of about equal length for all operations, so many that every SM has one
+		// whole tiles, or parts of about equal length for all matrices, so many that every SM has one
 		const long long share = std::max<long long>(OR_SPLIT_K / OR_BK, (work + OR_SMS - 1) / OR_SMS);
 		auto parts = [&](bool whole, int kb) { return whole ? 1 : (int)std::max<long long>(1, std::min<long long>(255, kb / share)); };
 		auto clocks = [&](bool whole) {
 			long long load[OR_SMS] = {0}, worst = 0;
 			int t = 0, used = 0;
-			each([&](int, int, int n, int kb) {
+			each([&](int, int n, int kb) {
 				const int s = parts(whole, kb);
 				if (s > 1) used += n * s;
 				const long long cost = item_clocks(bn, (kb + s - 1) / s);
@@ -1117,9 +1013,9 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 		const long long cost_split = tiles * 2 <= OR_SMS ? clocks(false) : cost;
 		const bool whole = cost <= cost_split;
 		int used = 0;
-		each([&](int i, int k, int n, int kb) {
-			split[i][k] = (unsigned char)parts(whole, kb);
-			if (split[i][k] > 1) used += n * split[i][k];
+		each([&](int i, int n, int kb) {
+			split[i][round] = (unsigned char)parts(whole, kb);
+			if (split[i][round] > 1) used += n * split[i][round];
 		});
 		if (used) *reduce |= 1ull << round;
 		*slots = std::max(*slots, used);
@@ -1128,31 +1024,10 @@ long long plan_width(const OrParams& P, int bn, unsigned char (*split)[OR_MAX_OP
 	return total;
 }
 
-// Grouped steps save multiply-adds (of matrices that are not nearly square) and cost rounds.
-bool may_group(int p, int q) { return p >= 64 && q > p + p / 16; }  // (a group's six p x p matrices instead of two)
-int choose_program(const OrProgram* prog, int p, int q)
-{
-	int best = 0;
-	double least = 0.0;
-	for (int v = 0; v < (may_group(p, q) ? OR_PROGRAMS : 1); ++v)
-	{
-		if (!groups_allowed(v, p)) continue;
-		double work = 0.0;
-		for (int k = 0; k < prog[v].count; ++k) work += (double)op_tiles(prog[v].op[k], p, q, 128) * op_kb(prog[v].op[k], p, q);
-		const double clocks = work * 900 / OR_SMS + (double)prog[v].rounds * (ROUND_CLOCKS + REDUCE_CLOCKS);
-		if (v == 0 || clocks < least)
-		{
-			best = v;
-			least = clocks;
-		}
-	}
-	return best;
-}
-
-size_t matrix_bytes(const OrMat& M, int planes)
+size_t matrix_bytes(const OrMat& M)
 {
 	const size_t p = round_up((size_t)M.p, 128), q = round_up((size_t)M.q, 128);
-	return (4 * p * q + 2 * planes * p * p) * sizeof(__half);
+	return (4 * p * q + 2 * OR_SQUARES * p * p) * sizeof(__half);
 }
 
 // Fills everything of P that does not depend on the workspace's address; returns the bytes of workspace.
@@ -1167,7 +1042,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	P.decay = a.decay;
 	P.eps = a.eps;
 	P.bad = a.bad;
-	P.s0 = make_programs(P.prog, OR_PROGRAMS, a);
+	P.s0 = make_program(P.prog, a.coef, a.steps);
 	for (int i = 0; i < count; ++i)
 	{
 		OrMat& M = P.mat[i];
@@ -1175,7 +1050,6 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.tall = M.m.rows > M.m.cols;
 		M.p = std::min(M.m.rows, M.m.cols);
 		M.q = std::max(M.m.rows, M.m.cols);
-		M.program = choose_program(P.prog, M.p, M.q);
 	}
 	// the matrices with the longest products first: what is left for the last CTAs of a round is small
 	std::stable_sort(P.mat, P.mat + count, [](const OrMat& x, const OrMat& y) { return (double)x.p * x.q > (double)y.p * y.q; });
@@ -1183,8 +1057,6 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 	for (int i = 0; i < count; ++i)
 	{
 		OrMat& M = P.mat[i];
-		const OrProgram& g = P.prog[M.program];
-		P.rounds = std::max(P.rounds, g.rounds);
 		M.ldx = (long long)round_up(M.q, 128);
 		M.planex = M.ldx * (long long)round_up(M.p, 128);
 		M.lds = (long long)round_up(M.p, 128);
@@ -1192,7 +1064,7 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 		M.units = P.units;
 		M.units_per_row = (M.m.cols + OR_UNIT - 1) / OR_UNIT;
 		P.units += M.units_per_row * ((M.m.rows + OR_UNIT - 1) / OR_UNIT);
-		bytes += matrix_bytes(M, g.planes);
+		bytes += matrix_bytes(M);
 	}
 	long long best = -1;
 	for (int bn : {128, 64})
@@ -1212,37 +1084,33 @@ size_t make_plan(OrParams& P, const OrthoArgs& a, const OrthoMatrix* m, int coun
 }
 
 template <int BN>
-bool make_maps(OrMaps& o, const OrMat& M, int planes)
+bool make_maps(OrMaps& o, const OrMat& M)
 {
 	return tc_make_parts_map(&o.xa, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, TC_BM) &&
 	       tc_make_parts_map(&o.xb, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, BN) &&
 	       tc_make_parts_map_mn(&o.xn, M.X, M.p, M.q, M.ldx, M.planex, 4, OR_BK, BN) &&
-	       tc_make_parts_map(&o.sa, M.S, M.p, M.p, M.lds, M.planes, 2 * planes, OR_BK, TC_BM) &&
-	       tc_make_parts_map(&o.sb, M.S, M.p, M.p, M.lds, M.planes, 2 * planes, OR_BK, BN);
+	       tc_make_parts_map(&o.sa, M.S, M.p, M.p, M.lds, M.planes, 2 * OR_SQUARES, OR_BK, TC_BM) &&
+	       tc_make_parts_map(&o.sb, M.S, M.p, M.p, M.lds, M.planes, 2 * OR_SQUARES, OR_BK, BN);
 }
 
 template <int BN>
 cudaError_t launch_width(OrParams& P, cudaStream_t s)
 {
 	for (int i = 0; i < P.count; ++i)
-		if (!make_maps<BN>(P.maps[i], P.mat[i], P.prog[P.mat[i].program].planes)) return cudaErrorInvalidValue;
+		if (!make_maps<BN>(P.maps[i], P.mat[i])) return cudaErrorInvalidValue;
 	int sms = 0;
 	cudaError_t e = prepare_tc_launch(reinterpret_cast<const void*>(ortho_kernel<BN>), OrSmem<BN>::TOTAL, &sms);
 	if (e != cudaSuccess) return e;
 	// no more CTAs than the largest round has items and pieces
 	int most = P.units;
-	for (int round = 0; round < P.rounds; ++round)
+	for (int round = 0; round < P.prog.count; ++round)
 	{
 		int n = 0, splits = 0;
 		for (int i = 0; i < P.count; ++i)
 		{
-			const OrProgram& g = P.prog[P.mat[i].program];
-			for (int k = g.first[round]; k < g.first[round + 1]; ++k)
-			{
-				const int tiles = op_tiles(g.op[k], P.mat[i].p, P.mat[i].q, BN);
-				n += tiles * P.split[i][k];
-				if (P.split[i][k] > 1) splits += tiles;
-			}
+			const int tiles = op_tiles(P.prog.op[round], P.mat[i].p, P.mat[i].q, BN);
+			n += tiles * P.split[i][round];
+			if (P.split[i][round] > 1) splits += tiles;
 		}
 		P.items[round] = n;
 		P.splits[round] = splits;
@@ -1284,8 +1152,8 @@ size_t ortho_workspace_bytes(const OrthoMatrix* m, int count)
 			OrMat M;
 			M.p = std::min(m[i].rows, m[i].cols);
 			M.q = std::max(m[i].rows, m[i].cols);
-			bytes += matrix_bytes(M, may_group(M.p, M.q) ? OR_PLANES : 2);
-			if (M.q > OR_SPLIT_K) parts += 2 * ceil(M.p / 128.0) * ceil(M.q / 64.0) * ceil(M.q / (double)OR_SPLIT_K);
+			bytes += matrix_bytes(M);
+			if (M.q > OR_SPLIT_K) parts += ceil(M.p / 128.0) * ceil(M.q / 64.0) * ceil(M.q / (double)OR_SPLIT_K);
 		}
 		most = std::max(most, bytes + (size_t)std::min(parts, (double)OR_SMS) * 128 * 128 * sizeof(float));
 	}
@@ -1321,8 +1189,8 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			while (n > 0) m[count++] = vectors[--n];
 		if (small)
 		{
-			const float s0 = make_programs(P.prog, 1, a);
-			const cudaError_t e = launch_ortho_small(a, P.prog[0], s0, m, count, status, reset, false, s);
+			const float s0 = make_program(P.prog, a.coef, a.steps);
+			const cudaError_t e = launch_ortho_small(a, P.prog, s0, m, count, status, reset, false, s);
 			if (e != cudaSuccess) return e;
 			continue;
 		}
@@ -1343,10 +1211,10 @@ cudaError_t launch_orthogonalize(const OrthoArgs& a, void* work, size_t work_byt
 			OrMat& M = P.mat[i];
 			M.X = reinterpret_cast<__half*>(at);
 			M.S = M.X + 4 * M.planex;
-			at += matrix_bytes(M, P.prog[M.program].planes);
+			at += matrix_bytes(M);
 		}
 		cudaError_t e = plan.bn == 128 ? launch_width<128>(P, s) : launch_width<64>(P, s);
-		if (e == cudaSuccess && n > 0) e = launch_ortho_small(a, P.prog[0], P.s0, vectors, n, status, false, true, s);
+		if (e == cudaSuccess && n > 0) e = launch_ortho_small(a, P.prog, P.s0, vectors, n, status, false, true, s);
 		if (e != cudaSuccess) return e;
 	}
 	return cudaSuccess;

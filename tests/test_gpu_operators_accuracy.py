@@ -214,3 +214,8 @@ def test_errors_of_small_matrices(g, p, q):
 @pytest.mark.parametrize("p,q", [(192, 192), (256, 256), (256, 1000), (500, 1000), (1000, 784), (1024, 1024), (20, 2048)])
 def test_errors_of_matrices(g, p, q):
     check_structured(g, min(p, q), max(p, q), tall=p > q)
+
+
+@pytest.mark.parametrize("p,q", [(512, 2048), (512, 4096), (300, 3000), (1024, 4096), (4096, 640)])
+def test_errors_of_flat_matrices(g, p, q):
+    check_structured(g, min(p, q), max(p, q), tall=p > q)
