@@ -219,3 +219,26 @@ def test_errors_of_matrices(g, p, q):
 @pytest.mark.parametrize("p,q", [(512, 2048), (512, 4096), (300, 3000), (1024, 4096), (4096, 640)])
 def test_errors_of_flat_matrices(g, p, q):
     check_structured(g, min(p, q), max(p, q), tall=p > q)
+
+
+SCHEDULE = [(1.2, -0.9, 0.5), (2.6, -2.4, 0.8), (0.7, 0.3, -0.1), (2.2, -1.4, 0.3), (0.9, -0.2, 0.15), (1.6, -0.7, 0.2)]
+
+
+@pytest.mark.parametrize("shapes", [[(1, 300), (500, 1), (1, 1)], [(20, 50), (1, 90), (64, 500), (30, 30)], [(300, 280), (40, 30), (1, 70)], [(400, 4096)],
+                                    [(4096, 400), (5, 6)]])
+def test_every_step_takes_its_own_coefficients(g, shapes):
+    """Single rows and columns, small matrices, tiles, and flat ones: the error is that of fp32 products with the same list, and no
+    other order of the list comes near."""
+    coef = fp32(SCHEDULE)
+    ins = [torch.randn(m, n, generator=gen(60 + i), device=DEV) for i, (m, n) in enumerate(shapes)]
+    outs = [torch.empty_like(a) for a in ins]
+    run_ortho(g, ins, outs, "f32", len(coef), SCHEDULE)
+    for a, b in zip(ins, outs):
+        exact = iterate(a.double(), len(coef), coef, 1e-7, torch.float64)
+        plain = float((iterate(a, len(coef), coef, 1e-7, torch.float32).double() - exact).norm() / exact.norm())
+        got = float((b.double() - exact).norm() / exact.norm())
+        assert got <= 2.5 * plain + 4 * U * 10.25 / 0.7, (tuple(a.shape), got, plain)
+        for k in range(len(coef) - 1):
+            other = coef[:k] + [coef[k + 1], coef[k]] + coef[k + 2:]
+            off = float((iterate(a.double(), len(coef), other, 1e-7, torch.float64) - exact).norm() / exact.norm())
+            assert off > 100 * got, (tuple(a.shape), k, off, got)
