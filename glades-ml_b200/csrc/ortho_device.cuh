@@ -5,6 +5,7 @@
 
 #include <cuda_bf16.h>
 
+#include "ortho_walk.h"
 #include "orthogonalize.h"
 #include "tc_device.cuh"
 
@@ -14,14 +15,6 @@ using namespace tc;
 // Three products a step, one behind the other: A = X X^T, R = b A + c A A, X <- a X + R X.
 constexpr int OR_MAX_OPS = 3 * ORTHO_MAX_STEPS;
 
-// Matrices of parts that an operation names: two p x p, and the two X.
-enum { ID_A = 0, ID_R = 1, ID_X = 2, ID_NONE = -1 };
-// out = f (A B^T or A B) + w E; the factors hold the parts' scales
-struct OrOp
-{
-	signed char a, b, e, out;  // out ID_NONE: the result
-	float f, w, so;
-};
 struct OrProgram
 {
 	OrOp op[OR_MAX_OPS];

@@ -39,9 +39,7 @@ namespace glb {
 using namespace tc;
 namespace {
 
-// k per pipeline stage.  A stage costs the multiplying warp two waits and a commit, about 350 clocks, whatever its MMAs take: with
-// stages of 32 k that bounded both tiles (530 clocks per 32 k on 128 columns, 350 to 400 now).
-constexpr int OR_BK = 64;
+static_assert(OR_BM == TC_BM, "tiles");
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_SMS = 148;
 constexpr int OR_SQUARES = 2;  // p x p matrices of parts: A and R
@@ -102,105 +100,6 @@ struct OrParams
 	double* sums;  // [matrix][grid] sums of squares
 	float4* part;  // parts of split tiles
 };
-
-// An operation's tiles of one matrix, of a symmetric product only those that reach the diagonal.
-__host__ __device__ inline bool op_symmetric(const OrOp& o) { return o.b < ID_X || o.a >= ID_X; }
-__host__ __device__ inline int op_kb(const OrOp& o, int p, int q) { return ((o.a >= ID_X ? q : p) + OR_BK - 1) / OR_BK; }
-__host__ __device__ inline int tiles_of_row(int mt, int tn, int bn)
-{
-	const int c = (mt * TC_BM + TC_BM - 1) / bn + 1;
-	return c < tn ? c : tn;
-}
-__host__ __device__ inline int op_tiles(const OrOp& o, int p, int q, int bn)
-{
-	const int tm = (p + TC_BM - 1) / TC_BM;
-	if (!op_symmetric(o)) return tm * ((q + bn - 1) / bn);
-	const int tn = (p + bn - 1) / bn;
-	// (in closed form but for the rows that tn cuts off)
-	int n = 0;
-	for (int mt = 0; mt < tm; ++mt) n += tiles_of_row(mt, tn, bn);
-	return n;
-}
-
-struct OrItem
-{
-	int mat, m0, n0, kb0, kb1, split, slot;  // slot: of a split tile's first part
-};
-// the tile t of operation o
-template <int BN>
-__device__ __forceinline__ void tile_origin(const OrOp& o, int p, int q, int t, int& m0, int& n0)
-{
-	const int tm = (p + TC_BM - 1) / TC_BM;
-	if (!op_symmetric(o))
-	{
-		m0 = (t % tm) * TC_BM;
-		n0 = (t / tm) * BN;
-		return;
-	}
-	const int tn = (p + BN - 1) / BN;
-	for (int mt = tm - 1;; --mt)
-	{
-		const int n = tiles_of_row(mt, tn, BN);
-		if (t < n || mt == 0)
-		{
-			m0 = mt * TC_BM;
-			n0 = t * BN;
-			return;
-		}
-		t -= n;
-	}
-}
-// item t < P.items[round] of a round
-template <int BN>
-__device__ __forceinline__ void find_item(const OrParams& P, int round, int t, OrItem& it)
-{
-	const OrOp& o = P.prog.op[round];
-	int slot = 0;
-	for (int i = 0;; ++i)
-	{
-		const OrMat& M = P.mat[i];
-		const int s = P.split[i][round];
-		const int n = op_tiles(o, M.p, M.q, BN) * s;
-		if (t < n)
-		{
-			const int tile = t / s, part = t - tile * s;
-			const int kb = op_kb(o, M.p, M.q);
-			it.mat = i;
-			it.split = s;
-			it.kb0 = kb * part / s;
-			it.kb1 = kb * (part + 1) / s;
-			it.slot = slot + t;
-			tile_origin<BN>(o, M.p, M.q, tile, it.m0, it.n0);
-			return;
-		}
-		t -= n;
-		if (s > 1) slot += n;
-	}
-}
-// tile t < P.splits[round] of a round's split matrices
-template <int BN>
-__device__ __forceinline__ void find_split(const OrParams& P, int round, int t, OrItem& it)
-{
-	const OrOp& o = P.prog.op[round];
-	int slot = 0;
-	for (int i = 0;; ++i)
-	{
-		const OrMat& M = P.mat[i];
-		const int s = P.split[i][round];
-		if (s < 2) continue;
-		const int n = op_tiles(o, M.p, M.q, BN);
-		if (t < n)
-		{
-			it.mat = i;
-			it.split = s;
-			it.slot = slot + t * s;
-			tile_origin<BN>(o, M.p, M.q, t, it.m0, it.n0);
-			return;
-		}
-		t -= n;
-		slot += n * s;
-	}
-}
 
 // ---- 32 x 32 pieces, a row per lane --------------------------------------------------------------------------------
 // 16-byte chunk k (0 .. 3 hi, 4 .. 7 lo) of row r in the warp's staging area
@@ -440,6 +339,14 @@ __device__ __forceinline__ bool meet(unsigned* arrived, unsigned all, volatile i
 	return *abort_flag != MEETING_LOST;
 }
 
+// A warp has been asked for an item that its round does not have.
+__device__ __noinline__ static void give_up(volatile int* abort_flag, int* err_flag, int lane)
+{
+	if (lane != 0) return;
+	*abort_flag = 1;
+	atomicExch(err_flag, 6);
+}
+
 template <int BN>
 __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __grid_constant__ OrParams P)
 {
@@ -650,7 +557,12 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	uint32_t aph = 0;
 	bool ok = true;
 	OrItem t;              // copying and multiplying warps: a round's first item is looked up in front of the barrier before it
-	if (warp < 2 && (int)blockIdx.x < P.items[0]) find_item<BN>(P, 0, blockIdx.x, t);
+	auto look_up = [&](int round, int ti) {
+		if (find_item<BN>(P, round, ti, t)) return true;
+		give_up(abort_flag, P.status, lane);
+		return false;
+	};
+	if (warp < 2 && (int)blockIdx.x < P.items[0]) ok = look_up(0, blockIdx.x);
 	for (int round = 0; met && round < P.prog.count; ++round)
 	{
 		const int items = P.items[round];
@@ -664,7 +576,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			const bool leader = elect_one();
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
-				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
+				if (ti != (int)blockIdx.x && !look_up(round, ti)) { ok = false; break; }
 				const OrMaps& mp = P.maps[t.mat];
 				const bool ax = o.a >= ID_X, bx = o.b >= ID_X;
 				const CUtensorMap* ma = ax ? &mp.xa : &mp.sa;
@@ -703,7 +615,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			const bool leader = elect_one();
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
-				if (ti != (int)blockIdx.x) find_item<BN>(P, round, ti, t);
+				if (ti != (int)blockIdx.x && !look_up(round, ti)) { ok = false; break; }
 				const uint32_t b_mn = o.b >= ID_X && o.a < ID_X ? 1u : 0u;
 				const uint32_t idesc = (1u << 4) | (b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 				const uint32_t idesc2 = (1u << 4) | (b_mn << 16) | ((uint32_t)(S::COLUMNS >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
@@ -751,7 +663,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 			const int quarter = warp & 3, half = (warp - S::FIRST) >> 2;
 			for (int ti = blockIdx.x; ok && ti < items; ti += gridDim.x)
 			{
-				find_item<BN>(P, round, ti, t);
+				if (!look_up(round, ti)) { ok = false; break; }
 				const OrMat& M = P.mat[t.mat];
 				const OrTarget target(M, o);
 				const float f = o.f;
@@ -822,7 +734,11 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 				// (neighbouring pieces on different SMs)
 				for (int k = (warp - S::FIRST) * (int)gridDim.x + (int)blockIdx.x; k < P.splits[round] * S::PIECES; k += warps)
 				{
-					find_split<BN>(P, round, k / S::PIECES, t);
+					if (!find_split<BN>(P, round, k / S::PIECES, t))
+					{
+						give_up(abort_flag, P.status, lane);
+						break;
+					}
 					const OrTarget target(P.mat[t.mat], o);
 					const int pc = k % S::PIECES;
 					const int r0 = t.m0 + pc / (BN / 32) * 32, c0 = t.n0 + pc % (BN / 32) * 32;
@@ -852,7 +768,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 		}
 		if (round + 1 < P.prog.count)
 		{
-			if (warp < 2 && (int)blockIdx.x < P.items[round + 1]) find_item<BN>(P, round + 1, blockIdx.x, t);
+			if (ok && warp < 2 && (int)blockIdx.x < P.items[round + 1]) ok = look_up(round + 1, blockIdx.x);
 			if (!meet(P.arrived, meeting += gridDim.x, abort_flag, P.status)) break;
 		}
 	}
