@@ -846,8 +846,14 @@ cudaError_t forward_elems(const LayerNormArgs& a, cudaStream_t s)
 	// (LN_SMS is even: a group that walks sees rows of one kind only, where every other row begins in the middle of a word)
 	const long long most = (long long)LN_SMS * std::max(1, (ELEMS == 16 ? 768 : 512) / threads);
 	const unsigned grid = (unsigned)(want < most ? want : most);
-	if (group > 32) norm_kernel<T, MODE, ELEMS, true><<<grid, threads, 0, s>>>(a, group);
-	else norm_kernel<T, MODE, ELEMS, false><<<grid, threads, 0, s>>>(a, group);
+	// (more than 16 elements per lane are rows of more than 4096: more lanes than a warp's)
+	if constexpr (ELEMS == 16)
+		if (group <= 32)
+		{
+			norm_kernel<T, MODE, ELEMS, false><<<grid, threads, 0, s>>>(a, group);
+			return cudaGetLastError();
+		}
+	norm_kernel<T, MODE, ELEMS, true><<<grid, threads, 0, s>>>(a, group);
 	return cudaGetLastError();
 }
 
