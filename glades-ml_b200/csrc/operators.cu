@@ -137,12 +137,14 @@ int run_ortho(const char* name, OrthoArgs& a, const std::vector<OrthoMatrix>& m,
 {
 	a.mat = m.data();
 	a.count = (int)m.size();
-	if (a.count == 0) return GL_OK;
+	if (a.count == 0 && (!d_work || work_bytes < (int64_t)ortho_workspace_bytes(nullptr, 0))) return GL_OK;
 	if (!d_work || work_bytes < (int64_t)ortho_workspace_bytes(a.mat, a.count))
 		return report_error(GL_ERR_INVALID, "%s: the workspace is too small", name);
 	if (int r = check_device(device)) return r;
 	OnDevice guard(device);
 	if (guard.error != cudaSuccess) return finish(name, guard.error);
+	// (a workspace needs no initialisation: its status is this call's, whatever it held)
+	if (a.count == 0) return finish(name, cudaMemsetAsync(ortho_status(d_work), 0, sizeof(int), static_cast<cudaStream_t>(stream)));
 	return finish(name, launch_orthogonalize(a, d_work, (size_t)work_bytes, static_cast<cudaStream_t>(stream)));
 }
 

@@ -136,6 +136,14 @@ def test_zero_matrices_give_zeros_without_eps_too(g, shapes):
         assert bool(((b.double() - exact).abs() <= ortho_tolerance(a, 5, coefs(5), 0.0, exact)).all())
 
 
+def test_status_behind_a_call_without_matrices(g):
+    items = g.ortho_items([])
+    bytes_ = g.orthogonalize_workspace(items)
+    work = torch.full((bytes_,), 0xFF, dtype=torch.uint8, device=DEV)
+    g.orthogonalize(items, work.data_ptr(), bytes_, stream=stream())
+    g.orthogonalize_status(work.data_ptr(), stream=stream())
+
+
 # ---- the orthogonalisation's error beside that of fp32 products ---------------------------------------------------------
 def fp32(coef):
     """Coefficients as the entry point holds them."""
