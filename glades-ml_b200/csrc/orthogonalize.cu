@@ -243,7 +243,7 @@ __device__ __forceinline__ void update_weights(const float (&v)[32], const Ortho
 // constant memory, whose first touch takes as long as a copy from L2.
 struct OrTarget
 {
-	float f, so;
+	float so;
 	int kind, p, q;  // kind: 0 the caller's matrix, 1 symmetric, 2 X
 	__half* D;
 	long long plane, ld;
@@ -256,7 +256,7 @@ struct OrTarget
 		plane = o.out >= ID_X ? M.planex : M.planes;
 		ld = o.out >= ID_X ? M.ldx : M.lds;
 		D = o.out >= ID_X ? M.X + 2 * (o.out - ID_X) * plane : M.S + 2 * (o.out < 0 ? 0 : o.out) * plane;
-		asm volatile("" : "+f"(f), "+f"(so), "+r"(p), "+r"(q), "+r"(kind), "+l"(plane), "+l"(ld), "+l"(D));
+		asm volatile("" : "+f"(so), "+r"(p), "+r"(q), "+r"(kind), "+l"(plane), "+l"(ld), "+l"(D));
 	}
 	// pieces that lie outside the matrix, or above the diagonal of a symmetric result (another piece's mirror image)
 	__device__ __forceinline__ bool needs(int r0, int c0) const { return r0 < p && (kind == 1 ? c0 <= r0 : c0 < q); }
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(OrSmem<BN>::THREADS, 1) ortho_kernel(const __g
 	uint8_t* tail = gen_base + S::TILES_BYTES + S::STAGING_BYTES + 8 * NBARS;
 	uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail);
 	volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + 4);
-	double* warp_sums = reinterpret_cast<double*>(tail + 8);  // 10 at most
+	double* warp_sums = reinterpret_cast<double*>(tail + 8);  // one per warp
 
 	cg::grid_group grid = cg::this_grid();
 	cudaTriggerProgrammaticLaunchCompletion();  // (single rows and columns have nothing to wait for)
