@@ -391,7 +391,8 @@ enum { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
 /* Layer norm of the rows of x [rows][n]: mean and variance (divided by n) of each row, xh = (x - mean) / sqrt(variance +
  * eps), y = gain * xh + shift.  x and y are of `type`, ldx and ldy (>= n) elements from row to row; gain and shift, fp32 [n],
  * may each be NULL (ones, zeros).  d_mean and d_rstd, fp32 [rows], receive mean and 1 / sqrt(variance + eps) for the backward
- * pass; each may be NULL.  All arithmetic is fp32, y is rounded once.  y may be x (with the same pitch).  rows may be 0. */
+ * pass; each may be NULL.  All arithmetic is fp32, y is rounded once.  y may be x (with the same pitch), and overlaps nothing
+ * otherwise.  rows may be 0. */
 int gl_layer_norm(const void* d_x, int64_t ldx, const float* d_gain, const float* d_shift, void* d_y, int64_t ldy, float* d_mean,
                   float* d_rstd, int64_t rows, int32_t n, float eps, int32_t type, void* stream, int32_t device);
 /* The backward pass: from dy (`type`, pitch lddy), x and the forward pass's mean and rstd: dx (`type`, pitch lddx, may be NULL,
@@ -405,11 +406,13 @@ int gl_layer_norm_backward(const void* d_dy, int64_t lddy, const void* d_x, int6
 /* Orthogonalisation of a list of matrices by Newton-Schulz products:
  *     X = U / (|U|_F + eps);  `steps` times:  A = X X^T,  X = a X + (b A + c A A) X
  * (for a tall matrix with X^T X from the right, the same numbers).  It keeps the singular vectors of U and brings the singular values
- * near 1.  coefficients: host array [steps][3] of a, b, c, or NULL: 3.4445, -4.7750, 2.0315 in every step; 1 <= steps <= 16.
- * Coefficients under which a singular value of [0, 1] could grow beyond 16 are refused (GL_ERR_INVALID).  Every product is
- * fp32-faithful (three fp16 products on tensor cores), the result is rounded to the output's type once.  A zero matrix
- * gives zeros; a matrix with a NaN or an infinity gives NaN.  In and out are row-major of `type`, pitches in elements; out may
- * be in.  The matrices are worked on at once: an output that is listed twice, or is another matrix's input, is refused.
+ * near 1.  Its error is relative to singular values of 1: where |U|_F lies so far below eps that all of the result is small, an
+ * element is exact to about 1e-9 (single rows and columns: to fp32's rounding).  coefficients: host array [steps][3] of a, b, c,
+ * or NULL: 3.4445, -4.7750, 2.0315 in every step; 1 <= steps <= 16.  Coefficients under which a singular value of [0, 1] could
+ * grow beyond 16 are refused (GL_ERR_INVALID).  Every product is fp32-faithful (three fp16 products on tensor cores) whatever the
+ * type, the result is rounded to the output's type once.  A zero matrix gives zeros, without an eps too; a matrix with a NaN or an
+ * infinity gives NaN.  In and out are row-major of `type`, pitches in elements; out may be in.  The matrices are worked on at once: an
+ * output that is listed twice, or is another matrix's input, is refused (other overlaps are not looked for, and not allowed).
  * (A column-major matrix is the transposed one row-major: its result comes out transposed too.) */
 typedef struct gl_ortho_item {
 	int32_t rows, cols;

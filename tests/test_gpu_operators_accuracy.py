@@ -136,6 +136,26 @@ def test_zero_matrices_give_zeros_without_eps_too(g, shapes):
         assert bool(((b.double() - exact).abs() <= ortho_tolerance(a, 5, coefs(5), 0.0, exact)).all())
 
 
+@pytest.mark.parametrize("size", [1e-6, 1e-8, 1e-10, 1e-13, 1e-30])
+@pytest.mark.parametrize("shapes", [[(1, 300), (200, 1)], [(40, 70), (90, 30)], [(300, 200), (260, 520)]])
+def test_matrices_far_below_eps(g, shapes, size):
+    """Where |U| lies below eps all of the result is small.  Parts of X_0 are exact to 2^-39 (half a step of the smallest fp16 number under
+    the scale of 2^14), those of every later X too, and a step multiplies by 3.4445 at most: 2^-39 * 3.4445 * (1 + 3.4445 + ..) of an
+    element, beside what is relative to the result.  Single rows and columns have no parts."""
+    ins = [gradient(m, n, 17) for m, n in shapes]
+    ins = [a * (size / a.double().norm().float()) for a in ins]
+    outs = [torch.full((a.shape[0], a.shape[1]), 7.0, device=DEV) for a in ins]
+    run_ortho(g, ins, outs, "f32")
+    for a, b in zip(ins, outs):
+        exact = iterate(a.double(), 5, fp32(coefs(5)), float(torch.tensor(1e-7, dtype=torch.float32)), torch.float64)
+        plain = float((iterate(a, 5, fp32(coefs(5)), 1e-7, torch.float32).double() - exact).abs().max())
+        tol = 2.5 * plain + 4 * U * 10.25 / 0.7 * float(exact.abs().max())
+        if min(a.shape) > 1:
+            tol += 2.0 ** -39 * sum(3.4445 ** k for k in range(1, 6))
+        assert float(exact.abs().max()) > 0.0
+        assert float((b.double() - exact).abs().max()) <= tol, tuple(a.shape)
+
+
 def test_status_behind_a_call_without_matrices(g):
     items = g.ortho_items([])
     bytes_ = g.orthogonalize_workspace(items)
