@@ -768,7 +768,7 @@ bool cluster_fused_fits(const NetView& n)
 static cudaError_t cluster_fused_config(const NetView& n, cudaLaunchConfig_t& cfg, cudaLaunchAttribute* attrs, unsigned grid, cudaStream_t s)
 {
 	const size_t bytes = cluster_fused_smem_bytes(n);
-	cudaError_t e = cudaFuncSetAttribute(cluster_fused_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(cluster_fused_kernel));
 	if (e != cudaSuccess) return e;
 	memset(&cfg, 0, sizeof cfg);
 	cfg.gridDim = dim3(grid);

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) gemm_skinny_kernel(const GemmArgs g)
 template <int EPI, int NN, int ROWS>
 static cudaError_t launch_skinny(const GemmArgs& g, long long blocks, size_t bytes, cudaStream_t s)
 {
-	const cudaError_t e = cudaFuncSetAttribute(gemm_skinny_kernel<EPI, NN, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	const cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(gemm_skinny_kernel<EPI, NN, ROWS>));
 	if (e != cudaSuccess) return e;
 	ChainedLaunch c(dim3((unsigned)blocks), 256, bytes, true, s);
 	return cudaLaunchKernelEx(&c.config, gemm_skinny_kernel<EPI, NN, ROWS>, g);

@@ -32,6 +32,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "tc_epilogue.cuh"
@@ -668,37 +669,66 @@ bool tc_make_operand_map_f32(void* out128, const float* ptr, int mn, long long R
 	          CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The shared-memory opt-in of a kernel and the SM count of the current device (both belong to a device, not to the process; kept
-// per kernel and device).
-cudaError_t prepare_tc_launch(const void* kernel, int smem_bytes, int* sm_count)
+// A kernel's limit of dynamic shared memory belongs to the context, not to a launch, and can be lowered.  So it is set once per kernel and
+// device, to the most that any launch asks for: launches of other sizes from other host threads then take nothing away from one
+// another.  bytes 0: as much as the kernel's own static shared memory leaves.
+static cudaError_t set_limit_once(const void* kernel, int bytes, int* dev)
 {
 	constexpr int kMaxDev = 64;
 	struct Done { const void* kernel; bool dev[kMaxDev]; };
 	static std::mutex mutex;
 	static std::vector<Done> done;
-	static int sms[kMaxDev] = {};
-	int dev = 0;
-	if (cudaError_t e = cudaGetDevice(&dev)) return e;
-	if (dev < 0 || dev >= kMaxDev) return cudaErrorInvalidDevice;
+	if (cudaError_t e = cudaGetDevice(dev)) return e;
+	if (*dev < 0 || *dev >= kMaxDev) return cudaErrorInvalidDevice;
 	std::lock_guard<std::mutex> lock(mutex);
 	Done* d = nullptr;
 	for (Done& x : done)
 		if (x.kernel == kernel) d = &x;
 	if (!d)
 	{
-		done.push_back(Done());
+		try
+		{
+			done.push_back(Done());
+		}
+		catch (const std::bad_alloc&)
+		{
+			return cudaErrorMemoryAllocation;
+		}
 		d = &done.back();
 		memset(d, 0, sizeof *d);
 		d->kernel = kernel;
 	}
-	if (!d->dev[dev])
+	if (d->dev[*dev]) return cudaSuccess;
+	if (bytes == 0)
 	{
-		if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes)) return e;
-		d->dev[dev] = true;
+		cudaFuncAttributes a;
+		if (cudaError_t e = cudaFuncGetAttributes(&a, kernel)) return e;
+		if (cudaError_t e = cudaDeviceGetAttribute(&bytes, cudaDevAttrMaxSharedMemoryPerBlockOptin, *dev)) return e;
+		bytes -= (int)a.sharedSizeBytes;
 	}
-	if (!sms[dev])
-		if (cudaError_t e = cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev)) return e;
-	*sm_count = sms[dev];
+	if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+	d->dev[*dev] = true;
+	return cudaSuccess;
+}
+cudaError_t allow_shared_memory(const void* kernel)
+{
+	int dev = 0;
+	return set_limit_once(kernel, 0, &dev);
+}
+
+// The shared-memory opt-in of a kernel, and the SM count of the current device (kept per device).
+cudaError_t prepare_tc_launch(const void* kernel, int smem_bytes, int* sm_count)
+{
+	static std::atomic<int> sms[64];
+	int dev = 0;
+	if (cudaError_t e = set_limit_once(kernel, smem_bytes, &dev)) return e;
+	int n = sms[dev];
+	if (n == 0)
+	{
+		if (cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev)) return e;
+		sms[dev] = n;
+	}
+	*sm_count = n;
 	return cudaSuccess;
 }
 

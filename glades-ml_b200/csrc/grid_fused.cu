@@ -1167,8 +1167,7 @@ cudaError_t launch_grid_fused(const GridFusedArgs& a, cudaStream_t s)
 	}
 	const size_t bytes = gf_smem_bytes(a.net, rows);
 	void* fn = grid_fused_function(rows, a.tma != nullptr);
-	// the attribute belongs to the current device: set it per launch (a cheap call) rather than cache it per process
-	const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	const cudaError_t e = allow_shared_memory(fn);
 	if (e != cudaSuccess) return e;
 	GridFusedArgs copy = a;
 	void* params[] = {&copy};

@@ -355,6 +355,9 @@ cudaError_t launch_activation_gradient(float* D, const float* A, long long rows,
 // param: gain | shift | dgain | dshift of n floats each; gain and shift -= step * their sums; flags[0] on a new value that is not finite
 cudaError_t launch_norm_update(float* param, int n, float step, int* flags, cudaStream_t s);
 
+// Lets a kernel's launches on the current device ask for as much dynamic shared memory as there is (gemm_tcgen05.cu).
+cudaError_t allow_shared_memory(const void* kernel);
+
 // ---- errors of entry points outside api.cu: the text that gl_last_error() returns; returns code
 int report_error(int code, const char* fmt, ...);
 

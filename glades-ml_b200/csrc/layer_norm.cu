@@ -873,8 +873,6 @@ cudaError_t backward_mode(const LayerNormArgs& a, int* ctas, cudaStream_t s)
 	*ctas = grid;
 	const int parts = group > 32 ? threads / group : threads / 32;
 	size_t smem = parts > 1 ? (size_t)parts * a.n * sizeof(float2) : 0;
-	// The limit of a kernel's shared memory is the context's, not the call's, and can be lowered: it is set once, to the most that
-	// any shape needs, so that threads with other shapes at the same time take nothing away from one another.
 	constexpr size_t most = MODE == BY_QUADS ? quads_bytes<T>(LN_GROUP_MAX) : sums_bytes;
 	auto go = [&](void (*kernel)(LayerNormArgs, int)) {
 		int sms = 0;

@@ -593,7 +593,7 @@ cudaError_t launch_standardize(const StandardizeArgs& a, cudaStream_t s)
 	if (a.write && tile >= 16 && a.rows >= tile && ((((uintptr_t)a.raw) | ((uintptr_t)a.x) | ((uintptr_t)a.y)) & 15) == 0)
 	{
 		const size_t bytes = 2 * ((size_t)tile * 4 * (a.cols + a.width) + 3 * 128);
-		e = cudaFuncSetAttribute(transform_tiles_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+		e = allow_shared_memory(reinterpret_cast<const void*>(transform_tiles_kernel));
 		if (e != cudaSuccess) return e;
 		const long long tiles = a.rows / tile;
 		ChainedLaunch c(dim3((unsigned)(tiles < 148 * 3 ? tiles : 148 * 3)), 256, bytes, true, s);

@@ -769,7 +769,7 @@ static cudaError_t launch_ref_small(const RefTrainArgs& a, size_t bytes, cudaStr
 {
 	void (*kernel)(RefTrainArgs) = a.net.H == 1 ? (a.net.mb == 1 ? ref_train_small_kernel<1, true> : ref_train_small_kernel<1, false>)
 	                                            : (a.net.mb == 1 ? ref_train_small_kernel<2, true> : ref_train_small_kernel<2, false>);
-	cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel));
 	if (e != cudaSuccess) return e;
 	kernel<<<1, ref_small_threads(a.net) + 64, bytes, s>>>(a);
 	return cudaGetLastError();
@@ -1051,14 +1051,14 @@ cudaError_t launch_ref_train(const RefTrainArgs& a, cudaStream_t s)
 	if (a.masks)
 	{
 		const size_t bytes = ref_train_dropout_smem_bytes(a.net);
-		cudaError_t e = cudaFuncSetAttribute(ref_train_dropout_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+		cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(ref_train_dropout_kernel));
 		if (e != cudaSuccess) return e;
 		ref_train_dropout_kernel<<<1, T, bytes, s>>>(a);
 		return cudaGetLastError();
 	}
 	if (const size_t small = ref_small_smem_bytes(a)) return launch_ref_small(a, small, s);
 	const size_t bytes = ref_train_smem_bytes(a.net, a.weights_in_smem != 0);
-	cudaError_t e = cudaFuncSetAttribute(ref_train_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(ref_train_kernel));
 	if (e != cudaSuccess) return e;
 	ref_train_kernel<<<1, T, bytes, s>>>(a);
 	return cudaGetLastError();

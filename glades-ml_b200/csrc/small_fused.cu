@@ -495,7 +495,7 @@ cudaError_t launch_small_fused(const SmallFusedArgs& a, cudaStream_t s)
 	const int sr = sf_samples(a.net);
 	const size_t bytes = sf_smem_bytes(a.net, sr);
 	const void* const kernel = small_fused_function(sr);
-	const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+	const cudaError_t e = allow_shared_memory(kernel);
 	if (e != cudaSuccess) return e;
 	int tiles = 0;
 	for (int l = 0; l <= a.net.H; ++l) tiles += (a.net.sizes[l] + 1) / 2 * sf_quads(a.net.sizes[l + 1]);
