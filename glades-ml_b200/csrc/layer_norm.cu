@@ -180,7 +180,9 @@ struct RowPlace
 //   fp32 8192 x 4096: 47 to 49 us, 5.5 to 5.7 TB/s (gain and shift in registers 54; 32 elements per lane 52)
 //   bf16 8192 x 4096: 33 us; each further 8192 rows 24, of which the copy of as many bytes takes 20.5 (one value per instruction 50;
 //                     32 elements per lane, gain and shift from L1, 36; a warp per row, or rows through shared memory, 43 to 50)
-//   bf16 10007 x 1025: 21 us (words with a branch for the halves 31; one value at a time 42)
+//   bf16 10007 x 1025: 21 us (words with a branch for the halves 31; one value at a time 42);  fp32 10007 x 1025, value by value: 37
+// The registers that three CTAs per SM leave (80) do not hold 16 values of 16 bits that are not read 16 bytes at a time: 36 to 44 bytes
+// a thread are spilled by words, 92 to 116 by values.  Nor do 128 hold 64 fp32 values: rows of 8193 to 16384 columns spill 236 to 492.
 template <class T, int MODE, int ELEMS, bool WIDE>
 __global__ void __launch_bounds__(LN_THREADS, ELEMS == 16 ? 3 : 2) norm_kernel(const LayerNormArgs p, int group)
 {
@@ -402,7 +404,9 @@ __global__ void __launch_bounds__(LN_GROUP_MAX) norm_long_kernel(const LayerNorm
 // registers; a CTA's groups are added in a fixed order and leave as one partial row, which norm_columns_kernel adds up: no atomics, two
 // runs give the same bits.  Every difference is scaled as it is taken, xh = (x - mu) r: sums of g (x - mu) and powers of r beside
 // them would leave fp32's range where activations are very large or very small.
-//   bf16 10007 x 1025: 35 us (one value at a time 164)
+//   bf16 10007 x 1025: 35 us (one value at a time 164);  fp32 10007 x 1025, value by value: 84;  bf16 30000 x 100: 19
+// A row's values, their columns' sums and the next row are more than the 128 registers of 512 threads: every instantiation of
+// norm_backward_kernel spills 128 to 344 bytes a thread.
 // A CTA's sums of the columns: its groups' are added in a fixed order in `sums`, [groups or (in-warp groups) warps][n], and leave as
 // one partial row.  A lane's access v begins at column first + v * group * VEC.
 template <bool APART, bool WIDE, int V, int PAIRS>

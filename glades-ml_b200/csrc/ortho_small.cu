@@ -1,7 +1,7 @@
 // Orthogonalisation of small matrices: one CTA per matrix, everything in its shared memory (the mathematics: orthogonalize.cu).
 // The same program on the same tensor-core operands, but no copies, no grid barriers and no symmetry: what bounds
-// a round here is the chain MMAs -> commit -> tensor-memory loads -> parts into shared memory -> block barrier, about a
-// microsecond against six of the cooperative kernel (its barrier alone takes one).
+// a round here is the chain MMAs -> commit -> tensor-memory loads -> parts into shared memory -> block barrier, 1.5
+// us against 6 of the cooperative kernel (its barrier alone takes one).
 //
 // Layout: a matrix of parts is stored in chunks of 64 columns, [chunk][hi | lo][row][64 halfs], rows of 128 bytes in the 128-byte
 // swizzle, `rows` = the short side rounded up to 16, filled with zeros.  The same bytes are a K-major operand (rows by k = columns,
