@@ -3,7 +3,7 @@ implementation: what a window leaves behind for the next pass (parts of the new 
 import numpy as np
 import pytest
 
-from test_gpu_normalised_networks import MUON, Plain, close
+from test_gpu_normalised_networks import MUON, Plain, close, data, make
 
 pytestmark = pytest.mark.gpu
 
@@ -103,4 +103,25 @@ def test_updates_and_norms_switched_between_windows(g, sizes, act, rows, engine,
     del plain.gain[norms[0]], plain.shift[norms[0]]
     window(4)
     close(net.forward(0, rows)[0], plain.forward(x), 1e-4)
+    net.close()
+
+
+@pytest.mark.parametrize("sizes,act,rows,norms,muons,tensor", [
+    ([784, 2048, 2048, 10], "tanh", 512, [1, 2], {0: (0.95, True, 0.01, 5), 1: (0.95, True, 0.01, 5), 2: (0.95, True, 0.01, 5)}, True),
+    ([784, 1000, 500, 10], "relu", 700, [1, 2], {0: MUON, 1: MUON}, False),  # fp32 tiles
+    ([1024, 4096, 1024], "tanh", 128, [1], {1: MUON}, True),
+])
+def test_window_of_wide_layers(g, sizes, act, rows, norms, muons, tensor):
+    """The benchmark networks' layers, one window and an inference pass."""
+    net, plain, rng = make(g, sizes, act, rows, 3, 0.05, g.GEMM_AUTO, norms, muons)
+    x, y = data(rng, plain, rows, sizes[0], sizes[-1])
+    net.set_data(x, y)
+    before = net.tensor_core_launches()
+    close(net.forward(0, rows)[0], plain.forward(x))
+    net.train_window(0, rows)
+    assert (net.tensor_core_launches() > before) == tensor
+    plain.window(x, y)
+    check(net, plain, muons, 1)
+    for l in norms:
+        close(net.get_norm_weights(l)[0], plain.gain[l])
     net.close()
