@@ -43,12 +43,13 @@ static_assert(OR_BM == TC_BM, "tiles");
 constexpr int OR_UNIT = 64;    // rows and columns of a piece of the elementwise phases
 constexpr int OR_SMS = 148;
 constexpr int OR_SQUARES = 2;  // p x p matrices of parts: A and R
+constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
 // An accumulator takes one stage, four additions, before it is drained.  The tensor core truncates as it adds: a sum of one sign loses
 // half a unit in the last place with every addition, and the polynomial multiplies an error that all singular values share by up to 15.
-// Against 64 bits, relative to the error of fp32 products, with 8 additions -> 4: random 512 x 4096 2.2 -> 1.3, 256 x 256 with near singular
-// values 1.5 -> 1.0.  (What is lost cannot be put back by a factor: sums that cancel, or of few products, lose less.  A factor
-// that made up for it on random matrices left diagonal and block diagonal ones 4 times further off than fp32 products.)
-constexpr int OR_SPLIT_K = 128; // k that a part of a split tile has at least
+// Against 64 bits, relative to the error of fp32 products, with 8 additions -> 4: random 256 x 1000 1.4 -> 0.8, 256 x 256 with near singular
+// values 1.6 -> 1.0, 192 x 192 with orthogonal rows 2.5 -> 1.5, for 1 to 6 % of the time.  (What is lost cannot be put back by a factor:
+// sums that cancel, or of few products, lose less.  A factor that made up for it on random matrices left diagonal and block diagonal
+// ones 4 times further off than fp32 products.)
 
 template <int BN>
 struct OrSmem
