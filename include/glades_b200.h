@@ -385,7 +385,8 @@ int gl_standardize_table(const float* d_raw, int64_t rows, int32_t cols, const i
 /* They queue their work on `stream` (a cudaStream_t of `device`; NULL: the legacy default stream) and return: no
  * synchronisation, no allocation, the current device as it was; a call can be captured into a CUDA graph.  Scratch memory is
  * the caller's: `d_work`, at least as many bytes as the operator's _workspace function says, any alignment, needs no
- * initialisation, belongs to one call (or graph replay) until that has finished.  Element types: */
+ * initialisation, belongs to one call (or graph replay) until that has finished.  Any number of host threads may call them at the
+ * same time.  Element types: */
 enum { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
 
 /* Layer norm of the rows of x [rows][n]: mean and variance (divided by n) of each row, xh = (x - mean) / sqrt(variance +
